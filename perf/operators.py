@@ -301,8 +301,10 @@ def _own(s):
     if c["op"] == "matmul":
         int8.matmul(s["x"], s["xs"], s["w"], s["ws"], s["y"], add=s["add"])
         return {"y": s["y"]}
-    cache = int8.Kv8Cache(s["k"], s["v"], s["ks"], s["vs"])
-    batch = int8.Kv8Batch(s["table"], s["cu"], s["len"], s["max_q"], s["max_kv"])
+    if "kv" not in s:  # a server describes its pages and its batch's buffers once
+        s["kv"] = int8.Kv8Cache(s["k"], s["v"], s["ks"], s["vs"])
+        s["batch"] = int8.Kv8Batch(s["table"], s["cu"], s["len"], s["max_q"], s["max_kv"])
+    cache, batch = s["kv"], s["batch"]
     if c["op"] == "append":
         int8.kv8_append(cache, batch, s["kn"], s["vn"], q=s["q"], q_out=s["q_out"], rope=s["rope"],
                         interleaved=c["interleaved"], q_norm=s["q_norm"], k_norm=s["k_norm"], eps=EPS)
