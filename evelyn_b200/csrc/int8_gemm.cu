@@ -1,0 +1,334 @@
+// int8_gemm.cu -- y[m][n] = (sum_k x[m][k] w[n][k]) * xs[m] * ws[n] (+ add[m][n]) over 8-bit
+// integers, on the 5th-generation tensor cores (tcgen05 kind::i8, exact int32 sums).
+//
+// The weight rows are the MMA's M dimension (128 TMEM lanes) and the tokens its N: a warp
+// reading one accumulator column back then holds 32 neighbouring outputs of one token, so the
+// row-major output is written in whole sectors without a transpose, and a product of few tokens
+// costs N = 16, not 128.
+//
+// One CTA works on tiles of 128 weight rows x NT tokens:
+//   warp 0     TMA producer: 128-byte K slices (128-byte swizzle) of both operands into a ring
+//              completing on mbarriers; ragged rows and a ragged K are zero-filled by TMA;
+//   warp 1     owns the tensor memory; one thread issues 4 MMAs (K = 32 each) per slice;
+//   warps 2-5  epilogue, one TMEM lane quadrant each; two accumulators, so a tile is written
+//              while the next one is multiplied.
+// With few tiles the K range is split over the CTAs of a cluster: the int32 partial tiles meet
+// through distributed shared memory, each CTA adding and writing its share of the columns, in
+// one launch, without a workspace, and exactly (integer sums).
+//
+// Bound: few tokens -- HBM, every weight byte once; many tokens -- the tensor pipe.
+// Every wait is bounded; on a timeout the CTA records DEV_ERR_WAIT_TIMEOUT, lets its copies and
+// MMAs land, frees its tensor memory and leaves.
+#include <cooperative_groups.h>
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+#include <atomic>
+
+#include "int8.cuh"
+
+namespace evl {
+namespace {
+
+constexpr uint32_t kTileN = 128;                    // weight rows per tile (TMEM lanes)
+constexpr uint32_t kSlice = 128;                    // K values (bytes) per stage: one swizzle atom
+constexpr uint32_t kThreads = 192;
+constexpr uint32_t kMaxStages = 12;
+constexpr uint32_t kSmemCap = 200 * 1024;
+
+struct Plan {
+    CUtensorMap wmap, xmap;
+    I8GemmArgs a;
+    uint32_t ntiles, mtiles;  // weight tiles, token tiles
+    uint32_t slices;          // of K
+    uint32_t split;           // CTAs (cluster) per tile
+    uint32_t stages;
+};
+
+__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int32_t x, int32_t y, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+            smem_addr(dst)),
+        "l"(map), "r"(x), "r"(y), "r"(smem_addr(bar))
+        : "memory");
+}
+// K-major operand, 128-byte swizzle: 8-row groups 1024 bytes apart
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr) {
+    return (uint64_t)((addr & 0x3FFFFu) >> 4) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// kind::i8: signed 8-bit A and B, K-major, int32 D, M = 128
+__host__ __device__ constexpr uint32_t i8_idesc(uint32_t n) {
+    return (2u << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | ((128u >> 4) << 24);
+}
+__device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_ld16(uint32_t t, uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(t)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ bool bwait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const uint64_t t0 = global_ns();
+    while (!mbar_try_wait(bar, parity)) {
+        if (*abort_flag) return false;
+        if (global_ns() - t0 > kWaitNs) {
+            *abort_flag = 1;
+            return false;
+        }
+    }
+    return true;
+}
+
+// One output: token m, weight row n.
+template <class T>
+__device__ __forceinline__ void put(const I8GemmArgs& a, uint32_t m, uint32_t n, int32_t acc, float xs, float ws) {
+    float y = __fmul_rn(__fmul_rn(__int2float_rn(acc), xs), ws);
+    if (a.add) y = __fadd_rn(y, to_f32(static_cast<const T*>(a.add)[(uint64_t)m * a.add_stride + n]));
+    static_cast<T*>(a.y)[(uint64_t)m * a.y_stride + n] = from_f32<T>(y);
+}
+
+template <uint32_t NT, class T>
+__global__ void __launch_bounds__(kThreads, 1) i8_gemm_kernel(const __grid_constant__ Plan P) {
+    namespace cg = cooperative_groups;
+    extern __shared__ uint8_t raw_smem[];
+    __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], d_full[2], d_empty[2], fin;
+    __shared__ uint32_t tmem_base;
+    __shared__ volatile int abort_flag;
+    constexpr uint32_t kStageBytes = (kTileN + NT) * kSlice;
+    constexpr uint32_t kCols = 2 * NT < 32 ? 32 : 2 * NT;  // two accumulators (a power of two)
+    const I8GemmArgs& a = P.a;
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    uint8_t* smem = raw_smem + ((1024u - (smem_addr(raw_smem) & 1023u)) & 1023u);
+    const uint32_t S = P.split, rank = blockIdx.x % S, tiles = P.ntiles * P.mtiles;
+    const uint32_t s0 = (uint32_t)((uint64_t)P.slices * rank / S), s1 = (uint32_t)((uint64_t)P.slices * (rank + 1) / S);
+
+    if (tid == 0) {
+        abort_flag = 0;
+        for (uint32_t i = 0; i < P.stages; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], 1);
+        }
+        for (uint32_t i = 0; i < 2; ++i) {
+            mbar_init(&d_full[i], 1);
+            mbar_init(&d_empty[i], 4);
+        }
+        mbar_init(&fin, 1);
+        fence_barrier_init();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_base)),
+                     "r"(kCols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_before();
+    __syncthreads();
+    tc_after();
+    const uint32_t tm = tmem_base;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t n = 0;
+            for (uint32_t tile = blockIdx.x / S; tile < tiles && !abort_flag; tile += gridDim.x / S) {
+                const int32_t w0 = (int32_t)(tile % P.ntiles * kTileN), x0 = (int32_t)(tile / P.ntiles * NT);
+                for (uint32_t c = s0; c < s1; ++c, ++n) {
+                    const uint32_t s = n % P.stages;
+                    if (n >= P.stages && !bwait(&empty[s], (n / P.stages - 1) & 1, &abort_flag)) break;
+                    uint8_t* dst = smem + s * kStageBytes;
+                    mbar_arrive_expect_tx(&full[s], kStageBytes);
+                    tma_load_2d(dst, &P.wmap, (int32_t)(c * kSlice), w0, &full[s]);
+                    tma_load_2d(dst + kTileN * kSlice, &P.xmap, (int32_t)(c * kSlice), x0, &full[s]);
+                }
+            }
+            if (abort_flag)  // copies in flight land before the CTA leaves
+                for (uint32_t s = 0; s < P.stages && s < n; ++s) mbar_wait(&full[s], ((n - 1 - s) / P.stages) & 1);
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            uint32_t n = 0, it = 0;
+            for (uint32_t tile = blockIdx.x / S; tile < tiles && !abort_flag; tile += gridDim.x / S, ++it) {
+                const uint32_t acc = tm + (it & 1) * NT;
+                if (it >= 2 && !bwait(&d_empty[it & 1], (it / 2 - 1) & 1, &abort_flag)) break;
+                tc_after();
+                for (uint32_t c = s0; c < s1; ++c, ++n) {
+                    const uint32_t s = n % P.stages;
+                    if (!bwait(&full[s], (n / P.stages) & 1, &abort_flag)) break;
+                    tc_after();
+                    const uint32_t at = smem_addr(smem + s * kStageBytes);
+                    const uint64_t da = smem_desc(at), db = smem_desc(at + kTileN * kSlice);
+#pragma unroll
+                    for (uint32_t k = 0; k < kSlice / 32; ++k)  // 32 bytes of K further inside the swizzle atom
+                        mma_i8(acc, da + 2 * k, db + 2 * k, i8_idesc(NT), c > s0 || k > 0);
+                    mma_commit(&empty[s]);
+                }
+                mma_commit(&d_full[it & 1]);
+            }
+            if (abort_flag) {  // the MMAs in flight end before the tensor memory is freed
+                mma_commit(&fin);
+                mbar_wait(&fin, 0);
+            }
+        }
+    } else {
+        const uint32_t quad = warp & 3, r = quad * 32 + lane;
+        uint32_t it = 0;
+        for (uint32_t tile = blockIdx.x / S; tile < tiles; tile += gridDim.x / S, ++it) {
+            const uint32_t n = tile % P.ntiles * kTileN + r, m0 = tile / P.ntiles * NT;
+            const bool live = n < a.out;
+            const float ws = live ? a.ws[n] : 0.f;
+            const uint32_t cols = min(NT, a.rows - m0);
+            bool ok = true;
+            if (lane == 0) ok = bwait(&d_full[it & 1], (it / 2) & 1, &abort_flag);
+            ok = __shfl_sync(0xffffffffu, (int)ok, 0);
+            if (!ok) break;
+            tc_after();
+            const uint32_t at = tm + (it & 1) * NT + ((quad * 32) << 16);
+            if (S == 1) {
+                for (uint32_t c = 0; c < cols; c += 16) {
+                    uint32_t v[16];
+                    tmem_ld16(at + c, v);
+                    tmem_ld_wait();
+                    if (live) {
+#pragma unroll
+                        for (uint32_t j = 0; j < 16; ++j)
+                            if (c + j < cols) put<T>(a, m0 + c + j, n, (int32_t)v[j], a.xs[m0 + c + j], ws);
+                    }
+                }
+            } else {  // this CTA's partial tile for the cluster, over the ring (all slices are read)
+                int32_t* part = reinterpret_cast<int32_t*>(smem);
+                for (uint32_t c = 0; c < cols; c += 16) {
+                    uint32_t v[16];
+                    tmem_ld16(at + c, v);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (uint32_t j = 0; j < 16; ++j) part[(c + j) * kTileN + r] = (int32_t)v[j];
+                }
+            }
+            tc_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&d_empty[it & 1]);
+        }
+    }
+    __syncwarp();
+    if (S > 1) {
+        cg::cluster_group cl = cg::this_cluster();
+        cl.sync();
+        const uint32_t tile = blockIdx.x / S, n0 = tile % P.ntiles * kTileN, m0 = tile / P.ntiles * NT;
+        const uint32_t cols = min(NT, a.rows - m0);
+        const int32_t* part = reinterpret_cast<const int32_t*>(smem);
+        for (uint32_t i = rank * kThreads + tid; i < cols * kTileN && !abort_flag; i += S * kThreads) {
+            int32_t acc = 0;
+            for (uint32_t k = 0; k < S; ++k) acc += *cl.map_shared_rank(part + i, k);
+            const uint32_t m = m0 + i / kTileN, n = n0 + i % kTileN;
+            if (n < a.out) put<T>(a, m, n, acc, a.xs[m], a.ws[n]);
+        }
+        cl.sync();  // the others read this CTA's tile until here
+    }
+    tc_before();
+    __syncthreads();
+    if (tid == 0 && abort_flag) flag_error(a.err, DEV_ERR_WAIT_TIMEOUT);
+    if (warp == 1)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "r"(kCols) : "memory");
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encoder() {
+    static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+    }();
+    return fn;
+}
+
+// [rows][cols] bytes, rows `stride` apart, read in boxes of box_rows x 128 bytes; outside: zeros
+bool make_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t stride, uint32_t box_rows) {
+    const cuuint64_t dims[2] = {cols, rows};
+    const cuuint64_t strides[1] = {stride};
+    const cuuint32_t box[2] = {kSlice, box_rows}, unit[2] = {1, 1};
+    return encoder() && encoder()(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, unit,
+                                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <uint32_t NT, class T> cudaError_t launch(Plan& p, int sms, cudaStream_t s) {
+    const I8GemmArgs& a = p.a;
+    constexpr uint32_t stage = (kTileN + NT) * kSlice;
+    if (!make_map(&p.wmap, a.w, a.out, a.cols, a.w_stride, kTileN) ||
+        !make_map(&p.xmap, a.x, a.rows, a.cols, a.x_stride, NT))
+        return cudaErrorInvalidValue;
+    p.ntiles = (a.out + kTileN - 1) / kTileN;
+    p.mtiles = (a.rows + NT - 1) / NT;
+    p.slices = (a.cols + kSlice - 1) / kSlice;
+    p.stages = std::min(kMaxStages, kSmemCap / stage);
+    const uint64_t tiles = (uint64_t)p.ntiles * p.mtiles;
+    if (tiles > 0x7fffffffull) return cudaErrorInvalidValue;
+    // split K while the tiles leave SMs free and every CTA keeps a few slices
+    p.split = 1;
+    while (p.split < 8 && tiles * p.split * 2 <= (uint64_t)sms && p.slices >= 4 * p.split) p.split *= 2;
+    // a cluster's partial tile lies over the ring
+    const uint32_t smem = std::max(p.stages * stage, p.split > 1 ? NT * kTileN * 4 : 0u) + 1024;
+    static std::atomic<bool> opted[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    if (!opted[dev].load()) {
+        e = cudaFuncSetAttribute(i8_gemm_kernel<NT, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemCap + 1024);
+        if (e != cudaSuccess) return e;
+        opted[dev] = true;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(p.split > 1 ? (uint32_t)tiles * p.split : (uint32_t)std::min<uint64_t>(tiles, sms));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = p.split;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, i8_gemm_kernel<NT, T>, p);
+}
+
+template <class T> cudaError_t by_tokens(Plan& p, int sms, cudaStream_t s) {
+    if (p.a.rows <= 16) return launch<16, T>(p, sms, s);
+    if (p.a.rows <= 32) return launch<32, T>(p, sms, s);
+    if (p.a.rows <= 64) return launch<64, T>(p, sms, s);
+    if (p.a.rows <= 128) return launch<128, T>(p, sms, s);
+    return launch<256, T>(p, sms, s);
+}
+
+}  // namespace
+
+cudaError_t launch_i8_gemm(const I8GemmArgs& a, int sms, cudaStream_t s) {
+    Plan p;
+    p.a = a;
+    switch (a.type) {
+        case GGML_F32: return by_tokens<float>(p, sms, s);
+        case GGML_F16: return by_tokens<__half>(p, sms, s);
+        case GGML_BF16: return by_tokens<__nv_bfloat16>(p, sms, s);
+        default: return cudaErrorInvalidValue;
+    }
+}
+
+}  // namespace evl

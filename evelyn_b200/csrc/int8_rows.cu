@@ -1,0 +1,121 @@
+// int8_rows.cu -- activation rows in 8 bits with one scale each, the left operand of the
+// integer product (int8_gemm.cu):
+//   a = max |x|, scale = a / 127, code = rint(x * (1 / scale)).
+// The row is read once into registers, its largest magnitude found as an integer maximum of
+// the absolute bits (which also finds an infinity or a NaN), and the codes written: input
+// bytes + one byte per value is all the traffic, so the kernel is bound by HBM. f32 throughout;
+// the products and the reciprocal are each rounded once, so the codes do not depend on the
+// launch shape.
+#include "int8.cuh"
+
+namespace evl {
+namespace {
+
+constexpr uint32_t kChunk = 8;  // values a thread loads together: one or two 16-byte loads, one 8-byte store
+
+__device__ __forceinline__ uint32_t block_umax(uint32_t v, uint32_t* red) {
+    v = __reduce_max_sync(0xffffffffu, v);
+    const uint32_t warps = blockDim.x >> 5;
+    if (warps == 1) return v;
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+    __syncthreads();
+    const uint32_t lane = threadIdx.x & 31;
+    return __reduce_max_sync(0xffffffffu, lane < warps ? red[lane] : 0u);
+}
+
+// One CTA per row, C chunks per thread in registers.
+template <class T, int C> __global__ void __launch_bounds__(1024) quantize_rows_kernel(const QuantRowsArgs a) {
+    __shared__ uint32_t red[32];
+    const uint64_t row = blockIdx.x;
+    const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
+    int8_t* codes = a.codes + row * a.code_stride;
+    const uint32_t chunks = a.cols / kChunk, tail = a.cols % kChunk, nt = blockDim.x;
+    float v[C][kChunk];
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+        const uint32_t c = threadIdx.x + i * nt;
+        if (c < chunks) {
+            load8(x + (uint64_t)c * kChunk, v[i]);
+        } else {
+            const uint32_t left = c == chunks ? tail : 0;
+#pragma unroll
+            for (uint32_t j = 0; j < kChunk; ++j) v[i][j] = j < left ? to_f32(x[(uint64_t)c * kChunk + j]) : 0.f;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < C; ++i)
+#pragma unroll
+        for (uint32_t j = 0; j < kChunk; ++j) m = max(m, abs_bits(v[i][j]));
+    m = block_umax(m, red);
+    const float scale = scale_of(m), inv = inverse_of(scale);
+    if (threadIdx.x == 0) a.scales[row] = scale;
+    const bool live = scale > 0.f;
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+        const uint32_t c = threadIdx.x + i * nt;
+        uint32_t q[kChunk];
+#pragma unroll
+        for (uint32_t j = 0; j < kChunk; ++j) q[j] = live ? code_bits(v[i][j], inv) : 0u;
+        if (c < chunks) {
+            *reinterpret_cast<uint2*>(codes + (uint64_t)c * kChunk) =
+                make_uint2(pack4(q[0], q[1], q[2], q[3]), pack4(q[4], q[5], q[6], q[7]));
+        } else if (c == chunks) {
+#pragma unroll
+            for (uint32_t j = 0; j < kChunk; ++j)
+                if (j < tail) codes[(uint64_t)c * kChunk + j] = (int8_t)q[j];
+        }
+    }
+}
+
+// Rows that do not start on the boundaries of wide loads (an odd row length, a view), and rows
+// too long for registers: values one by one, neighbouring threads on neighbouring values, the
+// row read a second time from L2.
+template <class T> __global__ void __launch_bounds__(512) quantize_rows_plain_kernel(const QuantRowsArgs a) {
+    __shared__ uint32_t red[32];
+    const uint64_t row = blockIdx.x;
+    const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
+    int8_t* codes = a.codes + row * a.code_stride;
+    uint32_t m = 0;
+#pragma unroll 8
+    for (uint32_t c = threadIdx.x; c < a.cols; c += blockDim.x) m = max(m, abs_bits(to_f32(x[c])));
+    m = block_umax(m, red);
+    const float scale = scale_of(m), inv = inverse_of(scale);
+    if (threadIdx.x == 0) a.scales[row] = scale;
+    const bool live = scale > 0.f;
+#pragma unroll 8
+    for (uint32_t c = threadIdx.x; c < a.cols; c += blockDim.x)
+        codes[c] = live ? (int8_t)code_bits(to_f32(x[c]), inv) : (int8_t)0;
+}
+
+template <class T> cudaError_t launch(const QuantRowsArgs& a, int sms, cudaStream_t s) {
+    const bool aligned = (reinterpret_cast<uintptr_t>(a.x) & 15) == 0 && (a.x_stride * sizeof(T)) % 16 == 0 &&
+                         (reinterpret_cast<uintptr_t>(a.codes) & 7) == 0 && a.code_stride % 8 == 0;
+    const uint32_t chunks = (a.cols + kChunk - 1) / kChunk;
+    if (!aligned || chunks > 4 * 1024) {
+        const uint32_t nt = a.cols >= 4096 ? 512 : a.cols >= 512 ? 128 : 32;
+        quantize_rows_plain_kernel<T><<<a.rows, nt, 0, s>>>(a);
+        return cudaGetLastError();
+    }
+    // few rows: as many threads as chunks, so that a row is one load deep; many rows: four
+    // chunks per thread, all in flight, and more rows on each SM
+    const int C = (a.rows <= (uint32_t)(2 * sms) && chunks <= 1024) ? 1 : chunks > 2048 || a.rows > (uint32_t)(2 * sms) ? 4 : 2;
+    const uint32_t nt = ((chunks + C - 1) / C + 31) / 32 * 32;
+    if (C == 1) quantize_rows_kernel<T, 1><<<a.rows, nt, 0, s>>>(a);
+    else if (C == 2) quantize_rows_kernel<T, 2><<<a.rows, nt, 0, s>>>(a);
+    else quantize_rows_kernel<T, 4><<<a.rows, nt, 0, s>>>(a);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_quantize_rows(const QuantRowsArgs& a, int sms, cudaStream_t s) {
+    switch (a.type) {
+        case GGML_F32: return launch<float>(a, sms, s);
+        case GGML_F16: return launch<__half>(a, sms, s);
+        case GGML_BF16: return launch<__nv_bfloat16>(a, sms, s);
+        default: return cudaErrorInvalidValue;
+    }
+}
+
+}  // namespace evl

@@ -83,6 +83,25 @@ class _TpShard(C.Structure):
                 ("vocab_rows", C.c_uint64 * 2)]
 
 
+class _Kv8Cache(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32), ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32),
+                ("page_size", C.c_uint32), ("n_pages", C.c_uint32), ("reserved", C.c_uint32),
+                ("d_k", C.c_void_p), ("d_v", C.c_void_p), ("d_k_scales", C.c_void_p), ("d_v_scales", C.c_void_p),
+                ("page_stride", C.c_uint64), ("scale_stride", C.c_uint64)]
+
+
+class _Kv8Batch(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32), ("n_seqs", C.c_uint32), ("total", C.c_uint32), ("max_new", C.c_uint32),
+                ("max_len", C.c_uint32), ("table_stride", C.c_uint32), ("d_page_table", C.c_void_p),
+                ("d_cu", C.c_void_p), ("d_len", C.c_void_p)]
+
+
+class _Kv8Prep(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32), ("rope_dim", C.c_uint32), ("rope_interleaved", C.c_uint32),
+                ("rope_len", C.c_uint32), ("d_rope", C.c_void_p), ("d_q_norm", C.c_void_p), ("d_k_norm", C.c_void_p),
+                ("eps", C.c_float), ("reserved", C.c_uint32)]
+
+
 @dataclasses.dataclass(frozen=True)
 class Config:
     """runtime.rs:93-110 (dense-attention fields)."""
@@ -158,6 +177,15 @@ SIGNATURES = {
                                           C.c_uint32, _P, _P, C.c_size_t, _P]),
     "evl_attention_decode_noalloc": (C.c_int, [_P, _P, _P, _P, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32,
                                                C.c_uint32, _P, _P]),
+    "evl_i8_quantize_rows": (C.c_int, [C.c_uint32, _P, C.c_uint64, C.c_uint32, C.c_uint32, _P, C.c_uint64, _P, _P]),
+    "evl_i8_matmul": (C.c_int, [_P, C.c_uint64, _P, C.c_uint32, _P, C.c_uint64, _P, C.c_uint32, C.c_uint32, C.c_uint32,
+                                _P, C.c_uint64, _P, C.c_uint64, _P, _P]),
+    "evl_kv8_append": (C.c_int, [C.POINTER(_Kv8Cache), C.POINTER(_Kv8Batch), C.POINTER(_Kv8Prep), C.c_uint32, _P,
+                                 C.c_uint64, _P, C.c_uint64, _P, C.c_uint64, C.c_uint32, _P, C.c_uint64, _P, _P]),
+    "evl_kv8_attention_workspace_bytes": (C.c_int, [C.POINTER(_Kv8Cache), C.POINTER(_Kv8Batch), C.c_uint32,
+                                                    C.POINTER(C.c_size_t)]),
+    "evl_kv8_attention": (C.c_int, [C.POINTER(_Kv8Cache), C.POINTER(_Kv8Batch), C.c_uint32, _P, C.c_uint64, C.c_uint32,
+                                    C.c_float, _P, C.c_uint64, _P, C.c_size_t, _P, _P]),
     "evl_remote_ffn_new": (C.c_int, [_P, C.c_size_t, C.POINTER(C.c_size_t), C.POINTER(C.c_char_p), C.c_uint32,
                                      C.POINTER(_P)]),
     "evl_remote_ffn_free": (None, [_P]),

@@ -258,6 +258,121 @@ evl_status evl_attention_decode_noalloc(const float* d_q, const void* d_k_pages,
                                         const int32_t* d_page_table, uint32_t t, uint32_t heads, uint32_t kv_heads,
                                         uint32_t head_dim, uint32_t page_size, float* d_out, void* stream);
 
+/* ------------------------------------------------------------------ 8-bit serving operators */
+/* The 8-bit half of a layer on caller buffers, for any number of tokens and sequences (no
+ * counterpart in the reference, whose activations and KV cache are f32): activation rows
+ * and the integer product, and a paged KV cache in 8 bits.
+ *
+ * Common rules. All d_ pointers are device memory; the call runs on the device that holds
+ * its first one (the calling thread's current device is left as it was) and is asynchronous
+ * on `stream` (a stream of that device; NULL: its default stream), so it can be captured
+ * into a graph. No call allocates device memory or keeps anything. `type` is the element
+ * type of the activations: 0 F32, 1 F16, 30 BF16. Arithmetic is f32 (integer sums exact),
+ * rounded once to the output type.
+ * A group of values in 8 bits is codes c in [-127, 127] and one f32 scale s, value s * c:
+ * s = max|x| / 127, c = x * (1 / s) rounded to nearest even. A group whose largest magnitude
+ * is below 2^-100 has s = 0 and codes 0; one that holds an infinity or a NaN has s = NaN and
+ * codes 0.
+ * d_err (optional, one int32 that the caller clears) receives 3 where device-side data names
+ * a position, token or page outside what the arguments describe -- that sequence (for a page:
+ * that block) is then skipped, its outputs left as they were or, for attention, computed
+ * without the block -- and 2 if a bounded device wait gave up. */
+
+/* Rows of activations to 8 bits, one scale per row: d_x [rows][cols], rows x_stride elements
+ * apart, to d_codes, rows code_stride bytes apart, and d_scales [rows]. Only [rows][cols]
+ * codes are written. rows may be 0. Fastest where rows of d_x start on 16-byte and rows of
+ * d_codes on 8-byte boundaries. */
+evl_status evl_i8_quantize_rows(uint32_t type, const void* d_x, uint64_t x_stride, uint32_t rows, uint32_t cols,
+                                int8_t* d_codes, uint64_t code_stride, float* d_scales, void* stream);
+/* Product of 8-bit matrices with a scale per token and per channel, on the tensor cores:
+ *   y[m][n] = (sum_k x[m][k] w[n][k]) * x_scales[m] * w_scales[n] (+ add[m][n])
+ * x [rows][cols] and w [out][cols] int8 with rows x_stride / w_stride bytes apart (multiples
+ * of 16, the buffers 16-byte aligned; what lies between cols and the stride is not read into
+ * the sums); d_add (optional) and d_y of `type`, rows add_stride / y_stride elements apart.
+ * d_add may be d_y (a residual added in place) but no other overlap with d_y is allowed.
+ * cols from 1 to 131071 (the int32 sums then cannot overflow); rows or out may be 0. */
+evl_status evl_i8_matmul(const int8_t* d_x, uint64_t x_stride, const float* d_x_scales, uint32_t rows,
+                         const int8_t* d_w, uint64_t w_stride, const float* d_w_scales, uint32_t out, uint32_t cols,
+                         uint32_t type, const void* d_add, uint64_t add_stride, void* d_y, uint64_t y_stride,
+                         int32_t* d_err, void* stream);
+
+/* A paged KV cache in 8 bits, one scale per block of 16 positions and kv head:
+ *   codes of page p, head h, row r:  d_k + p * page_stride + (h * page_size + r) * head_dim
+ *   its scale:  d_k_scales[p * scale_stride + h * (page_size / 16) + r / 16]
+ * and the same for d_v. head_dim 64, 128 or 256; page_size 16, 32 or 64; page_stride (bytes)
+ * a multiple of 16, the code buffers 16-byte aligned. A block's first append sets its codes
+ * and scale, so pages need no initial value. */
+typedef struct evl_kv8_cache {
+    uint32_t struct_size; /* sizeof(evl_kv8_cache) */
+    uint32_t kv_heads, head_dim, page_size, n_pages, reserved;
+    int8_t* d_k;
+    int8_t* d_v;
+    float* d_k_scales;
+    float* d_v_scales;
+    uint64_t page_stride;  /* bytes */
+    uint64_t scale_stride; /* floats */
+} evl_kv8_cache;
+
+/* The sequences of a call: sequence s has the new tokens [cu[s], cu[s+1]) of `total`, and
+ * len[s] positions once they are appended, so token i of it stands at position
+ * len[s] - (cu[s+1] - cu[s]) + i. d_cu [n_seqs + 1] does not decrease; a sequence may have no
+ * new token. max_new and max_len bound the tokens and lengths (they size the launch; a larger
+ * device value is an error 3). d_page_table [n_seqs][table_stride]: the page of positions
+ * [j * page_size, (j + 1) * page_size) at j; entries past a sequence's length are not read. */
+typedef struct evl_kv8_batch {
+    uint32_t struct_size; /* sizeof(evl_kv8_batch) */
+    uint32_t n_seqs, total, max_new, max_len, table_stride;
+    const int32_t* d_page_table;
+    const int32_t* d_cu;
+    const int32_t* d_len;
+} evl_kv8_batch;
+
+/* How queries and keys are made ready: an RMS norm per head (weights [head_dim] f32, optional),
+ * then the rotation of the first rope_dim dimensions by row `position` of d_rope
+ * [rope_len][rope_dim / 2][2] f32 (cos, sin; optional), pairs (i, i + rope_dim / 2) or, with
+ * rope_interleaved, (2i, 2i + 1). rope_dim: a multiple of 4, at most head_dim; d_rope 16-byte
+ * aligned. The norm's sum and root are computed in 64 bits and rounded once. */
+typedef struct evl_kv8_prep {
+    uint32_t struct_size; /* sizeof(evl_kv8_prep) */
+    uint32_t rope_dim, rope_interleaved, rope_len;
+    const float* d_rope;
+    const float* d_q_norm;
+    const float* d_k_norm;
+    float eps;
+    uint32_t reserved;
+} evl_kv8_prep;
+
+/* Appends the batch's new keys and values (d_k, d_v [total][kv_heads][head_dim] of `type`,
+ * tokens k_stride / v_stride elements apart) to the cache, keys made ready by `prep` (NULL: as
+ * they are), and makes the queries ready on the way: d_q [total][heads][head_dim], tokens
+ * q_stride apart, to d_q_out (d_q NULL: none; d_q_out may be d_q with the same stride). A block's
+ * scale is the largest of its values / 127 since its first position was written: when new
+ * tokens raise it, the codes of the block's earlier positions move to the new scale,
+ * rint(c * (s_old / s_new)). Rows of the block behind the sequence's last token are left as
+ * they were. No two sequences of a call may write to the same block. Appending again at
+ * positions already written (a rewound sequence) replaces them; the block keeps its scale
+ * unless its first position is among them. d_k, d_v, d_q, d_q_out 16-byte aligned, strides
+ * multiples of 16 bytes. */
+evl_status evl_kv8_append(const evl_kv8_cache* cache, const evl_kv8_batch* batch, const evl_kv8_prep* prep,
+                          uint32_t type, const void* d_k, uint64_t k_stride, const void* d_v, uint64_t v_stride,
+                          const void* d_q, uint64_t q_stride, uint32_t heads, void* d_q_out, uint64_t q_out_stride,
+                          int32_t* d_err, void* stream);
+/* Device workspace of evl_kv8_attention for this cache, batch bounds (n_seqs, max_new,
+ * max_len) and number of heads, on the current device; it may be 0. Host only. */
+evl_status evl_kv8_attention_workspace_bytes(const evl_kv8_cache* cache, const evl_kv8_batch* batch, uint32_t heads,
+                                             size_t* bytes);
+/* Attention of the batch's new tokens (appended before) over the cache: row (token, head)
+ * attends the positions up to its own with softmax(scale * q . k), query head h reading kv
+ * head h / (heads / kv_heads). d_q and d_out [total][heads][head_dim] of `type`, tokens q_stride /
+ * out_stride elements apart, 16-byte aligned, strides multiples of 16 bytes. heads a multiple of
+ * kv_heads. scale 0: 1 / sqrt(head_dim). A row that sees no position gives zeros; a query row that
+ * holds an infinity or a NaN gives NaN. Rows of d_out that belong to no sequence are left as they
+ * were. d_workspace: evl_kv8_attention_workspace_bytes, 256-byte aligned, needing no initial
+ * value; calls that may overlap in time need one each. */
+evl_status evl_kv8_attention(const evl_kv8_cache* cache, const evl_kv8_batch* batch, uint32_t type, const void* d_q,
+                             uint64_t q_stride, uint32_t heads, float scale, void* d_out, uint64_t out_stride,
+                             void* d_workspace, size_t workspace_bytes, int32_t* d_err, void* stream);
+
 /* ------------------------------------------------------------------ AARNN routing (src/remote.rs) */
 typedef struct evl_endpoint_stats { /* EndpointStats, remote.rs:13-24 */
     uint64_t calls, failures, retries;
