@@ -78,7 +78,7 @@ struct Kv8AttnArgs {
     uint8_t* ws = nullptr;
     int32_t* err = nullptr;
 };
-uint64_t kv8_attention_ws_bytes(const Kv8Cache& c, const Kv8Batch& b, uint32_t heads, int sms);
+uint64_t kv8_attention_ws_bytes(const Kv8Cache& c, const Kv8Batch& b, uint32_t heads, uint32_t type, int sms);
 cudaError_t launch_kv8_attention(const Kv8AttnArgs& a, int sms, cudaStream_t s);
 
 }  // namespace evl

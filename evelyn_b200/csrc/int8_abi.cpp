@@ -260,16 +260,17 @@ evl_status evl_kv8_append(const evl_kv8_cache* cache, const evl_kv8_batch* batch
     });
 }
 
-evl_status evl_kv8_attention_workspace_bytes(const evl_kv8_cache* cache, const evl_kv8_batch* batch, uint32_t heads,
-                                             size_t* bytes) {
+evl_status evl_kv8_attention_workspace_bytes(const evl_kv8_cache* cache, const evl_kv8_batch* batch, uint32_t type,
+                                             uint32_t heads, size_t* bytes) {
     return guarded([&] {
         require(bytes, "null argument");
+        elem_bytes(type);
         const Kv8Cache c = cache_of(cache);
         const Kv8Batch b = batch_of(batch);
         require(heads >= 1 && heads % c.kv_heads == 0, "heads must be a multiple of kv_heads");
         int dev = 0;
         cuda_check(cudaGetDevice(&dev), "cudaGetDevice");
-        *bytes = (size_t)kv8_attention_ws_bytes(c, b, heads, sm_count(dev));
+        *bytes = (size_t)kv8_attention_ws_bytes(c, b, heads, type, sm_count(dev));
     });
 }
 
@@ -292,7 +293,7 @@ evl_status evl_kv8_attention(const evl_kv8_cache* cache, const evl_kv8_batch* ba
         require(aligned(d_err, 4), "d_err must be 4-byte aligned");
         OnDeviceOf on(d_q);
         const int sms = sm_count(on.dev);
-        const uint64_t need = kv8_attention_ws_bytes(a.c, a.b, heads, sms);
+        const uint64_t need = kv8_attention_ws_bytes(a.c, a.b, heads, type, sms);
         if (need) {
             require(d_workspace && aligned(d_workspace, 256), "workspace must be 256-byte aligned");
             require(workspace_bytes >= need, "workspace too small; size it with evl_kv8_attention_workspace_bytes");

@@ -26,6 +26,7 @@
 // chunk leaves (O, M, l) in the workspace for kv8_join_kernel.
 // Bound: HBM, (2 head_dim + 1/2) bytes per position and kv head.
 #include <algorithm>
+#include <atomic>
 
 #include "int8.cuh"
 
@@ -43,7 +44,8 @@ struct Plan {
     uint32_t row_tiles;  // per (sequence, kv head)
     uint32_t chunk;      // blocks of 16 positions per split
     uint32_t splits;
-    float* part_o;       // [sequence][kv head][row tile][split][kRows][head_dim]
+    uint32_t tile_rows;  // rows of a tile: kRows, or those of the prompt kernel
+    float* part_o;       // [sequence][kv head][row tile][split][tile_rows][head_dim]
     float2* part_ml;     // same without head_dim: (M, l)
 };
 
@@ -376,13 +378,13 @@ template <class T, int HD> __global__ void __launch_bounds__(128) kv8_join_kerne
     const int32_t i = (int32_t)(blockIdx.x * 4 + (threadIdx.x >> 5));
     const Span sp = span_of(a, s);
     if (!sp.ok || i >= sp.n_new) return;
-    const uint32_t h = head / P.group, row = (uint32_t)i * P.group + head % P.group, tile = row / kRows;
+    const uint32_t h = head / P.group, row = (uint32_t)i * P.group + head % P.group, tile = row / P.tile_rows;
     const int32_t rows = sp.n_new * (int32_t)P.group;
-    const int32_t seen = sp.base + (min((int32_t)((tile + 1) * kRows), rows) - 1) / (int32_t)P.group + 1;
+    const int32_t seen = sp.base + (min((int32_t)((tile + 1) * P.tile_rows), rows) - 1) / (int32_t)P.group + 1;
     const uint32_t n = seen > 0 ? ((uint32_t)(seen + 15) / 16 + P.chunk - 1) / P.chunk : 1;
     const uint64_t at = (((uint64_t)s * a.c.kv_heads + h) * P.row_tiles + tile) * P.splits;
     float m = kNegBig;
-    for (uint32_t k = lane; k < n; k += 32) m = fmaxf(m, P.part_ml[(at + k) * kRows + row % kRows].x);
+    for (uint32_t k = lane; k < n; k += 32) m = fmaxf(m, P.part_ml[(at + k) * P.tile_rows + row % P.tile_rows].x);
     m = warp_max(m);
     constexpr int N = HD / 64;
     float v[N][2], sum = 0.f;
@@ -390,7 +392,7 @@ template <class T, int HD> __global__ void __launch_bounds__(128) kv8_join_kerne
     for (int c = 0; c < N; ++c) v[c][0] = v[c][1] = 0.f;
 #pragma unroll 4
     for (uint32_t k = 0; k < n; ++k) {
-        const uint64_t p = (at + k) * kRows + row % kRows;
+        const uint64_t p = (at + k) * P.tile_rows + row % P.tile_rows;
         const float2 ml = P.part_ml[p];
         const float f = exp2_fast(ml.x - m);
         sum = fmaf(ml.y, f, sum);
@@ -407,57 +409,556 @@ template <class T, int HD> __global__ void __launch_bounds__(128) kv8_join_kerne
     for (int c = 0; c < N; ++c) store2(out + 64 * c + 2 * lane, v[c][0] * inv, v[c][1] * inv);
 }
 
+// ------------------------------------------------------------------ prompts
+// kv8_tile_kernel: many rows per kv head, on the 5th-generation tensor cores. A CTA takes RT row
+// tiles of 128 rows (token, head) of one (sequence, kv head) and walks the positions NP at a time:
+//   4 producer warps  codes to f16 (exact) into a ring of shared-memory stages, K and V alike:
+//                     64 dims x NP positions per 128-byte-swizzled panel. The score product reads
+//                     them K-major, the value product MN-major, so no transpose is made;
+//   1 MMA thread      S = q K^T into tensor memory (two buffers per row tile, so the next scores
+//                     are multiplied while this step's softmax runs), O += P V with P read
+//                     from tensor memory;
+//   4 softmax warps   per row tile, one row per thread: scores to registers, running maximum,
+//                     weights to f16 over the scores' own columns. O is rescaled (read, multiplied,
+//                     written back) only when a score passes the row's maximum by 2^8.
+// q is scaled by a power of two per row and held in one f16 part (16-bit inputs: exact) or two
+// (f32 inputs, TERMS = 2; then P is also two parts, two products each). The block scales enter as
+// in the kernel above; the value scale as an added log2 where one rounding of the weights follows
+// anyway (TERMS = 1).
+// Bound: the exponentials (16 a clock and SM) and the tensor pipe, about equally.
+constexpr uint32_t kTileRows = 128;
+constexpr uint32_t kTileMin = 48;  // rows per (sequence, kv head) from which it is used
+
+struct Role {  // per (HD, TERMS)
+    uint32_t rt, np, stages;
+};
+__host__ __device__ constexpr Role role_of(int hd, int terms) {
+    return hd == 256 ? (terms == 2 ? Role{1, 32, 2} : Role{1, 64, 2}) : terms == 2 ? Role{1, 64, 3} : Role{2, 64, 3};
+}
+__host__ __device__ constexpr uint32_t tile_smem(int hd, int terms) {
+    return role_of(hd, terms).rt * terms * kTileRows * hd * 2 +
+           role_of(hd, terms).stages * (2 * role_of(hd, terms).np * hd * 2) + 1024;
+}
+
+__device__ __forceinline__ bool bwait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const uint64_t t0 = global_ns();
+    while (!mbar_try_wait(bar, parity)) {
+        if (*abort_flag) return false;
+        if (global_ns() - t0 > kWaitNs) {
+            *abort_flag = 1;
+            return false;
+        }
+    }
+    return true;
+}
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
+                 : "memory");
+}
+// shared-memory operand, 128-byte swizzle. lbo: bytes between 64-element panels (MN-major), sbo: between 8-row groups
+__device__ __forceinline__ uint64_t swizzled_desc(uint32_t addr, uint32_t lbo) {
+    return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           (1ull << 46) | (2ull << 61);
+}
+__host__ __device__ constexpr uint32_t f16_idesc(uint32_t n, bool b_mn_major) {
+    return (1u << 4) | ((b_mn_major ? 1u : 0u) << 16) | ((n >> 3) << 17) | ((kTileRows >> 4) << 24);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t t, uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
+          "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
+          "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(t)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t t, const uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(t),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
+        "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
+        "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t t, const uint32_t* v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(t), "r"(v[0]), "r"(v[1]),
+                 "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// byte offset of 16-byte piece `p` (8 f16 values) of row r in panels of `rows` rows
+__device__ __forceinline__ uint32_t panel_at(uint32_t rows, uint32_t r, uint32_t p) {
+    return (p >> 3) * (rows * 128u) + r * 128u + (((p & 7u) ^ (r & 7u)) << 4);
+}
+// 16 codes to f16, two 16-byte pieces
+__device__ __forceinline__ void codes_to_panel(uint8_t* panel, uint32_t rows, uint32_t r, uint32_t c, uint4 w, bool zero) {
+    uint32_t h[8];
+    const uint32_t in[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t b = zero ? 0x80808080u : in[i] ^ 0x80808080u;
+        h[2 * i] = codes_h2(b, 0x4140);
+        h[2 * i + 1] = codes_h2(b, 0x4342);
+    }
+    *reinterpret_cast<uint4*>(panel + panel_at(rows, r, 2 * c)) = make_uint4(h[0], h[1], h[2], h[3]);
+    *reinterpret_cast<uint4*>(panel + panel_at(rows, r, 2 * c + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
+}
+
+template <class T, int HD>
+__global__ void __launch_bounds__(32 * (4 * role_of(HD, sizeof(T) == 4 ? 2 : 1).rt + 5), 1)
+    kv8_tile_kernel(const __grid_constant__ Plan P) {
+    constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
+    constexpr Role R = role_of(HD, TERMS);
+    constexpr uint32_t RT = R.rt, NP = R.np, ST = R.stages, NB = NP / 16;
+    constexpr uint32_t kQPart = kTileRows * HD * 2;   // one f16 part of a row tile's q
+    constexpr uint32_t kKv = NP * HD * 2;             // K (or V) of a stage
+    constexpr uint32_t kSoftWarps = 4 * RT, kTileCols = RT == 2 ? 256 : 512;  // tensor memory columns per row tile
+    extern __shared__ uint8_t raw_smem[];
+    __shared__ __align__(8) uint64_t kv_full[ST], kv_empty[ST], s_full[RT][2], p_full[RT], o_done[RT], q_full, fin;
+    __shared__ float f_sk[ST][NB], f_e[ST][NB], f_down[ST][NB], f_mant[ST][NB];
+    __shared__ uint32_t tmem_base;
+    __shared__ volatile int abort_flag;
+    const Kv8AttnArgs& a = P.a;
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    // the last row tiles see the most positions: they go first
+    const uint32_t tile = P.row_tiles - 1 - blockIdx.x / P.splits, split = blockIdx.x % P.splits, h = blockIdx.y, s = blockIdx.z;
+    const Span sp = span_of(a, s);
+    if (!sp.ok) {
+        if (tid == 0) flag_error(a.err, DEV_ERR_POSITION);
+        return;
+    }
+    const int32_t rows = sp.n_new * (int32_t)P.group, r0 = (int32_t)(tile * (RT * kTileRows));
+    if (r0 >= rows) return;
+    const int32_t nrow = min((int32_t)(RT * kTileRows), rows - r0);
+    const int32_t seen = sp.base + (r0 + nrow - 1) / (int32_t)P.group + 1;
+    const int32_t nblk = seen > 0 ? (seen + 15) / 16 : 0;
+    const int32_t b0 = (int32_t)(split * P.chunk), b1 = min(nblk, b0 + (int32_t)P.chunk);
+    if (b0 >= nblk && split > 0) return;
+    const uint32_t steps = b1 > b0 ? (uint32_t)(b1 - b0 + (int32_t)NB - 1) / NB : 0;
+
+    uint8_t* smem = raw_smem + ((1024u - (smem_addr(raw_smem) & 1023u)) & 1023u);
+    uint8_t* sq = smem;                                  // [RT][TERMS] q panels
+    uint8_t* skv = smem + RT * TERMS * kQPart;           // [ST][K | V]
+    if (tid == 0) {
+        abort_flag = 0;
+        for (uint32_t i = 0; i < ST; ++i) {
+            mbar_init(&kv_full[i], 4);
+            mbar_init(&kv_empty[i], 1);
+        }
+        for (uint32_t i = 0; i < RT; ++i) {
+            mbar_init(&s_full[i][0], 1);
+            mbar_init(&s_full[i][1], 1);
+            mbar_init(&p_full[i], 4);
+            mbar_init(&o_done[i], 1);
+        }
+        mbar_init(&q_full, kSoftWarps);
+        mbar_init(&fin, 1);
+        fence_barrier_init();
+    }
+    if (warp == kSoftWarps + 4) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_base)),
+                     "r"(512)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_before();
+    __syncthreads();
+    tc_after();
+    const uint32_t tm = tmem_base;
+
+    if (warp < kSoftWarps) {
+        // ---------------------------------------------------------------- softmax: one row per thread
+        const uint32_t rt = warp >> 2, quad = warp & 3, lr = quad * 32 + lane;
+        const int32_t row = r0 + (int32_t)(rt * kTileRows + lr);
+        const bool live = row < rows;
+        const int32_t row_c = min(row, rows - 1), tok = row_c / (int32_t)P.group;
+        const uint32_t head = h * P.group + (uint32_t)(row_c % (int32_t)P.group);
+        float step;
+        {
+            const T* q = static_cast<const T*>(a.q) + (uint64_t)(sp.q0 + tok) * a.q_stride + (uint64_t)head * HD;
+            uint32_t m = 0;
+#pragma unroll 4
+            for (int d = 0; d < HD; d += 8) {
+                float v[8];
+                load8(q + d, v);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) m = max(m, abs_bits(v[i]));
+            }
+            const bool bad = m >= 0x7f800000u;
+            const int sh = min(100, 10 - ((int)(m >> 23) - 126));  // largest magnitude just under 2^10
+            const float up = exp2f((float)sh);
+            step = bad ? __uint_as_float(0x7fc00000u) : exp2f((float)-sh) * a.scale * 1.4426950408889634f;
+            uint8_t* panel = sq + rt * TERMS * kQPart;
+#pragma unroll 4
+            for (int d = 0; d < HD; d += 8) {
+                float v[8];
+                load8(q + d, v);
+                uint32_t hi[4], lo[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float x = bad ? 0.f : v[2 * i] * up, y = bad ? 0.f : v[2 * i + 1] * up;
+                    hi[i] = pack_h2(x, y);
+                    if (TERMS == 2) {
+                        const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi[i]));
+                        lo[i] = pack_h2(x - back.x, y - back.y);
+                    }
+                }
+                const uint32_t at = panel_at(kTileRows, lr, d / 8);
+                *reinterpret_cast<uint4*>(panel + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                if (TERMS == 2) *reinterpret_cast<uint4*>(panel + kQPart + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&q_full);
+        }
+        const int32_t last = live ? sp.base + tok : -1;
+        // no row of this warp hides a position before this one
+        const int32_t open = sp.base + min(r0 + (int32_t)(rt * kTileRows + quad * 32), rows - 1) / (int32_t)P.group;
+        const uint32_t to = tm + rt * kTileCols + ((quad * 32) << 16);  // O, then the score buffers
+        float M = kNegBig, l = 0.f;
+        bool ok = true;
+        for (uint32_t j = 0; j < steps && ok; ++j) {
+            const uint32_t st = j % ST;
+            ok = bwait(&kv_full[st], (j / ST) & 1, &abort_flag) && bwait(&s_full[rt][j & 1], (j >> 1) & 1, &abort_flag);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_after();
+            const uint32_t ts = to + HD + (j & 1) * NP;
+            uint32_t v[NP];
+#pragma unroll
+            for (uint32_t c = 0; c < NP; c += 32) tmem_ld32(ts + c, *reinterpret_cast<uint32_t(*)[32]>(v + c));
+            tmem_ld_wait();
+            float mx = -INFINITY;
+            const int32_t p0 = (b0 + (int32_t)(j * NB)) * 16;
+#pragma unroll
+            for (uint32_t b = 0; b < NB; ++b) {
+                const float f = step * f_sk[st][b], e = f_e[st][b];
+#pragma unroll
+                for (uint32_t i = 0; i < 16; ++i) {
+                    float x = fmaf(__uint_as_float(v[16 * b + i]), f, e);
+                    v[16 * b + i] = __float_as_uint(x);
+                }
+            }
+            if (p0 + (int32_t)NP - 1 > open || !live) {  // (or a row past the last one)
+#pragma unroll
+                for (uint32_t i = 0; i < NP; ++i)
+                    if (p0 + (int32_t)i > last) v[i] = 0xff800000u;  // -infinity
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < NP; ++i) mx = fmaxf(mx, __uint_as_float(v[i]));
+            if (__any_sync(0xffffffffu, mx > M + kSlack)) {
+                const float m = fmaxf(M, mx), f = exp2_fast(M - m);
+                M = m;
+                l *= f;
+                if (j > 0) {
+                    ok = __all_sync(0xffffffffu, bwait(&o_done[rt], (j - 1) & 1, &abort_flag));
+                    if (!ok) break;
+                    tc_after();
+                    for (uint32_t c = 0; c < HD; c += 32) {
+                        uint32_t o[32];
+                        tmem_ld32(to + c, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                        tmem_st32(to + c, o);
+                    }
+                }
+            }
+#pragma unroll
+            for (uint32_t b = 0; b < NB; ++b) {
+                float sum = 0.f;
+                uint32_t hi[8], lo[8];
+                const float mant = TERMS == 2 ? f_mant[st][b] : 1.f;
+#pragma unroll
+                for (uint32_t i = 0; i < 8; ++i) {
+                    const float w0 = exp2_fast(__uint_as_float(v[16 * b + 2 * i]) - M);
+                    const float w1 = exp2_fast(__uint_as_float(v[16 * b + 2 * i + 1]) - M);
+                    sum += w0 + w1;
+                    if (TERMS == 2) {
+                        const float q0 = w0 * mant, q1 = w1 * mant;
+                        hi[i] = pack_h2(q0, q1);
+                        const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi[i]));
+                        lo[i] = pack_h2(q0 - back.x, q1 - back.y);
+                    } else {
+                        hi[i] = pack_h2(w0, w1);
+                    }
+                }
+                l = fmaf(sum, f_down[st][b], l);
+                tmem_st8(ts + 8 * b, hi);
+                if (TERMS == 2) tmem_st8(ts + NP / 2 + 8 * b, lo);
+            }
+            tmem_st_wait();
+            tc_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[rt]);
+        }
+        if (steps && ok) ok = __all_sync(0xffffffffu, bwait(&o_done[rt], (steps - 1) & 1, &abort_flag));
+        tc_after();
+        if (ok) {
+            const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);  // a row that sees nothing: zeros
+            T* out = static_cast<T*>(a.out) + (uint64_t)(sp.q0 + tok) * a.out_stride + (uint64_t)head * HD;
+            const uint64_t slot = ((((uint64_t)s * a.c.kv_heads + h) * P.row_tiles + tile) * P.splits + split) * P.tile_rows +
+                                  rt * kTileRows + lr;
+            if (live && P.splits > 1) P.part_ml[slot] = make_float2(M, l);
+            for (uint32_t c = 0; c < HD; c += 32) {
+                uint32_t o[32];
+                if (steps) {
+                    tmem_ld32(to + c, o);
+                    tmem_ld_wait();
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] = 0;
+                }
+                if (!live) continue;
+                if (P.splits > 1) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4)
+                        *reinterpret_cast<uint4*>(P.part_o + slot * HD + c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4)
+                        *reinterpret_cast<float4*>(out + c + i) =
+                            make_float4(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv,
+                                        __uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8) {
+                        T y[8];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) y[k] = from_f32<T>(__uint_as_float(o[i + k]) * inv);
+                        *reinterpret_cast<uint4*>(out + c + i) = *reinterpret_cast<uint4*>(y);
+                    }
+                }
+            }
+        }
+    } else if (warp < kSoftWarps + 4) {
+        // ---------------------------------------------------------------- producers
+        const uint32_t pt = tid - 32 * kSoftWarps;  // 0..127
+        constexpr uint32_t CPR = HD / 16, N = NP * CPR / 128;  // 16-code pieces per row, per thread and operand
+        const int32_t* table = a.b.table + (uint64_t)s * a.b.table_stride;
+        const uint32_t bpp = a.c.page_size / 16;
+        auto page_of = [&](int32_t blk) {
+            if (blk >= b1) return -1;
+            const int32_t p = __ldg(table + (uint32_t)blk / bpp);
+            if (p >= 0 && (uint32_t)p < a.c.n_pages) return p;
+            flag_error(a.err, DEV_ERR_POSITION);
+            return -1;
+        };
+        uint4 k[N], v[N];
+        bool zero[N];
+        float sk = 0.f, sv = 0.f;
+        bool hidden = true;
+        auto load = [&](uint32_t j) {
+#pragma unroll
+            for (uint32_t i = 0; i < N; ++i) {
+                const uint32_t piece = pt + 128 * i, r = piece / CPR, c = piece % CPR;
+                const int32_t blk = b0 + (int32_t)(j * NB + r / 16), page = page_of(blk);
+                k[i] = v[i] = make_uint4(0, 0, 0, 0);
+                zero[i] = false;
+                if (page >= 0) {
+                    const uint64_t at = (uint64_t)page * a.c.page_stride +
+                                        ((uint64_t)h * a.c.page_size + (uint32_t)blk % bpp * 16 + r % 16) * HD + 16 * c;
+                    k[i] = ldg_nc(a.c.k + at);
+                    v[i] = ldg_nc(a.c.v + at);
+                    zero[i] = abs_bits(__ldg(a.c.vs + (uint64_t)page * a.c.scale_stride + h * bpp + (uint32_t)blk % bpp)) <
+                              0x00800000u;
+                }
+            }
+            if (pt < NB) {
+                const int32_t blk = b0 + (int32_t)(j * NB + pt), page = page_of(blk);
+                hidden = page < 0;
+                if (!hidden) {
+                    const uint64_t at = (uint64_t)page * a.c.scale_stride + h * bpp + (uint32_t)blk % bpp;
+                    sk = __ldg(a.c.ks + at);
+                    sv = __ldg(a.c.vs + at);
+                }
+            }
+        };
+        if (steps) load(0);
+        for (uint32_t j = 0; j < steps; ++j) {
+            const uint32_t st = j % ST;
+            if (j >= ST && !__all_sync(0xffffffffu, bwait(&kv_empty[st], (j / ST - 1) & 1, &abort_flag))) break;
+            uint8_t* dst = skv + st * 2 * kKv;
+#pragma unroll
+            for (uint32_t i = 0; i < N; ++i) {
+                const uint32_t piece = pt + 128 * i, r = piece / CPR, c = piece % CPR;
+                codes_to_panel(dst, NP, r, c, k[i], false);
+                codes_to_panel(dst + kKv, NP, r, c, v[i], zero[i]);  // (codes under a scale of 0 stand for 0)
+            }
+            if (pt < NB) {
+                const uint32_t sb = __float_as_uint(sv);
+                const int eb = (int)((sb >> 23) & 0xffu);
+                const bool plain = eb > 0 && eb < 255;
+                const bool bad = eb == 255;  // not finite; below the normal numbers: zeros
+                f_sk[st][pt] = hidden ? 0.f : sk;
+                if (TERMS == 2) {
+                    f_mant[st][pt] = plain ? __uint_as_float((sb & 0x807fffffu) | 0x3f800000u) : 1.f;
+                    f_down[st][pt] = plain ? __uint_as_float((uint32_t)(254 - eb) << 23) : 1.f;
+                    f_e[st][pt] = hidden ? -INFINITY : plain ? (float)(eb - 127) : bad ? __uint_as_float(0x7fc00000u) : 0.f;
+                } else {
+                    f_down[st][pt] = plain ? __fdiv_rn(1.f, sv) : 1.f;
+                    f_e[st][pt] = hidden ? -INFINITY : plain ? log2f(sv) : bad ? __uint_as_float(0x7fc00000u) : 0.f;
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&kv_full[st]);
+            if (j + 1 < steps) load(j + 1);
+        }
+    } else if (lane == 0 && steps) {
+        // ---------------------------------------------------------------- MMA
+        bool ok = bwait(&q_full, 0, &abort_flag);
+        auto scores = [&](uint32_t j) {
+            const uint32_t st = j % ST;
+            ok = ok && bwait(&kv_full[st], (j / ST) & 1, &abort_flag);
+            if (!ok) return;
+            tc_after();
+            const uint32_t kb = smem_addr(skv + st * 2 * kKv);
+#pragma unroll
+            for (uint32_t t = 0; t < RT; ++t) {
+                const uint32_t d = tm + t * kTileCols + HD + (j & 1) * NP;
+                const uint32_t qb = smem_addr(sq + t * TERMS * kQPart);
+#pragma unroll
+                for (uint32_t x = 0; x < (uint32_t)TERMS; ++x)
+#pragma unroll
+                    for (uint32_t k = 0; k < HD / 16; ++k)
+                        mma_ss(d, swizzled_desc(qb + x * kQPart + (k / 4) * (kTileRows * 128) + (k % 4) * 32, 16),
+                               swizzled_desc(kb + (k / 4) * (NP * 128) + (k % 4) * 32, 16), f16_idesc(NP, false), x > 0 || k > 0);
+                mma_commit(&s_full[t][j & 1]);
+            }
+        };
+        scores(0);
+        for (uint32_t j = 0; j < steps && ok; ++j) {
+            if (j + 1 < steps) scores(j + 1);
+            const uint32_t st = j % ST, vb = smem_addr(skv + st * 2 * kKv + kKv);
+#pragma unroll
+            for (uint32_t t = 0; t < RT; ++t) {
+                ok = ok && bwait(&p_full[t], j & 1, &abort_flag);
+                if (!ok) break;
+                tc_after();
+                const uint32_t d = tm + t * kTileCols, p = d + HD + (j & 1) * NP;
+#pragma unroll
+                for (uint32_t x = 0; x < (uint32_t)TERMS; ++x)
+#pragma unroll
+                    for (uint32_t k = 0; k < NP / 16; ++k)
+                        mma_ts(d, p + x * (NP / 2) + 8 * k, swizzled_desc(vb + k * 2048, NP * 128), f16_idesc(HD, true),
+                               j > 0 || x > 0 || k > 0);
+                mma_commit(&o_done[t]);
+            }
+            if (ok) mma_commit(&kv_empty[st]);
+        }
+        if (!ok) {  // the MMAs in flight end before the tensor memory is freed
+            mma_commit(&fin);
+            mbar_wait(&fin, 0);
+        }
+    }
+    __syncwarp();
+    tc_before();
+    __syncthreads();
+    if (tid == 0 && abort_flag) flag_error(a.err, DEV_ERR_WAIT_TIMEOUT);
+    if (warp == kSoftWarps + 4)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "r"(512) : "memory");
+}
+
 struct Shape {
-    uint32_t group, row_tiles, chunk, splits;
+    uint32_t group, row_tiles, tile_rows, chunk, splits;
+    bool tiles;      // the prompt kernel
     uint64_t slots;  // partials
 };
-Shape shape_of(const Kv8Cache& c, const Kv8Batch& b, uint32_t heads, int sms) {
+Shape shape_of(const Kv8Cache& c, const Kv8Batch& b, uint32_t heads, uint32_t type, int sms) {
     Shape r;
     r.group = heads / c.kv_heads;
-    r.row_tiles = (uint32_t)(((uint64_t)std::max(1u, b.max_new) * r.group + kRows - 1) / kRows);
+    const uint64_t rows = (uint64_t)std::max(1u, b.max_new) * r.group;
+    r.tiles = rows >= kTileMin;
+    const Role role = role_of((int)c.head_dim, type == GGML_F32 ? 2 : 1);
+    r.tile_rows = r.tiles ? role.rt * kTileRows : kRows;
+    r.row_tiles = (uint32_t)((rows + r.tile_rows - 1) / r.tile_rows);
     const uint32_t blocks = std::max(1u, (b.max_len + 15) / 16);
-    // chunks of positions: enough CTAs for three on every SM, at least 8 blocks (two per warp) each
+    // chunks of positions: enough CTAs for three on every SM (the prompt kernel: one), each with
+    // at least 8 blocks (two per warp; the prompt kernel: 32, eight steps)
     const uint64_t tiles = (uint64_t)b.n_seqs * c.kv_heads * r.row_tiles;
-    const uint64_t want = std::max<uint64_t>(1, (3ull * sms) / std::max<uint64_t>(1, tiles));
-    r.chunk = std::max(8u, (uint32_t)((blocks + want - 1) / want));
+    const uint64_t want = std::max<uint64_t>(1, (r.tiles ? 1ull : 3ull) * sms / std::max<uint64_t>(1, tiles));
+    r.chunk = std::max(r.tiles ? 32u : 8u, (uint32_t)((blocks + want - 1) / want));
+    r.chunk = (r.chunk + 3) / 4 * 4;
     r.splits = (blocks + r.chunk - 1) / r.chunk;
     r.slots = tiles * r.splits;
     return r;
 }
 
-template <class T, int HD> cudaError_t launch(const Plan& p, cudaStream_t s) {
-    kv8_split_kernel<T, HD>
-        <<<dim3(p.splits, p.row_tiles * p.a.c.kv_heads, p.a.b.n_seqs), 32 * kWarps, 0, s>>>(p);
+template <class T, int HD> cudaError_t launch(const Plan& p, bool tiles, cudaStream_t s) {
+    if (tiles) {
+        constexpr int terms = sizeof(T) == 4 ? 2 : 1;
+        constexpr uint32_t smem = tile_smem(HD, terms), threads = 32 * (4 * role_of(HD, terms).rt + 5);
+        static std::atomic<bool> opted[64];
+        int dev = 0;
+        cudaError_t e = cudaGetDevice(&dev);
+        if (e != cudaSuccess) return e;
+        if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+        if (!opted[dev].load()) {
+            e = cudaFuncSetAttribute(kv8_tile_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+            if (e != cudaSuccess) return e;
+            opted[dev] = true;
+        }
+        kv8_tile_kernel<T, HD><<<dim3(p.row_tiles * p.splits, p.a.c.kv_heads, p.a.b.n_seqs), threads, smem, s>>>(p);
+    } else {
+        kv8_split_kernel<T, HD>
+            <<<dim3(p.splits, p.row_tiles * p.a.c.kv_heads, p.a.b.n_seqs), 32 * kWarps, 0, s>>>(p);
+    }
     if (p.splits > 1)
         kv8_join_kernel<T, HD><<<dim3((p.a.b.max_new + 3) / 4, p.a.heads, p.a.b.n_seqs), 128, 0, s>>>(p);
     return cudaGetLastError();
 }
-template <class T> cudaError_t by_dim(const Plan& p, cudaStream_t s) {
-    return p.a.c.head_dim == 64 ? launch<T, 64>(p, s) : p.a.c.head_dim == 128 ? launch<T, 128>(p, s) : launch<T, 256>(p, s);
+template <class T> cudaError_t by_dim(const Plan& p, bool tiles, cudaStream_t s) {
+    return p.a.c.head_dim == 64    ? launch<T, 64>(p, tiles, s)
+           : p.a.c.head_dim == 128 ? launch<T, 128>(p, tiles, s)
+                                   : launch<T, 256>(p, tiles, s);
 }
 
 }  // namespace
 
-uint64_t kv8_attention_ws_bytes(const Kv8Cache& c, const Kv8Batch& b, uint32_t heads, int sms) {
-    const Shape sh = shape_of(c, b, heads, sms);
-    return sh.splits == 1 ? 0 : sh.slots * kRows * (c.head_dim + 2) * 4;
+uint64_t kv8_attention_ws_bytes(const Kv8Cache& c, const Kv8Batch& b, uint32_t heads, uint32_t type, int sms) {
+    const Shape sh = shape_of(c, b, heads, type, sms);
+    return sh.splits == 1 ? 0 : sh.slots * sh.tile_rows * (c.head_dim + 2) * 4;
 }
 
 cudaError_t launch_kv8_attention(const Kv8AttnArgs& a, int sms, cudaStream_t s) {
-    const Shape sh = shape_of(a.c, a.b, a.heads, sms);
-    if ((uint64_t)sh.row_tiles * a.c.kv_heads > 65535 || a.heads > 65535) return cudaErrorInvalidValue;
+    const Shape sh = shape_of(a.c, a.b, a.heads, a.type, sms);
+    if ((!sh.tiles && (uint64_t)sh.row_tiles * a.c.kv_heads > 65535) || (uint64_t)sh.row_tiles * sh.splits > 0x7fffffffull)
+        return cudaErrorInvalidValue;
     Plan p;
     p.a = a;
     p.group = sh.group;
     p.row_tiles = sh.row_tiles;
+    p.tile_rows = sh.tile_rows;
     p.chunk = sh.chunk;
     p.splits = sh.splits;
     p.part_o = reinterpret_cast<float*>(a.ws);
-    p.part_ml = reinterpret_cast<float2*>(p.part_o + sh.slots * kRows * a.c.head_dim);
+    p.part_ml = reinterpret_cast<float2*>(p.part_o + sh.slots * sh.tile_rows * a.c.head_dim);
     switch (a.type) {
-        case GGML_F32: return by_dim<float>(p, s);
-        case GGML_F16: return by_dim<__half>(p, s);
-        case GGML_BF16: return by_dim<__nv_bfloat16>(p, s);
+        case GGML_F32: return by_dim<float>(p, sh.tiles, s);
+        case GGML_F16: return by_dim<__half>(p, sh.tiles, s);
+        case GGML_BF16: return by_dim<__nv_bfloat16>(p, sh.tiles, s);
         default: return cudaErrorInvalidValue;
     }
 }

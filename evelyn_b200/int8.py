@@ -42,6 +42,23 @@ def _kind(t) -> int:
         return _kinds.setdefault(t.dtype, _TYPES[name])
 
 
+# What the checks of a call found, by the types, shapes and strides of its tensors (never by
+# their addresses): a call whose tensors are laid out like an earlier one's is not checked again.
+_plans: dict = {}
+_MOST_PLANS = 4096
+
+
+def _layout(*tensors) -> tuple:
+    return tuple([None if t is None else (t.dtype, t.shape, t.stride()) for t in tensors])
+
+
+def _planned(key: tuple, plan):
+    if len(_plans) >= _MOST_PLANS:
+        _plans.clear()
+    _plans[key] = plan
+    return plan
+
+
 def _need(ok: bool, msg: str):
     if not ok:
         raise EvelynError(1, msg)
@@ -76,18 +93,23 @@ def _err(err) -> Optional[int]:
     if err is None:
         return None
     _named(err, "int32", "err")
-    _need(err.shape.numel() >= 1, "err must hold one value")
+    _need(err.numel() >= 1, "err must hold one value")
     return err.data_ptr()
 
 
 def quantize_rows(x, codes, scales, stream: int = 0) -> None:
     """Rows of x [rows][cols] to codes [rows][cols] int8 and scales [rows] float32:
     scale = max|x| / 127, code = round(x / scale) (evl_i8_quantize_rows)."""
-    kind, xs, cs = _kind(x), _rows(x, "x"), _rows(codes, "codes")
-    rows, cols = x.shape
-    _named(codes, "int8", "codes")
-    _need(tuple(codes.shape) == (rows, cols), "codes must have the shape of x")
-    _flat(scales, rows, "float32", "scales")
+    key = ("rows", _layout(x, codes, scales))
+    plan = _plans.get(key)
+    if plan is None:
+        kind, xs, cs = _kind(x), _rows(x, "x"), _rows(codes, "codes")
+        rows, cols = x.shape
+        _named(codes, "int8", "codes")
+        _need(tuple(codes.shape) == (rows, cols), "codes must have the shape of x")
+        _flat(scales, rows, "float32", "scales")
+        plan = _planned(key, (kind, xs, rows, cols, cs))
+    kind, xs, rows, cols, cs = plan
     _check(runtime.lib().evl_i8_quantize_rows(kind, x.data_ptr(), xs, rows, cols, codes.data_ptr(), cs,
                                               scales.data_ptr(), stream))
 
@@ -95,21 +117,26 @@ def quantize_rows(x, codes, scales, stream: int = 0) -> None:
 def matmul(x, x_scales, w, w_scales, y, add=None, err=None, stream: int = 0) -> None:
     """y [rows][out] = (x [rows][cols] @ w [out][cols]^T) * x_scales[:, None] * w_scales (+ add),
     x and w int8 with rows on 16-byte boundaries, int32 sums (evl_i8_matmul)."""
-    kind, xst, wst, yst = _kind(y), _rows(x, "x"), _rows(w, "w"), _rows(y, "y")
-    rows, cols = x.shape
-    out = w.shape[0]
-    _named(x, "int8", "x")
-    _named(w, "int8", "w")
-    _need(w.shape[1] == cols, "x and w must have the same number of columns")
-    _need(tuple(y.shape) == (rows, out), "y must be [rows of x][rows of w]")
-    _flat(x_scales, rows, "float32", "x_scales")
-    _flat(w_scales, out, "float32", "w_scales")
-    ast = 0
-    if add is not None:
-        ast = _rows(add, "add")
-        _need(tuple(add.shape) == (rows, out) and add.dtype == y.dtype, "add must have the shape and type of y")
-    # (a single row has no stride; the operand's next 16-byte boundary stands in)
-    xst, wst = (-(-s // 16) * 16 if n <= 1 else s for s, n in ((xst, rows), (wst, out)))
+    key = ("matmul", _layout(x, x_scales, w, w_scales, y, add))
+    plan = _plans.get(key)
+    if plan is None:
+        kind, xst, wst, yst = _kind(y), _rows(x, "x"), _rows(w, "w"), _rows(y, "y")
+        rows, cols = x.shape
+        out = w.shape[0]
+        _named(x, "int8", "x")
+        _named(w, "int8", "w")
+        _need(w.shape[1] == cols, "x and w must have the same number of columns")
+        _need(tuple(y.shape) == (rows, out), "y must be [rows of x][rows of w]")
+        _flat(x_scales, rows, "float32", "x_scales")
+        _flat(w_scales, out, "float32", "w_scales")
+        ast = 0
+        if add is not None:
+            ast = _rows(add, "add")
+            _need(tuple(add.shape) == (rows, out) and add.dtype == y.dtype, "add must have the shape and type of y")
+        # (a single row has no stride; the operand's next 16-byte boundary stands in)
+        xst, wst = (-(-s // 16) * 16 if n <= 1 else s for s, n in ((xst, rows), (wst, out)))
+        plan = _planned(key, (kind, xst, wst, yst, ast, rows, out, cols))
+    kind, xst, wst, yst, ast, rows, out, cols = plan
     _check(runtime.lib().evl_i8_matmul(x.data_ptr(), xst, x_scales.data_ptr(), rows, w.data_ptr(), wst,
                                        w_scales.data_ptr(), out, cols, kind, _ptr(add), ast, y.data_ptr(), yst,
                                        _err(err), stream))
@@ -176,38 +203,48 @@ def kv8_append(cache: Kv8Cache, batch: Kv8Batch, k, v, q=None, q_out=None, rope=
     """Appends k, v [tokens][kv heads][head dim] to the cache and makes q [tokens][heads][head dim]
     ready into q_out (evl_kv8_append): an RMS norm per head with q_norm / k_norm [head dim]
     float32, then the rotation by rope [positions][rope dim / 2][2] float32 (cos, sin)."""
+    key = ("append", cache.kv_heads, cache.head_dim, interleaved, _layout(k, v, q, q_out, rope, q_norm, k_norm))
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _planned(key, _append_plan(cache, k, v, q, q_out, rope, q_norm, k_norm))
+    total, kind, kst, vst, qst, ost, heads, rl, rd = plan
+    prep = None
+    if rope is not None or q_norm is not None or k_norm is not None:
+        prep = C.byref(_Kv8Prep(_PREP_BYTES, rd, int(interleaved), rl, _ptr(rope), _ptr(q_norm), _ptr(k_norm), eps, 0))
+    _check(runtime.lib().evl_kv8_append(cache._ref, batch._of(total, cache.page_size), prep, kind, k.data_ptr(), kst,
+                                        v.data_ptr(), vst, _ptr(q), qst, heads, _ptr(q_out), ost, _err(err), stream))
+
+
+_PREP_BYTES = C.sizeof(_Kv8Prep)
+
+
+def _append_plan(cache, k, v, q, q_out, rope, q_norm, k_norm):
     total, dim, kind = k.shape[0], cache.head_dim, _kind(k)
     hk, kst = _heads(k, total, dim, "k")
     hv, vst = _heads(v, total, dim, "v")
     _need(hk == cache.kv_heads and hv == hk and v.dtype == k.dtype, "k and v must have the cache's heads and one type")
-    heads = qst = ost = 0
+    heads = qst = ost = rd = rl = 0
     if q is not None or q_out is not None:
         _need(q is not None and q_out is not None, "q and q_out go together")
         heads, qst = _heads(q, total, dim, "q")
         oh, ost = _heads(q_out, total, dim, "q_out")
         _need(oh == heads and q.dtype == k.dtype and q_out.dtype == k.dtype, "q and q_out must have one shape and k's type")
-    prep = None
-    if rope is not None or q_norm is not None or k_norm is not None:
-        rd = rl = 0
-        if rope is not None:
-            _named(rope, "float32", "rope")
-            _need(len(rope.shape) == 3 and rope.shape[2] == 2, "rope must be [positions][rope dim / 2][2]")
-            rl, rd = rope.shape[0], 2 * rope.shape[1]
-            _need(_rows(rope, "rope", 3) == rd, "rope must be contiguous")
-        for t, what in ((q_norm, "q_norm"), (k_norm, "k_norm")):
-            if t is not None:
-                _flat(t, dim, "float32", what)
-        prep = C.byref(_Kv8Prep(C.sizeof(_Kv8Prep), rd, int(interleaved), rl, _ptr(rope), _ptr(q_norm), _ptr(k_norm),
-                                eps, 0))
-    _check(runtime.lib().evl_kv8_append(cache._ref, batch._of(total, cache.page_size), prep, kind, k.data_ptr(), kst,
-                                        v.data_ptr(), vst, _ptr(q), qst, heads, _ptr(q_out), ost, _err(err), stream))
+    if rope is not None:
+        _named(rope, "float32", "rope")
+        _need(len(rope.shape) == 3 and rope.shape[2] == 2, "rope must be [positions][rope dim / 2][2]")
+        rl, rd = rope.shape[0], 2 * rope.shape[1]
+        _need(_rows(rope, "rope", 3) == rd, "rope must be contiguous")
+    for t, what in ((q_norm, "q_norm"), (k_norm, "k_norm")):
+        if t is not None:
+            _flat(t, dim, "float32", what)
+    return total, kind, kst, vst, qst, ost, heads, rl, rd
 
 
 def kv8_attention_workspace(cache: Kv8Cache, batch: Kv8Batch, q) -> int:
     """Bytes of workspace that kv8_attention needs for queries of q's shape (may be 0)."""
     n = C.c_size_t()
     _check(runtime.lib().evl_kv8_attention_workspace_bytes(cache._ref, batch._of(q.shape[0], cache.page_size),
-                                                           q.shape[1], C.byref(n)))
+                                                           _kind(q), q.shape[1], C.byref(n)))
     return int(n.value)
 
 
@@ -216,11 +253,19 @@ def kv8_attention(cache: Kv8Cache, batch: Kv8Batch, q, out, scale: float = 0.0, 
     """out [tokens][heads][head dim] = attention of q over the cache, each token up to its own
     position (evl_kv8_attention); scale 0 is 1 / sqrt(head dim). workspace: a device buffer of
     kv8_attention_workspace bytes, 256-byte aligned."""
-    total, kind = q.shape[0], _kind(q)
-    heads, qst = _heads(q, total, cache.head_dim, "q")
-    oh, ost = _heads(out, total, cache.head_dim, "out")
-    _need(oh == heads and out.dtype == q.dtype, "out must have the shape and type of q")
-    size = 0 if workspace is None else workspace.shape.numel() * workspace.element_size()
+    key = ("attention", cache.head_dim, _layout(q, out, workspace))
+    plan = _plans.get(key)
+    if plan is None:
+        total, kind = q.shape[0], _kind(q)
+        heads, qst = _heads(q, total, cache.head_dim, "q")
+        oh, ost = _heads(out, total, cache.head_dim, "out")
+        _need(oh == heads and out.dtype == q.dtype, "out must have the shape and type of q")
+        size = 0
+        if workspace is not None:
+            _need(workspace.numel() <= 1 or workspace.stride()[-1] == 1, "workspace must be contiguous")
+            size = workspace.numel() * workspace.element_size()
+        plan = _planned(key, (total, kind, heads, qst, ost, size))
+    total, kind, heads, qst, ost, size = plan
     _check(runtime.lib().evl_kv8_attention(cache._ref, batch._of(total, cache.page_size), kind, q.data_ptr(), qst, heads,
-                                           scale, out.data_ptr(), ost, _ptr(workspace) if size else None, size,
+                                           scale, out.data_ptr(), ost, workspace.data_ptr() if size else None, size,
                                            _err(err), stream))

@@ -183,7 +183,7 @@ SIGNATURES = {
     "evl_kv8_append": (C.c_int, [C.POINTER(_Kv8Cache), C.POINTER(_Kv8Batch), C.POINTER(_Kv8Prep), C.c_uint32, _P,
                                  C.c_uint64, _P, C.c_uint64, _P, C.c_uint64, C.c_uint32, _P, C.c_uint64, _P, _P]),
     "evl_kv8_attention_workspace_bytes": (C.c_int, [C.POINTER(_Kv8Cache), C.POINTER(_Kv8Batch), C.c_uint32,
-                                                    C.POINTER(C.c_size_t)]),
+                                                    C.c_uint32, C.POINTER(C.c_size_t)]),
     "evl_kv8_attention": (C.c_int, [C.POINTER(_Kv8Cache), C.POINTER(_Kv8Batch), C.c_uint32, _P, C.c_uint64, C.c_uint32,
                                     C.c_float, _P, C.c_uint64, _P, C.c_size_t, _P, _P]),
     "evl_remote_ffn_new": (C.c_int, [_P, C.c_size_t, C.POINTER(C.c_size_t), C.POINTER(C.c_char_p), C.c_uint32,

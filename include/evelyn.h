@@ -357,10 +357,10 @@ evl_status evl_kv8_append(const evl_kv8_cache* cache, const evl_kv8_batch* batch
                           uint32_t type, const void* d_k, uint64_t k_stride, const void* d_v, uint64_t v_stride,
                           const void* d_q, uint64_t q_stride, uint32_t heads, void* d_q_out, uint64_t q_out_stride,
                           int32_t* d_err, void* stream);
-/* Device workspace of evl_kv8_attention for this cache, batch bounds (n_seqs, max_new,
- * max_len) and number of heads, on the current device; it may be 0. Host only. */
-evl_status evl_kv8_attention_workspace_bytes(const evl_kv8_cache* cache, const evl_kv8_batch* batch, uint32_t heads,
-                                             size_t* bytes);
+/* Device workspace of evl_kv8_attention for this cache, batch bounds (n_seqs, total, max_new,
+ * max_len), type and number of heads, on the current device; it may be 0. Host only. */
+evl_status evl_kv8_attention_workspace_bytes(const evl_kv8_cache* cache, const evl_kv8_batch* batch, uint32_t type,
+                                             uint32_t heads, size_t* bytes);
 /* Attention of the batch's new tokens (appended before) over the cache: row (token, head)
  * attends the positions up to its own with softmax(scale * q . k), query head h reading kv
  * head h / (heads / kv_heads). d_q and d_out [total][heads][head_dim] of `type`, tokens q_stride /

@@ -89,7 +89,7 @@ def values(codes, scales, table_row, n):
     return c.transpose(0, 2, 1, 3).reshape(-1, codes.shape[1], codes.shape[3])[:n]
 
 
-def attention(q, k, v, first, scale):
+def attention(q, k, v, first, scale, weight_eps=0.0):
     """q [tokens][heads][dim] at positions first + i over k, v [positions][kv heads][dim], float64.
     Returns the output and a bound on an f32 implementation's error (see the GPU tests)."""
     q = q.astype(np.float64)
@@ -112,5 +112,8 @@ def attention(q, k, v, first, scale):
             dx += 6 * 2.0 ** -24 * (np.abs(x).max() + 40)
             # weights: exp2 2^-22, two f16 parts 2^-22; the sums over blocks of 16, warps and chunks
             dw = 2.0 ** -21 + (n / 16 + 16) * 2.0 ** -23
-            tol[i, h] = (2 * dx + 2 * dw) * (w @ np.abs(vv)).max() + 1e-30
+            # weight_eps: weights rounded once to fewer bits, each off by at most that share of
+            # itself: |sum (w + dw) v - sum w v| <= weight_eps sum w |v| (the sum that divides them is
+            # of the weights before that rounding)
+            tol[i, h] = (2 * dx + 2 * dw + weight_eps) * (w @ np.abs(vv)).max() + 1e-30
     return out, tol

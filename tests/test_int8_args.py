@@ -14,7 +14,7 @@ class Fake:
     """A tensor's description, at an address that is never read."""
 
     def __init__(self, shape, dtype="float32", stride=None, at=1 << 20):
-        self.shape, self.dtype, self._at = _Shape(shape), dtype, at
+        self.shape, self.dtype, self._at = tuple(shape), dtype, at
         self._stride = stride or tuple(int(np.prod(shape[i + 1:])) for i in range(len(shape)))
 
     def stride(self):
@@ -23,13 +23,11 @@ class Fake:
     def data_ptr(self):
         return self._at
 
+    def numel(self):
+        return int(np.prod(self.shape))
+
     def element_size(self):
         return {"float32": 4, "float16": 2, "bfloat16": 2, "int8": 1, "uint8": 1, "int32": 4, "float64": 8}[self.dtype]
-
-
-class _Shape(tuple):
-    def numel(self):
-        return int(np.prod(self))
 
 
 def refused(kind, word, fn, *a, **k):
@@ -137,9 +135,9 @@ def test_struct_sizes_are_checked():
     lib = runtime.lib()
     c, b = runtime._Kv8Cache(), runtime._Kv8Batch()
     n = C.c_size_t()
-    assert lib.evl_kv8_attention_workspace_bytes(C.byref(c), C.byref(b), 2, C.byref(n)) == 1
+    assert lib.evl_kv8_attention_workspace_bytes(C.byref(c), C.byref(b), 0, 2, C.byref(n)) == 1
     assert b"struct_size" in lib.evl_last_error()
-    assert lib.evl_kv8_attention_workspace_bytes(None, C.byref(b), 2, C.byref(n)) == 1
+    assert lib.evl_kv8_attention_workspace_bytes(None, C.byref(b), 0, 2, C.byref(n)) == 1
     assert lib.evl_kv8_append(None, None, None, 0, None, 0, None, 0, None, 0, 0, None, 0, None, None) == 1
 
 
