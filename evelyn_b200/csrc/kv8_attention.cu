@@ -8,7 +8,9 @@
 //   x = q . ck (an integer) * (sk * scale * log2 e * step of q) + e,  e = exponent of sv
 //   w = 2^(x - M),  l += w * 2^-e,  O += (w * sv 2^-e) * cv,  o = O / l
 // so w times a mantissa in [1, 2) meets the codes, whatever the size of the value scale, and
-// the power of two leaves the sum exactly.
+// the power of two leaves the sum exactly. Where e is far below M (value scales that differ by more
+// than 2^80) w would leave f32's range while the sum still needs it: such a block's weights
+// are kept 2^d larger, and 2^-d joins the mantissa and the power of two (aside()).
 //
 // Small-batch kernel (kv8_split_kernel): up to 8 rows (token, head) per CTA that share a kv head;
 // positions are the M dimension of the warp's products.
@@ -70,6 +72,19 @@ __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+// 2^from to 2^to for a sum of weights, in two steps: the ratio alone may leave f32's range
+__device__ __forceinline__ float rebase(float l, float from, float to) {
+    const float f = exp2_fast(0.5f * (from - to));
+    return (l * f) * f;
+}
+constexpr float kFar = 80.f;
+constexpr float kZeroExp = -100.f, kZeroDown = 1.2676506002282294e30f;  // 2^100
+// d >= 0 and 2^-d for a block of exponent e under the maximum M
+__device__ __forceinline__ float aside(float e, float M, float& f) {
+    const float d = fmaxf(0.f, M - kFar - e);
+    f = exp2_fast(-d);
+    return d;
 }
 // bytes 0, 1 (or 2, 3) of w, biased codes c + 128, as an exact f16 pair: 0x6400 | b is 1024 + b
 __device__ __forceinline__ uint32_t codes_h2(uint32_t w, uint32_t sel) {
@@ -250,13 +265,14 @@ __global__ void __launch_bounds__(32 * kWarps) kv8_split_kernel(const __grid_con
                     for (int i = 0; i < 3; ++i)
                         mma_s8(acc[i], cur.k[c][0][2 * j], cur.k[c][1][2 * j], cur.k[c][0][2 * j + 1],
                                cur.k[c][1][2 * j + 1], qb[i][c][2 * j], qb[i][c][2 * j + 1]);
-            // value scale = mant * 2^e; 0 (a block of zeros) and non-finite ones keep e = 0
+            // value scale = mant * 2^e; 0 (a block of zeros) must not raise the maximum of rows that
+            // see other blocks: kZeroExp; a scale that is not finite reaches the output as it is
             const uint32_t sb = __float_as_uint(cur.sv);
             const int eb = (int)((sb >> 23) & 0xffu);
             const bool plain = eb > 0 && eb < 255;
-            const float e = plain ? (float)(eb - 127) : 0.f;
-            const float mant = plain ? __uint_as_float((sb & 0x807fffffu) | 0x3f800000u) : cur.sv;
-            const float down = plain ? __uint_as_float((uint32_t)(254 - eb) << 23) : 1.f;  // 2^-e
+            const float e = plain ? (float)(eb - 127) : eb ? 0.f : kZeroExp;
+            const float mant = plain ? __uint_as_float((sb & 0x807fffffu) | 0x3f800000u) : eb ? cur.sv : 0.f;
+            const float down = plain ? __uint_as_float((uint32_t)(254 - eb) << 23) : eb ? 1.f : kZeroDown;  // 2^-e
             float x[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -279,23 +295,32 @@ __global__ void __launch_bounds__(32 * kWarps) kv8_split_kernel(const __grid_con
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
                     m = fmaxf(M[j], m);
                     const float f = exp2_fast(M[j] - m);
+                    l[j] = rebase(l[j], M[j], m);
                     M[j] = m;
-                    l[j] *= f;
 #pragma unroll
                     for (int i = 0; i < MT; ++i) o[i][j] *= f, o[i][j + 2] *= f;
                 }
             }
+            float off[2] = {M[0], M[1]}, mt[2] = {mant, mant}, dn[2] = {down, down};
+            if (e < fmaxf(M[0], M[1]) - kFar) {  // (rare)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    float f;
+                    off[j] -= aside(e, M[j], f);
+                    mt[j] *= f, dn[j] *= f;
+                }
+            }
             float w[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] = exp2_fast(x[j] - M[j & 1]);
-            l[0] = fmaf(w[0] + w[2], down, l[0]);
-            l[1] = fmaf(w[1] + w[3], down, l[1]);
+            for (int j = 0; j < 4; ++j) w[j] = exp2_fast(x[j] - off[j & 1]);
+            l[0] = fmaf(w[0] + w[2], dn[0], l[0]);
+            l[1] = fmaf(w[1] + w[3], dn[1], l[1]);
             uint32_t ph[2], pl[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 // (a hidden position has weight 0 even where the block's scale is not finite)
-                const float p0 = w[2 * i] > 0.f ? w[2 * i] * mant : 0.f;
-                const float p1 = w[2 * i + 1] > 0.f ? w[2 * i + 1] * mant : 0.f;
+                const float p0 = w[2 * i] > 0.f ? w[2 * i] * mt[0] : 0.f;
+                const float p1 = w[2 * i + 1] > 0.f ? w[2 * i + 1] * mt[1] : 0.f;
                 const uint32_t hi = pack_h2(p0, p1);
                 const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi));
                 ph[i] = transpose8(hi);
@@ -354,7 +379,7 @@ __global__ void __launch_bounds__(32 * kWarps) kv8_split_kernel(const __grid_con
             const float2 ml = sml[k][r];
             const float f = exp2_fast(ml.x - m);
             const float4 p = *reinterpret_cast<const float4*>(&so[k][r][d]);
-            sum = fmaf(ml.y, f, sum);
+            sum += rebase(ml.y, ml.x, m);
             v[0] = fmaf(p.x, f, v[0]), v[1] = fmaf(p.y, f, v[1]), v[2] = fmaf(p.z, f, v[2]), v[3] = fmaf(p.w, f, v[3]);
         }
         if (P.splits == 1) {
@@ -395,7 +420,7 @@ template <class T, int HD> __global__ void __launch_bounds__(128) kv8_join_kerne
         const uint64_t p = (at + k) * P.tile_rows + row % P.tile_rows;
         const float2 ml = P.part_ml[p];
         const float f = exp2_fast(ml.x - m);
-        sum = fmaf(ml.y, f, sum);
+        sum += rebase(ml.y, ml.x, m);
 #pragma unroll
         for (int c = 0; c < N; ++c) {
             const float2 w = *reinterpret_cast<const float2*>(P.part_o + p * HD + 64 * c + 2 * lane);
@@ -429,16 +454,26 @@ template <class T, int HD> __global__ void __launch_bounds__(128) kv8_join_kerne
 constexpr uint32_t kTileRows = 128;
 constexpr uint32_t kTileMin = 48;  // rows per (sequence, kv head) from which it is used
 
-struct Role {  // per (HD, TERMS)
-    uint32_t rt, np, stages;
+struct Role {  // per (HD, TERMS): row tiles, positions per step, stages of f16 panels, of codes
+    uint32_t rt, np, stages, raw;
 };
 __host__ __device__ constexpr Role role_of(int hd, int terms) {
-    return hd == 256 ? (terms == 2 ? Role{1, 32, 2} : Role{1, 64, 2}) : terms == 2 ? Role{1, 64, 3} : Role{2, 64, 3};
+    return hd == 256 ? (terms == 2 ? Role{1, 32, 2, 2} : Role{1, 64, 2, 1}) : terms == 2 ? Role{1, 64, 2, 4} : Role{2, 64, 2, 4};
 }
 __host__ __device__ constexpr uint32_t tile_smem(int hd, int terms) {
     return role_of(hd, terms).rt * terms * kTileRows * hd * 2 +
-           role_of(hd, terms).stages * (2 * role_of(hd, terms).np * hd * 2) + 1024;
+           role_of(hd, terms).np * hd * (4 * role_of(hd, terms).stages + 2 * role_of(hd, terms).raw) + 1024;
 }
+static_assert(tile_smem(256, 2) <= 232448 && tile_smem(256, 1) <= 232448 && tile_smem(128, 1) <= 232448, "shared memory");
+
+__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async4(void* dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_addr(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 __device__ __forceinline__ bool bwait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
     if (mbar_try_wait(bar, parity)) return true;
@@ -489,15 +524,11 @@ __device__ __forceinline__ void tmem_ld32(uint32_t t, uint32_t (&v)[32]) {
         : "r"(t)
         : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t t, const uint32_t (&v)[32]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
-        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(t),
-        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
-        "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
-        "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
-        : "memory");
+__device__ __forceinline__ void tmem_ld8(uint32_t t, uint32_t (&v)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+                 : "r"(t)
+                 : "memory");
 }
 __device__ __forceinline__ void tmem_st8(uint32_t t, const uint32_t* v) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(t), "r"(v[0]), "r"(v[1]),
@@ -525,18 +556,23 @@ __device__ __forceinline__ void codes_to_panel(uint8_t* panel, uint32_t rows, ui
     *reinterpret_cast<uint4*>(panel + panel_at(rows, r, 2 * c + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
 }
 
+__device__ __forceinline__ void producers_sync() {
+    __syncwarp();
+    asm volatile("barrier.cta.sync 1, 128;" ::: "memory");
+}
+
 template <class T, int HD>
 __global__ void __launch_bounds__(32 * (4 * role_of(HD, sizeof(T) == 4 ? 2 : 1).rt + 5), 1)
     kv8_tile_kernel(const __grid_constant__ Plan P) {
     constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
     constexpr Role R = role_of(HD, TERMS);
-    constexpr uint32_t RT = R.rt, NP = R.np, ST = R.stages, NB = NP / 16;
+    constexpr uint32_t RT = R.rt, NP = R.np, ST = R.stages, RAW = R.raw, NB = NP / 16;
     constexpr uint32_t kQPart = kTileRows * HD * 2;   // one f16 part of a row tile's q
     constexpr uint32_t kKv = NP * HD * 2;             // K (or V) of a stage
     constexpr uint32_t kSoftWarps = 4 * RT, kTileCols = RT == 2 ? 256 : 512;  // tensor memory columns per row tile
     extern __shared__ uint8_t raw_smem[];
-    __shared__ __align__(8) uint64_t kv_full[ST], kv_empty[ST], s_full[RT][2], p_full[RT], o_done[RT], q_full, fin;
-    __shared__ float f_sk[ST][NB], f_e[ST][NB], f_down[ST][NB], f_mant[ST][NB];
+    __shared__ __align__(8) uint64_t kv_full[ST], kv_empty[ST], s_full[RT][2], p_full[RT][2], o_done[RT], q_full, fin;
+    __shared__ float raw_sk[RAW][NB], raw_sv[RAW][NB], f_sk[ST][NB], f_e[ST][NB], f_down[ST][NB], f_mant[ST][NB];
     __shared__ uint32_t tmem_base;
     __shared__ volatile int abort_flag;
     const Kv8AttnArgs& a = P.a;
@@ -559,7 +595,8 @@ __global__ void __launch_bounds__(32 * (4 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
 
     uint8_t* smem = raw_smem + ((1024u - (smem_addr(raw_smem) & 1023u)) & 1023u);
     uint8_t* sq = smem;                                  // [RT][TERMS] q panels
-    uint8_t* skv = smem + RT * TERMS * kQPart;           // [ST][K | V]
+    uint8_t* skv = smem + RT * TERMS * kQPart;           // [ST][K | V] f16 panels
+    uint8_t* sraw = skv + ST * 2 * kKv;                  // [RAW][K | V] codes, 16 bytes per thread and piece
     if (tid == 0) {
         abort_flag = 0;
         for (uint32_t i = 0; i < ST; ++i) {
@@ -569,7 +606,9 @@ __global__ void __launch_bounds__(32 * (4 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
         for (uint32_t i = 0; i < RT; ++i) {
             mbar_init(&s_full[i][0], 1);
             mbar_init(&s_full[i][1], 1);
-            mbar_init(&p_full[i], 4);
+            // (one per buffer: a warp may finish the next step's weights before another has this one's)
+            mbar_init(&p_full[i][0], 4);
+            mbar_init(&p_full[i][1], 4);
             mbar_init(&o_done[i], 1);
         }
         mbar_init(&q_full, kSoftWarps);
@@ -607,8 +646,8 @@ __global__ void __launch_bounds__(32 * (4 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
             }
             const bool bad = m >= 0x7f800000u;
             const int sh = min(100, 10 - ((int)(m >> 23) - 126));  // largest magnitude just under 2^10
-            const float up = exp2f((float)sh);
-            step = bad ? __uint_as_float(0x7fc00000u) : exp2f((float)-sh) * a.scale * 1.4426950408889634f;
+            const float up = copysignf(exp2f((float)sh), a.scale);  // (so that the factor is not negative)
+            step = bad ? __uint_as_float(0x7fc00000u) : exp2f((float)-sh) * fabsf(a.scale) * 1.4426950408889634f;
             uint8_t* panel = sq + rt * TERMS * kQPart;
 #pragma unroll 4
             for (int d = 0; d < HD; d += 8) {
@@ -649,69 +688,86 @@ __global__ void __launch_bounds__(32 * (4 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
 #pragma unroll
             for (uint32_t c = 0; c < NP; c += 32) tmem_ld32(ts + c, *reinterpret_cast<uint32_t(*)[32]>(v + c));
             tmem_ld_wait();
-            float mx = -INFINITY;
             const int32_t p0 = (b0 + (int32_t)(j * NB)) * 16;
-#pragma unroll
-            for (uint32_t b = 0; b < NB; ++b) {
-                const float f = step * f_sk[st][b], e = f_e[st][b];
-#pragma unroll
-                for (uint32_t i = 0; i < 16; ++i) {
-                    float x = fmaf(__uint_as_float(v[16 * b + i]), f, e);
-                    v[16 * b + i] = __float_as_uint(x);
-                }
-            }
-            if (p0 + (int32_t)NP - 1 > open || !live) {  // (or a row past the last one)
+            const bool masked = __any_sync(0xffffffffu, p0 + (int32_t)NP - 1 > open || !live);
+            if (masked) {
 #pragma unroll
                 for (uint32_t i = 0; i < NP; ++i)
                     if (p0 + (int32_t)i > last) v[i] = 0xff800000u;  // -infinity
             }
+            // the largest score: of each block's products, then by the block's factor (not negative)
+            float mx = -INFINITY, f[NB], e[NB];
 #pragma unroll
-            for (uint32_t i = 0; i < NP; ++i) mx = fmaxf(mx, __uint_as_float(v[i]));
+            for (uint32_t b = 0; b < NB; ++b) {
+                f[b] = step * f_sk[st][b];
+                e[b] = f_e[st][b];
+                float m = __uint_as_float(v[16 * b]);
+#pragma unroll
+                for (uint32_t i = 1; i < 16; ++i) m = fmaxf(m, __uint_as_float(v[16 * b + i]));
+                // (a hidden block and a factor of 0: 0 * -infinity is not a number)
+                mx = fmaxf(mx, m == -INFINITY ? m : fmaf(m, f[b], e[b]));
+            }
             if (__any_sync(0xffffffffu, mx > M + kSlack)) {
-                const float m = fmaxf(M, mx), f = exp2_fast(M - m);
+                const float m = fmaxf(M, mx), f8 = exp2_fast(M - m);
+                l = rebase(l, M, m);
                 M = m;
-                l *= f;
                 if (j > 0) {
                     ok = __all_sync(0xffffffffu, bwait(&o_done[rt], (j - 1) & 1, &abort_flag));
                     if (!ok) break;
                     tc_after();
-                    for (uint32_t c = 0; c < HD; c += 32) {
-                        uint32_t o[32];
-                        tmem_ld32(to + c, o);
+#pragma unroll 1
+                    for (uint32_t c = 0; c < HD; c += 8) {  // (rare: in few registers)
+                        uint32_t o[8];
+                        tmem_ld8(to + c, o);
                         tmem_ld_wait();
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                        tmem_st32(to + c, o);
+                        for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f8);
+                        tmem_st8(to + c, o);
                     }
                 }
             }
+            bool far = false;
 #pragma unroll
-            for (uint32_t b = 0; b < NB; ++b) {
-                float sum = 0.f;
-                uint32_t hi[8], lo[8];
-                const float mant = TERMS == 2 ? f_mant[st][b] : 1.f;
+            for (uint32_t b = 0; b < NB; ++b) far |= e[b] < M - kFar && e[b] != -INFINITY;
+            auto weights = [&](auto rare) {  // rare: hidden positions, or a block far below the maximum
+                constexpr bool RARE = decltype(rare)::value;
 #pragma unroll
-                for (uint32_t i = 0; i < 8; ++i) {
-                    const float w0 = exp2_fast(__uint_as_float(v[16 * b + 2 * i]) - M);
-                    const float w1 = exp2_fast(__uint_as_float(v[16 * b + 2 * i + 1]) - M);
-                    sum += w0 + w1;
-                    if (TERMS == 2) {
-                        const float q0 = w0 * mant, q1 = w1 * mant;
-                        hi[i] = pack_h2(q0, q1);
-                        const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi[i]));
-                        lo[i] = pack_h2(q0 - back.x, q1 - back.y);
-                    } else {
+                for (uint32_t b = 0; b < NB; ++b) {
+                    float sum = 0.f;
+                    uint32_t hi[8], lo[8];
+                    float mant = TERMS == 2 ? f_mant[st][b] : 1.f, off = e[b] - M, down = f_down[st][b];
+                    if (RARE && off < -kFar && off != -INFINITY) {
+                        float f;
+                        off += aside(e[b], M, f);
+                        mant *= f, down *= f;
+                    }
+#pragma unroll
+                    for (uint32_t i = 0; i < 8; ++i) {
+                        const float x0 = __uint_as_float(v[16 * b + 2 * i]), x1 = __uint_as_float(v[16 * b + 2 * i + 1]);
+                        float w0 = exp2_fast(fmaf(x0, f[b], off)), w1 = exp2_fast(fmaf(x1, f[b], off));
+                        if (RARE) {  // (a product itself is never infinite)
+                            w0 = x0 == -INFINITY ? 0.f : w0;
+                            w1 = x1 == -INFINITY ? 0.f : w1;
+                        }
+                        sum += w0 + w1;
+                        if (TERMS == 2 || RARE) w0 *= mant, w1 *= mant;
                         hi[i] = pack_h2(w0, w1);
+                        if (TERMS == 2) {
+                            const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi[i]));
+                            lo[i] = pack_h2(w0 - back.x, w1 - back.y);
+                        }
                     }
+                    l = fmaf(sum, down, l);
+                    tmem_st8(ts + 8 * b, hi);
+                    if (TERMS == 2) tmem_st8(ts + NP / 2 + 8 * b, lo);
                 }
-                l = fmaf(sum, f_down[st][b], l);
-                tmem_st8(ts + 8 * b, hi);
-                if (TERMS == 2) tmem_st8(ts + NP / 2 + 8 * b, lo);
-            }
+            };
+            if (masked || __any_sync(0xffffffffu, far)) weights(std::true_type{});
+            else weights(std::false_type{});
             tmem_st_wait();
             tc_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[rt]);
+            if (lane == 0) mbar_arrive(&p_full[rt][j & 1]);
         }
         if (steps && ok) ok = __all_sync(0xffffffffu, bwait(&o_done[rt], (steps - 1) & 1, &abort_flag));
         tc_after();
@@ -765,67 +821,89 @@ __global__ void __launch_bounds__(32 * (4 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
             flag_error(a.err, DEV_ERR_POSITION);
             return -1;
         };
-        uint4 k[N], v[N];
-        bool zero[N];
-        float sk = 0.f, sv = 0.f;
-        bool hidden = true;
-        auto load = [&](uint32_t j) {
+        // Codes travel ahead in a ring of their own: every thread copies the pieces that it will
+        // widen itself (asynchronously, RAW steps ahead), the scales are copied beside them.
+        // RAW + 1 steps ahead the page of each of the thread's pieces is looked up.
+        uint32_t page[N];
+        constexpr uint32_t kNone = 0xffffffffu;
+        auto pages = [&](uint32_t j) {
+#pragma unroll
+            for (uint32_t i = 0; i < N; ++i) page[i] = (uint32_t)page_of(b0 + (int32_t)(j * NB + (pt + 128 * i) / CPR / 16));
+        };
+        uint32_t gone = 0;  // bits: this thread's pieces of step j % RAW without a page
+        auto fetch = [&](uint32_t j) {
+            uint8_t* raw = sraw + (j % RAW) * (2 * NP * HD);
 #pragma unroll
             for (uint32_t i = 0; i < N; ++i) {
                 const uint32_t piece = pt + 128 * i, r = piece / CPR, c = piece % CPR;
-                const int32_t blk = b0 + (int32_t)(j * NB + r / 16), page = page_of(blk);
-                k[i] = v[i] = make_uint4(0, 0, 0, 0);
-                zero[i] = false;
-                if (page >= 0) {
-                    const uint64_t at = (uint64_t)page * a.c.page_stride +
-                                        ((uint64_t)h * a.c.page_size + (uint32_t)blk % bpp * 16 + r % 16) * HD + 16 * c;
-                    k[i] = ldg_nc(a.c.k + at);
-                    v[i] = ldg_nc(a.c.v + at);
-                    zero[i] = abs_bits(__ldg(a.c.vs + (uint64_t)page * a.c.scale_stride + h * bpp + (uint32_t)blk % bpp)) <
-                              0x00800000u;
-                }
-            }
-            if (pt < NB) {
-                const int32_t blk = b0 + (int32_t)(j * NB + pt), page = page_of(blk);
-                hidden = page < 0;
-                if (!hidden) {
-                    const uint64_t at = (uint64_t)page * a.c.scale_stride + h * bpp + (uint32_t)blk % bpp;
-                    sk = __ldg(a.c.ks + at);
-                    sv = __ldg(a.c.vs + at);
+                const uint32_t sub = (uint32_t)(b0 + (int32_t)(j * NB + r / 16)) % bpp;
+                const uint32_t bit = 1u << (j % RAW * N + i);
+                gone = page[i] == kNone ? gone | bit : gone & ~bit;
+                if (page[i] != kNone) {
+                    const uint64_t at = (uint64_t)page[i] * a.c.page_stride + ((uint64_t)h * a.c.page_size + sub * 16 + r % 16) * HD + 16 * c;
+                    cp_async16(raw + 16 * piece, a.c.k + at);
+                    cp_async16(raw + NP * HD + 16 * piece, a.c.v + at);
+                    if (c == 0 && r % 16 == 0) {
+                        const uint64_t sc = (uint64_t)page[i] * a.c.scale_stride + h * bpp + sub;
+                        cp_async4(&raw_sk[j % RAW][r / 16], a.c.ks + sc);
+                        cp_async4(&raw_sv[j % RAW][r / 16], a.c.vs + sc);
+                    }
+                } else if (c == 0 && r % 16 == 0) {
+                    raw_sk[j % RAW][r / 16] = __uint_as_float(0xff800000u);  // -infinity: hidden
                 }
             }
         };
-        if (steps) load(0);
+        pages(0);
+#pragma unroll
+        for (uint32_t j = 0; j < RAW; ++j) {
+            if (j < steps) {
+                fetch(j);
+                pages(j + 1);
+            }
+            cp_async_commit();
+        }
         for (uint32_t j = 0; j < steps; ++j) {
-            const uint32_t st = j % ST;
-            if (j >= ST && !__all_sync(0xffffffffu, bwait(&kv_empty[st], (j / ST - 1) & 1, &abort_flag))) break;
+            const uint32_t st = j % ST, rs = j % RAW;
+            cp_async_wait<(int)RAW - 1>();
+            producers_sync();  // everyone's scales of this step
+            if (j >= ST && !__all_sync(0xffffffffu, bwait(&kv_empty[st], (j / ST - 1) & 1, &abort_flag))) abort_flag = 1;
+            const uint8_t* raw = sraw + rs * (2 * NP * HD);
             uint8_t* dst = skv + st * 2 * kKv;
 #pragma unroll
             for (uint32_t i = 0; i < N; ++i) {
                 const uint32_t piece = pt + 128 * i, r = piece / CPR, c = piece % CPR;
-                codes_to_panel(dst, NP, r, c, k[i], false);
-                codes_to_panel(dst + kKv, NP, r, c, v[i], zero[i]);  // (codes under a scale of 0 stand for 0)
+                const bool none = gone >> (rs * N + i) & 1;
+                const uint4 k = *reinterpret_cast<const uint4*>(raw + 16 * piece);
+                const uint4 v = *reinterpret_cast<const uint4*>(raw + NP * HD + 16 * piece);
+                codes_to_panel(dst, NP, r, c, k, none);
+                // codes under a scale of 0 (or below the normal numbers) stand for 0
+                codes_to_panel(dst + kKv, NP, r, c, v, none || abs_bits(raw_sv[rs][r / 16]) < 0x00800000u);
             }
             if (pt < NB) {
+                const float sk = raw_sk[rs][pt], sv = raw_sv[rs][pt];
                 const uint32_t sb = __float_as_uint(sv);
                 const int eb = (int)((sb >> 23) & 0xffu);
-                const bool plain = eb > 0 && eb < 255;
-                const bool bad = eb == 255;  // not finite; below the normal numbers: zeros
+                const bool plain = eb > 0 && eb < 255, bad = eb == 255, hidden = sk == -INFINITY;
                 f_sk[st][pt] = hidden ? 0.f : sk;
                 if (TERMS == 2) {
                     f_mant[st][pt] = plain ? __uint_as_float((sb & 0x807fffffu) | 0x3f800000u) : 1.f;
-                    f_down[st][pt] = plain ? __uint_as_float((uint32_t)(254 - eb) << 23) : 1.f;
-                    f_e[st][pt] = hidden ? -INFINITY : plain ? (float)(eb - 127) : bad ? __uint_as_float(0x7fc00000u) : 0.f;
+                    f_down[st][pt] = plain ? __uint_as_float((uint32_t)(254 - eb) << 23) : kZeroDown;
+                    f_e[st][pt] = hidden ? -INFINITY : plain ? (float)(eb - 127) : bad ? __uint_as_float(0x7fc00000u) : kZeroExp;
                 } else {
-                    f_down[st][pt] = plain ? __fdiv_rn(1.f, sv) : 1.f;
-                    f_e[st][pt] = hidden ? -INFINITY : plain ? log2f(sv) : bad ? __uint_as_float(0x7fc00000u) : 0.f;
+                    f_down[st][pt] = plain ? __fdiv_rn(1.f, sv) : kZeroDown;
+                    f_e[st][pt] = hidden ? -INFINITY : plain ? log2f(sv) : bad ? __uint_as_float(0x7fc00000u) : kZeroExp;
                 }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
+            producers_sync();  // everyone's reads of this step's codes and scales
             if (lane == 0) mbar_arrive(&kv_full[st]);
-            if (j + 1 < steps) load(j + 1);
+            if (j + RAW < steps) {
+                fetch(j + RAW);
+                pages(j + RAW + 1);
+            }
+            cp_async_commit();  // (after an abort the loop runs out quickly: every wait gives up at once)
         }
+        cp_async_wait<0>();
     } else if (lane == 0 && steps) {
         // ---------------------------------------------------------------- MMA
         bool ok = bwait(&q_full, 0, &abort_flag);
@@ -854,7 +932,7 @@ __global__ void __launch_bounds__(32 * (4 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
             const uint32_t st = j % ST, vb = smem_addr(skv + st * 2 * kKv + kKv);
 #pragma unroll
             for (uint32_t t = 0; t < RT; ++t) {
-                ok = ok && bwait(&p_full[t], j & 1, &abort_flag);
+                ok = ok && bwait(&p_full[t][j & 1], (j >> 1) & 1, &abort_flag);
                 if (!ok) break;
                 tc_after();
                 const uint32_t d = tm + t * kTileCols, p = d + HD + (j & 1) * NP;

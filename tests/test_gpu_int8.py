@@ -326,12 +326,13 @@ def test_attention_many_tokens(kind, dim, page, heads, hk, lens, new):
     assert int(kv.err) == 0
 
 
-def test_attention_long_and_scaled():
+@pytest.mark.parametrize("lens,new", [([20001, 9], [1, 1]), ([2100, 70], [50, 64])])
+@pytest.mark.parametrize("scale", [0.3, -0.2])
+def test_attention_long_and_scaled(lens, new, scale):
     rng = np.random.default_rng(5)
-    lens = [20001, 9]
     kv = Kv(rng, 2, 128, 64, lens)
-    q = dev(rng.standard_normal((2, 8, 128)).astype(np.float32))
-    _check(kv, lens, [1, 1], q, _attend(kv, lens, [1, 1], q, "f32", scale=0.3), "f32", scale=np.float32(0.3))
+    q = dev(rng.standard_normal((sum(new), 8, 128)).astype(np.float32))
+    _check(kv, lens, new, q, _attend(kv, lens, new, q, "f32", scale=scale), "f32", scale=np.float32(scale))
 
 
 def test_attention_strided_views():
@@ -351,22 +352,27 @@ def test_attention_strided_views():
     assert not host(out[:, :4]).any() and not host(out[:, 8:]).any()
 
 
-def test_attention_scales_of_any_size():
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+@pytest.mark.parametrize("new", [4, 13])
+def test_attention_scales_of_any_size(kind, new):
     """Blocks of zeros (scale 0), huge and tiny value scales side by side, keys of scale 0."""
     rng = np.random.default_rng(7)
     kv = Kv(rng, 1, 128, 16, [160])
     pg = kv.table[0]
     kv.vs[pg[0]], kv.v[pg[0]] = 0, 0
-    kv.vs[pg[1]], kv.vs[pg[2]], kv.vs[pg[3]] = 1e-30, 1e20, 1e19
+    # (f16 outputs hold up to 65504)
+    kv.vs[pg[1]], kv.vs[pg[2]], kv.vs[pg[3]] = (1e-30, 1e20, 1e19) if kind == "f32" else (1e-30, 100, 1e-3)
     kv.ks[pg[4]], kv.k[pg[4]] = 0, 0
     kv.vs[pg[5]] = 0  # codes of any value under a scale of 0 stand for 0
     kv.dv.copy_(dev(kv.v)), kv.dk.copy_(dev(kv.k)), kv.dks.copy_(dev(kv.ks)), kv.dvs.copy_(dev(kv.vs))
-    q = dev(rng.standard_normal((4, 4, 128)).astype(np.float32))
-    for lens, new in (([160], [4]), ([16], [4]), ([30], [4]), ([96], [4])):
-        _check(kv, lens, new, q, _attend(kv, lens, new, q, "f32"), "f32")
+    q = dev(rng.standard_normal((new, 4, 128)).astype(np.float32), kind)
+    for n in (160, 16, 30, 96):
+        _check(kv, [n], [new], q, _attend(kv, [n], [new], q, kind), kind)
 
 
-def test_attention_ignores_what_it_does_not_see():
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [40, 90])
+def test_attention_ignores_what_it_does_not_see(kind, n):
     """Codes and scales past the length, other pages and hidden blocks may hold anything."""
     rng = np.random.default_rng(8)
     kv = Kv(rng, 2, 64, 32, [100])
@@ -377,41 +383,48 @@ def test_attention_ignores_what_it_does_not_see():
     kv.ks[kv.free], kv.vs[kv.free] = np.nan, np.inf
     for d, a in ((kv.dk, kv.k), (kv.dv, kv.v), (kv.dks, kv.ks), (kv.dvs, kv.vs)):
         d.copy_(dev(a))
-    q = dev(rng.standard_normal((40, 2, 64)).astype(np.float32))
-    _check(kv, [100], [40], q, _attend(kv, [100], [40], q, "f32"), "f32")
+    q = dev(rng.standard_normal((n, 2, 64)).astype(np.float32), kind)
+    _check(kv, [100], [n], q, _attend(kv, [100], [n], q, kind), kind)
     # a block that is not finite reaches the tokens that see it, and no other
     blk = kv.table[0][2]  # positions 64..95
     for s in (kv.dks, kv.dvs):
         keep = s.clone()
         s[int(blk), 0, 0] = float("nan")  # positions 64..79 of kv head 0
-        got = host(_attend(kv, [100], [40], q, "f32"))
+        got = host(_attend(kv, [100], [n], q, kind))
         s.copy_(keep)
-        assert np.isnan(got[4:, 0]).all() and np.isfinite(got[:4]).all() and np.isfinite(got[:, 1]).all()
+        see = n - 36  # the tokens before it stand at positions up to 63
+        assert np.isnan(got[see:, 0]).all() and np.isfinite(got[:see]).all() and np.isfinite(got[:, 1]).all()
 
 
-def test_attention_queries_that_are_not_finite():
+@pytest.mark.parametrize("n", [3, 30])
+def test_attention_queries_that_are_not_finite(n):
     rng = np.random.default_rng(13)
     kv = Kv(rng, 1, 128, 16, [50])
-    q = rng.standard_normal((3, 2, 128)).astype(np.float32)
+    q = rng.standard_normal((n, 2, 128)).astype(np.float32)
     q[0, 1, 5], q[2, 0, 100] = np.nan, np.inf
     q[1, 1] = 0
     dq = dev(q)
-    got = host(_attend(kv, [50], [3], dq, "f32"))
+    got = host(_attend(kv, [50], [n], dq, "f32"))
     assert np.isnan(got[0, 1]).all() and np.isnan(got[2, 0]).all()
     q[0, 1], q[2, 0] = 0, 0
     fine = np.isfinite(got).all(-1)
-    assert fine.sum() == 4
-    want = host(_attend(kv, [50], [3], dev(q), "f32"))
+    assert fine.sum() == 2 * n - 2
+    want = host(_attend(kv, [50], [n], dev(q), "f32"))
     assert same(got[fine], want[fine])
 
 
-def test_attention_skips_what_is_out_of_range():
+@pytest.mark.parametrize("many", [False, True])
+def test_attention_skips_what_is_out_of_range(many):
+    """(many: max_new large enough for the prompt kernel)"""
     rng = np.random.default_rng(14)
     kv = Kv(rng, 1, 64, 16, [64, 64, 64])
     kv.table[1, 2] = kv.k.shape[0] + 7
     t = gu.torch()
     q = dev(rng.standard_normal((3, 2, 64)).astype(np.float32))
     b = int8.Kv8Batch(dev(kv.table), dev(np.arange(4, dtype=np.int32)), dev(np.array([64, 64, 65], np.int32)), 1, 64)
+    if many:  # three sequences of one token in a launch for up to 60
+        q = dev(rng.standard_normal((60, 2, 64)).astype(np.float32))
+        b = int8.Kv8Batch(dev(kv.table), dev(np.arange(4, dtype=np.int32)), dev(np.array([64, 64, 65], np.int32)), 60, 64)
     out = t.full(q.shape, 7.0, device="cuda:0")
     ws = t.empty(int8.kv8_attention_workspace(kv.cache, b, q) + 256, dtype=t.uint8, device="cuda:0")
     int8.kv8_attention(kv.cache, b, q, out, workspace=ws, err=kv.err)
