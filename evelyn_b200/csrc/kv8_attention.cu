@@ -458,11 +458,12 @@ struct Role {  // per (HD, TERMS): row tiles, positions per step, stages of f16 
     uint32_t rt, np, stages, raw;
 };
 __host__ __device__ constexpr Role role_of(int hd, int terms) {
-    return hd == 256 ? (terms == 2 ? Role{1, 32, 2, 2} : Role{1, 64, 2, 1}) : terms == 2 ? Role{1, 64, 2, 4} : Role{2, 64, 2, 4};
+    return hd == 256 ? (terms == 2 ? Role{1, 32, 2, 1} : Role{1, 32, 3, 3}) : terms == 2 ? Role{1, 64, 2, 4} : Role{2, 64, 2, 4};
 }
 __host__ __device__ constexpr uint32_t tile_smem(int hd, int terms) {
     return role_of(hd, terms).rt * terms * kTileRows * hd * 2 +
-           role_of(hd, terms).np * hd * (4 * role_of(hd, terms).stages + 2 * role_of(hd, terms).raw) + 1024;
+           role_of(hd, terms).np * hd * (4 * role_of(hd, terms).stages + 2 * role_of(hd, terms).raw) +
+           role_of(hd, terms).raw * role_of(hd, terms).np * (hd / 4 + 1) + 1024;
 }
 static_assert(tile_smem(256, 2) <= 232448 && tile_smem(256, 1) <= 232448 && tile_smem(128, 1) <= 232448, "shared memory");
 
@@ -492,6 +493,12 @@ __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
                  : "memory");
+}
+// one lane of a converged warp, in the form that tells the compiler so
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(p));
+    return p != 0;
 }
 // shared-memory operand, 128-byte swizzle. lbo: bytes between 64-element panels (MN-major), sbo: between 8-row groups
 __device__ __forceinline__ uint64_t swizzled_desc(uint32_t addr, uint32_t lbo) {
@@ -556,11 +563,6 @@ __device__ __forceinline__ void codes_to_panel(uint8_t* panel, uint32_t rows, ui
     *reinterpret_cast<uint4*>(panel + panel_at(rows, r, 2 * c + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
 }
 
-__device__ __forceinline__ void producers_sync() {
-    __syncwarp();
-    asm volatile("barrier.cta.sync 1, 128;" ::: "memory");
-}
-
 template <class T, int HD>
 __global__ void __launch_bounds__(32 * (4 * role_of(HD, sizeof(T) == 4 ? 2 : 1).rt + 5), 1)
     kv8_tile_kernel(const __grid_constant__ Plan P) {
@@ -571,8 +573,11 @@ __global__ void __launch_bounds__(32 * (4 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
     constexpr uint32_t kKv = NP * HD * 2;             // K (or V) of a stage
     constexpr uint32_t kSoftWarps = 4 * RT, kTileCols = RT == 2 ? 256 : 512;  // tensor memory columns per row tile
     extern __shared__ uint8_t raw_smem[];
-    __shared__ __align__(8) uint64_t kv_full[ST], kv_empty[ST], s_full[RT][2], p_full[RT][2], o_done[RT], q_full, fin;
-    __shared__ float raw_sk[RAW][NB], raw_sv[RAW][NB], f_sk[ST][NB], f_e[ST][NB], f_down[ST][NB], f_mant[ST][NB];
+    constexpr uint32_t FS = ST + 2;  // steps of block factors
+    // (a slot comes back when the scores of the step 2 after it are done: its own weights are then done)
+    __shared__ __align__(8) uint64_t k_full[ST], k_empty[ST], v_full[ST], v_empty[ST], f_full[FS];
+    __shared__ __align__(8) uint64_t s_full[RT][2], p_full[RT][2], o_done[RT], q_full, fin;
+    __shared__ float f_sk[FS][NB], f_e[FS][NB], f_down[FS][NB], f_mant[FS][NB];
     __shared__ uint32_t tmem_base;
     __shared__ volatile int abort_flag;
     const Kv8AttnArgs& a = P.a;
@@ -597,12 +602,17 @@ __global__ void __launch_bounds__(32 * (4 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
     uint8_t* sq = smem;                                  // [RT][TERMS] q panels
     uint8_t* skv = smem + RT * TERMS * kQPart;           // [ST][K | V] f16 panels
     uint8_t* sraw = skv + ST * 2 * kKv;                  // [RAW][K | V] codes, 16 bytes per thread and piece
+    float* raw_sv = reinterpret_cast<float*>(sraw + RAW * 2 * NP * HD);  // [RAW][piece][thread] value scales
+    float* raw_f = raw_sv + RAW * NP * HD / 16;                          // [RAW][block][K, V] scales
     if (tid == 0) {
         abort_flag = 0;
         for (uint32_t i = 0; i < ST; ++i) {
-            mbar_init(&kv_full[i], 4);
-            mbar_init(&kv_empty[i], 1);
+            mbar_init(&k_full[i], 4);
+            mbar_init(&k_empty[i], 1);
+            mbar_init(&v_full[i], 4);
+            mbar_init(&v_empty[i], 1);
         }
+        for (uint32_t i = 0; i < FS; ++i) mbar_init(&f_full[i], 1);
         for (uint32_t i = 0; i < RT; ++i) {
             mbar_init(&s_full[i][0], 1);
             mbar_init(&s_full[i][1], 1);
@@ -678,8 +688,8 @@ __global__ void __launch_bounds__(32 * (4 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
         float M = kNegBig, l = 0.f;
         bool ok = true;
         for (uint32_t j = 0; j < steps && ok; ++j) {
-            const uint32_t st = j % ST;
-            ok = bwait(&kv_full[st], (j / ST) & 1, &abort_flag) && bwait(&s_full[rt][j & 1], (j >> 1) & 1, &abort_flag);
+            const uint32_t st = j % FS;
+            ok = bwait(&f_full[st], (j / FS) & 1, &abort_flag) && bwait(&s_full[rt][j & 1], (j >> 1) & 1, &abort_flag);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_after();
@@ -769,6 +779,9 @@ __global__ void __launch_bounds__(32 * (4 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
             __syncwarp();
             if (lane == 0) mbar_arrive(&p_full[rt][j & 1]);
         }
+        // (one phase after the other: a parity says nothing about a phase two steps away. Inside the loop
+        // the scores of step j imply the product of step j - 2)
+        if (steps > 1 && ok) ok = __all_sync(0xffffffffu, bwait(&o_done[rt], (steps - 2) & 1, &abort_flag));
         if (steps && ok) ok = __all_sync(0xffffffffu, bwait(&o_done[rt], (steps - 1) & 1, &abort_flag));
         tc_after();
         if (ok) {
@@ -813,43 +826,51 @@ __global__ void __launch_bounds__(32 * (4 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
         const uint32_t pt = tid - 32 * kSoftWarps;  // 0..127
         constexpr uint32_t CPR = HD / 16, N = NP * CPR / 128;  // 16-code pieces per row, per thread and operand
         const int32_t* table = a.b.table + (uint64_t)s * a.b.table_stride;
-        const uint32_t bpp = a.c.page_size / 16;
+        const uint32_t lb = 31 - __clz(a.c.page_size / 16);  // log2 of the blocks of a page: 0, 1 or 2
         auto page_of = [&](int32_t blk) {
             if (blk >= b1) return -1;
-            const int32_t p = __ldg(table + (uint32_t)blk / bpp);
+            const int32_t p = __ldg(table + ((uint32_t)blk >> lb));
             if (p >= 0 && (uint32_t)p < a.c.n_pages) return p;
             flag_error(a.err, DEV_ERR_POSITION);
             return -1;
         };
         // Codes travel ahead in a ring of their own: every thread copies the pieces that it will
-        // widen itself (asynchronously, RAW steps ahead), the scales are copied beside them.
-        // RAW + 1 steps ahead the page of each of the thread's pieces is looked up.
-        uint32_t page[N];
-        constexpr uint32_t kNone = 0xffffffffu;
+        // widen itself, and the scales that it will need, RAW steps ahead and asynchronously, so the
+        // producers never wait for one another. RAW + 1 steps ahead the page of each of the
+        // thread's pieces is looked up.
+        int32_t page[N], fpage = -1;  // fpage: of block pt of the step, for its factors
         auto pages = [&](uint32_t j) {
 #pragma unroll
-            for (uint32_t i = 0; i < N; ++i) page[i] = (uint32_t)page_of(b0 + (int32_t)(j * NB + (pt + 128 * i) / CPR / 16));
+            for (uint32_t i = 0; i < N; ++i) page[i] = page_of(b0 + (int32_t)(j * NB + (pt + 128 * i) / CPR / 16));
+            if (pt < NB) fpage = page_of(b0 + (int32_t)(j * NB + pt));
         };
-        uint32_t gone = 0;  // bits: this thread's pieces of step j % RAW without a page
+        uint32_t gone = 0;  // bits: this thread's pieces (and factors) of step j % RAW without a page
+        auto scale_at = [&](int32_t pg, uint32_t sub) { return (uint64_t)pg * a.c.scale_stride + (h << lb) + sub; };
         auto fetch = [&](uint32_t j) {
-            uint8_t* raw = sraw + (j % RAW) * (2 * NP * HD);
+            const uint32_t rs = j % RAW;
+            uint8_t* raw = sraw + rs * (2 * NP * HD);
+            gone &= ~(((2u << N) - 1) << (rs * (N + 1)));
 #pragma unroll
             for (uint32_t i = 0; i < N; ++i) {
                 const uint32_t piece = pt + 128 * i, r = piece / CPR, c = piece % CPR;
-                const uint32_t sub = (uint32_t)(b0 + (int32_t)(j * NB + r / 16)) % bpp;
-                const uint32_t bit = 1u << (j % RAW * N + i);
-                gone = page[i] == kNone ? gone | bit : gone & ~bit;
-                if (page[i] != kNone) {
-                    const uint64_t at = (uint64_t)page[i] * a.c.page_stride + ((uint64_t)h * a.c.page_size + sub * 16 + r % 16) * HD + 16 * c;
+                const uint32_t sub = (uint32_t)(b0 + (int32_t)(j * NB + r / 16)) & ((1u << lb) - 1);
+                if (page[i] >= 0) {
+                    const uint64_t at = (uint64_t)page[i] * a.c.page_stride +
+                                        (uint64_t)(h * a.c.page_size + sub * 16 + r % 16) * HD + 16 * c;
                     cp_async16(raw + 16 * piece, a.c.k + at);
                     cp_async16(raw + NP * HD + 16 * piece, a.c.v + at);
-                    if (c == 0 && r % 16 == 0) {
-                        const uint64_t sc = (uint64_t)page[i] * a.c.scale_stride + h * bpp + sub;
-                        cp_async4(&raw_sk[j % RAW][r / 16], a.c.ks + sc);
-                        cp_async4(&raw_sv[j % RAW][r / 16], a.c.vs + sc);
-                    }
-                } else if (c == 0 && r % 16 == 0) {
-                    raw_sk[j % RAW][r / 16] = __uint_as_float(0xff800000u);  // -infinity: hidden
+                    cp_async4(&raw_sv[(rs * N + i) * 128 + pt], a.c.vs + scale_at(page[i], sub));
+                } else {
+                    gone |= 1u << (rs * (N + 1) + i);
+                }
+            }
+            if (pt < NB) {
+                const uint32_t sub = (uint32_t)(b0 + (int32_t)(j * NB + pt)) & ((1u << lb) - 1);
+                if (fpage >= 0) {
+                    cp_async4(&raw_f[(rs * NB + pt) * 2], a.c.ks + scale_at(fpage, sub));
+                    cp_async4(&raw_f[(rs * NB + pt) * 2 + 1], a.c.vs + scale_at(fpage, sub));
+                } else {
+                    gone |= 1u << (rs * (N + 1) + N);
                 }
             }
         };
@@ -862,59 +883,73 @@ __global__ void __launch_bounds__(32 * (4 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
             }
             cp_async_commit();
         }
-        for (uint32_t j = 0; j < steps; ++j) {
-            const uint32_t st = j % ST, rs = j % RAW;
+        for (uint32_t j = 0; j < steps; ++j) {  // (after an abort the loop runs out quickly: every wait gives up at once)
+            const uint32_t st = j % ST, rs = j % RAW, fs = j % FS;
             cp_async_wait<(int)RAW - 1>();
-            producers_sync();  // everyone's scales of this step
-            if (j >= ST && !__all_sync(0xffffffffu, bwait(&kv_empty[st], (j / ST - 1) & 1, &abort_flag))) abort_flag = 1;
             const uint8_t* raw = sraw + rs * (2 * NP * HD);
             uint8_t* dst = skv + st * 2 * kKv;
-#pragma unroll
-            for (uint32_t i = 0; i < N; ++i) {
-                const uint32_t piece = pt + 128 * i, r = piece / CPR, c = piece % CPR;
-                const bool none = gone >> (rs * N + i) & 1;
-                const uint4 k = *reinterpret_cast<const uint4*>(raw + 16 * piece);
-                const uint4 v = *reinterpret_cast<const uint4*>(raw + NP * HD + 16 * piece);
-                codes_to_panel(dst, NP, r, c, k, none);
-                // codes under a scale of 0 (or below the normal numbers) stand for 0
-                codes_to_panel(dst + kKv, NP, r, c, v, none || abs_bits(raw_sv[rs][r / 16]) < 0x00800000u);
-            }
+            if (j >= ST) bwait(&k_empty[st], (j / ST - 1) & 1, &abort_flag);
             if (pt < NB) {
-                const float sk = raw_sk[rs][pt], sv = raw_sv[rs][pt];
+                const bool hidden = gone >> (rs * (N + 1) + N) & 1;
+                const float sk = raw_f[(rs * NB + pt) * 2], sv = raw_f[(rs * NB + pt) * 2 + 1];
                 const uint32_t sb = __float_as_uint(sv);
                 const int eb = (int)((sb >> 23) & 0xffu);
-                const bool plain = eb > 0 && eb < 255, bad = eb == 255, hidden = sk == -INFINITY;
-                f_sk[st][pt] = hidden ? 0.f : sk;
+                const bool plain = eb > 0 && eb < 255, bad = eb == 255;
+                f_sk[fs][pt] = hidden ? 0.f : sk;
                 if (TERMS == 2) {
-                    f_mant[st][pt] = plain ? __uint_as_float((sb & 0x807fffffu) | 0x3f800000u) : 1.f;
-                    f_down[st][pt] = plain ? __uint_as_float((uint32_t)(254 - eb) << 23) : kZeroDown;
-                    f_e[st][pt] = hidden ? -INFINITY : plain ? (float)(eb - 127) : bad ? __uint_as_float(0x7fc00000u) : kZeroExp;
+                    f_mant[fs][pt] = plain ? __uint_as_float((sb & 0x807fffffu) | 0x3f800000u) : 1.f;
+                    f_down[fs][pt] = plain ? __uint_as_float((uint32_t)(254 - eb) << 23) : kZeroDown;
+                    f_e[fs][pt] = hidden ? -INFINITY : plain ? (float)(eb - 127) : bad ? __uint_as_float(0x7fc00000u) : kZeroExp;
                 } else {
-                    f_down[st][pt] = plain ? __fdiv_rn(1.f, sv) : kZeroDown;
-                    f_e[st][pt] = hidden ? -INFINITY : plain ? log2f(sv) : bad ? __uint_as_float(0x7fc00000u) : kZeroExp;
+                    f_down[fs][pt] = plain ? __fdiv_rn(1.f, sv) : kZeroDown;
+                    f_e[fs][pt] = hidden ? -INFINITY : plain ? log2f(sv) : bad ? __uint_as_float(0x7fc00000u) : kZeroExp;
                 }
             }
+#pragma unroll
+            for (uint32_t i = 0; i < N; ++i) {
+                const uint32_t piece = pt + 128 * i;
+                codes_to_panel(dst, NP, piece / CPR, piece % CPR, *reinterpret_cast<const uint4*>(raw + 16 * piece),
+                               gone >> (rs * (N + 1) + i) & 1);
+            }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            producers_sync();  // everyone's reads of this step's codes and scales
-            if (lane == 0) mbar_arrive(&kv_full[st]);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&k_full[st]);
+            if (pt == 0) mbar_arrive(&f_full[fs]);
+            if (j >= ST) bwait(&v_empty[st], (j / ST - 1) & 1, &abort_flag);
+#pragma unroll
+            for (uint32_t i = 0; i < N; ++i) {
+                const uint32_t piece = pt + 128 * i;
+                // codes under a scale of 0 (or below the normal numbers) stand for 0
+                const bool none = (gone >> (rs * (N + 1) + i) & 1) || abs_bits(raw_sv[(rs * N + i) * 128 + pt]) < 0x00800000u;
+                codes_to_panel(dst + kKv, NP, piece / CPR, piece % CPR,
+                               *reinterpret_cast<const uint4*>(raw + NP * HD + 16 * piece), none);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&v_full[st]);
             if (j + RAW < steps) {
                 fetch(j + RAW);
                 pages(j + RAW + 1);
             }
-            cp_async_commit();  // (after an abort the loop runs out quickly: every wait gives up at once)
+            cp_async_commit();
         }
         cp_async_wait<0>();
-    } else if (lane == 0 && steps) {
+    } else if (steps && elect_one()) {
         // ---------------------------------------------------------------- MMA
         bool ok = bwait(&q_full, 0, &abort_flag);
         auto scores = [&](uint32_t j) {
             const uint32_t st = j % ST;
-            ok = ok && bwait(&kv_full[st], (j / ST) & 1, &abort_flag);
+            ok = ok && bwait(&k_full[st], (j / ST) & 1, &abort_flag);
             if (!ok) return;
             tc_after();
             const uint32_t kb = smem_addr(skv + st * 2 * kKv);
 #pragma unroll
             for (uint32_t t = 0; t < RT; ++t) {
+                // the buffer holds the weights of step j - 2 until their product has ended (products of
+                // different shapes are not ordered by their issue)
+                ok = ok && (j < 2 || bwait(&o_done[t], (j - 2) & 1, &abort_flag));
+                if (!ok) return;
+                tc_after();
                 const uint32_t d = tm + t * kTileCols + HD + (j & 1) * NP;
                 const uint32_t qb = smem_addr(sq + t * TERMS * kQPart);
 #pragma unroll
@@ -925,11 +960,13 @@ __global__ void __launch_bounds__(32 * (4 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
                                swizzled_desc(kb + (k / 4) * (NP * 128) + (k % 4) * 32, 16), f16_idesc(NP, false), x > 0 || k > 0);
                 mma_commit(&s_full[t][j & 1]);
             }
+            mma_commit(&k_empty[st]);
         };
         scores(0);
         for (uint32_t j = 0; j < steps && ok; ++j) {
             if (j + 1 < steps) scores(j + 1);
             const uint32_t st = j % ST, vb = smem_addr(skv + st * 2 * kKv + kKv);
+            ok = ok && bwait(&v_full[st], (j / ST) & 1, &abort_flag);
 #pragma unroll
             for (uint32_t t = 0; t < RT; ++t) {
                 ok = ok && bwait(&p_full[t][j & 1], (j >> 1) & 1, &abort_flag);
@@ -944,7 +981,7 @@ __global__ void __launch_bounds__(32 * (4 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
                                j > 0 || x > 0 || k > 0);
                 mma_commit(&o_done[t]);
             }
-            if (ok) mma_commit(&kv_empty[st]);
+            if (ok) mma_commit(&v_empty[st]);
         }
         if (!ok) {  // the MMAs in flight end before the tensor memory is freed
             mma_commit(&fin);
