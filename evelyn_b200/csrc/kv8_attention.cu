@@ -437,6 +437,7 @@ template <class T, int HD> __global__ void __launch_bounds__(128) kv8_join_kerne
 // ------------------------------------------------------------------ prompts
 // kv8_tile_kernel: many rows per kv head, on the 5th-generation tensor cores. A CTA takes RT row
 // tiles of 128 rows (token, head) of one (sequence, kv head) and walks the positions NP at a time:
+//   1 factor warp     the blocks' scales, and what follows from them, into a small ring;
 //   4 producer warps  codes to f16 (exact) into a ring of shared-memory stages, K and V alike:
 //                     64 dims x NP positions per 128-byte-swizzled panel. The score product reads
 //                     them K-major, the value product MN-major, so no transpose is made;
@@ -458,20 +459,16 @@ struct Role {  // per (HD, TERMS): row tiles, positions per step, stages of f16 
     uint32_t rt, np, stages, raw;
 };
 __host__ __device__ constexpr Role role_of(int hd, int terms) {
-    return hd == 256 ? (terms == 2 ? Role{1, 32, 2, 1} : Role{1, 32, 3, 3}) : terms == 2 ? Role{1, 64, 2, 4} : Role{2, 64, 2, 4};
+    return hd == 256 ? (terms == 2 ? Role{1, 32, 2, 2} : Role{1, 32, 3, 3}) : terms == 2 ? Role{1, 64, 2, 4} : Role{2, 64, 2, 4};
 }
 __host__ __device__ constexpr uint32_t tile_smem(int hd, int terms) {
     return role_of(hd, terms).rt * terms * kTileRows * hd * 2 +
-           role_of(hd, terms).np * hd * (4 * role_of(hd, terms).stages + 2 * role_of(hd, terms).raw) +
-           role_of(hd, terms).raw * role_of(hd, terms).np * (hd / 4 + 1) + 1024;
+           role_of(hd, terms).np * hd * (4 * role_of(hd, terms).stages + 2 * role_of(hd, terms).raw) + 1024;
 }
 static_assert(tile_smem(256, 2) <= 232448 && tile_smem(256, 1) <= 232448 && tile_smem(128, 1) <= 232448, "shared memory");
 
 __device__ __forceinline__ void cp_async16(void* dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(dst)), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async4(void* dst, const void* src) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_addr(dst)), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -564,7 +561,7 @@ __device__ __forceinline__ void codes_to_panel(uint8_t* panel, uint32_t rows, ui
 }
 
 template <class T, int HD>
-__global__ void __launch_bounds__(32 * (4 * role_of(HD, sizeof(T) == 4 ? 2 : 1).rt + 5), 1)
+__global__ void __launch_bounds__(32 * (4 * role_of(HD, sizeof(T) == 4 ? 2 : 1).rt + 6), 1)
     kv8_tile_kernel(const __grid_constant__ Plan P) {
     constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
     constexpr Role R = role_of(HD, TERMS);
@@ -573,11 +570,10 @@ __global__ void __launch_bounds__(32 * (4 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
     constexpr uint32_t kKv = NP * HD * 2;             // K (or V) of a stage
     constexpr uint32_t kSoftWarps = 4 * RT, kTileCols = RT == 2 ? 256 : 512;  // tensor memory columns per row tile
     extern __shared__ uint8_t raw_smem[];
-    constexpr uint32_t FS = ST + 2;  // steps of block factors
-    // (a slot comes back when the scores of the step 2 after it are done: its own weights are then done)
-    __shared__ __align__(8) uint64_t k_full[ST], k_empty[ST], v_full[ST], v_empty[ST], f_full[FS];
+    constexpr uint32_t FS = 8;  // steps of block factors
+    __shared__ __align__(8) uint64_t k_full[ST], k_empty[ST], v_full[ST], v_empty[ST], f_full[FS], f_empty[FS];
     __shared__ __align__(8) uint64_t s_full[RT][2], p_full[RT][2], o_done[RT], q_full, fin;
-    __shared__ float f_sk[FS][NB], f_e[FS][NB], f_down[FS][NB], f_mant[FS][NB];
+    __shared__ float4 f_blk[FS][NB];  // key scale, exponent of the value scale, 2^-exponent, mantissa
     __shared__ uint32_t tmem_base;
     __shared__ volatile int abort_flag;
     const Kv8AttnArgs& a = P.a;
@@ -602,8 +598,6 @@ __global__ void __launch_bounds__(32 * (4 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
     uint8_t* sq = smem;                                  // [RT][TERMS] q panels
     uint8_t* skv = smem + RT * TERMS * kQPart;           // [ST][K | V] f16 panels
     uint8_t* sraw = skv + ST * 2 * kKv;                  // [RAW][K | V] codes, 16 bytes per thread and piece
-    float* raw_sv = reinterpret_cast<float*>(sraw + RAW * 2 * NP * HD);  // [RAW][piece][thread] value scales
-    float* raw_f = raw_sv + RAW * NP * HD / 16;                          // [RAW][block][K, V] scales
     if (tid == 0) {
         abort_flag = 0;
         for (uint32_t i = 0; i < ST; ++i) {
@@ -612,7 +606,10 @@ __global__ void __launch_bounds__(32 * (4 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
             mbar_init(&v_full[i], 4);
             mbar_init(&v_empty[i], 1);
         }
-        for (uint32_t i = 0; i < FS; ++i) mbar_init(&f_full[i], 1);
+        for (uint32_t i = 0; i < FS; ++i) {
+            mbar_init(&f_full[i], 1);
+            mbar_init(&f_empty[i], kSoftWarps);
+        }
         for (uint32_t i = 0; i < RT; ++i) {
             mbar_init(&s_full[i][0], 1);
             mbar_init(&s_full[i][1], 1);
@@ -706,11 +703,12 @@ __global__ void __launch_bounds__(32 * (4 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
                     if (p0 + (int32_t)i > last) v[i] = 0xff800000u;  // -infinity
             }
             // the largest score: of each block's products, then by the block's factor (not negative)
-            float mx = -INFINITY, f[NB], e[NB];
+            float mx = -INFINITY, f[NB], e[NB], down[NB], mant[NB];
 #pragma unroll
             for (uint32_t b = 0; b < NB; ++b) {
-                f[b] = step * f_sk[st][b];
-                e[b] = f_e[st][b];
+                const float4 w = f_blk[st][b];
+                f[b] = step * w.x;
+                e[b] = w.y, down[b] = w.z, mant[b] = w.w;
                 float m = __uint_as_float(v[16 * b]);
 #pragma unroll
                 for (uint32_t i = 1; i < 16; ++i) m = fmaxf(m, __uint_as_float(v[16 * b + i]));
@@ -738,18 +736,18 @@ __global__ void __launch_bounds__(32 * (4 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
             }
             bool far = false;
 #pragma unroll
-            for (uint32_t b = 0; b < NB; ++b) far |= e[b] < M - kFar && e[b] != -INFINITY;
+            for (uint32_t b = 0; b < NB; ++b) far |= (e[b] < M - kFar && e[b] != -INFINITY) || mant[b] == 0.f;
             auto weights = [&](auto rare) {  // rare: hidden positions, or a block far below the maximum
                 constexpr bool RARE = decltype(rare)::value;
 #pragma unroll
                 for (uint32_t b = 0; b < NB; ++b) {
                     float sum = 0.f;
                     uint32_t hi[8], lo[8];
-                    float mant = TERMS == 2 ? f_mant[st][b] : 1.f, off = e[b] - M, down = f_down[st][b];
+                    float off = e[b] - M, mt = mant[b], dn = down[b];
                     if (RARE && off < -kFar && off != -INFINITY) {
                         float f;
                         off += aside(e[b], M, f);
-                        mant *= f, down *= f;
+                        mt *= f, dn *= f;
                     }
 #pragma unroll
                     for (uint32_t i = 0; i < 8; ++i) {
@@ -760,14 +758,14 @@ __global__ void __launch_bounds__(32 * (4 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
                             w1 = x1 == -INFINITY ? 0.f : w1;
                         }
                         sum += w0 + w1;
-                        if (TERMS == 2 || RARE) w0 *= mant, w1 *= mant;
+                        if (TERMS == 2 || RARE) w0 *= mt, w1 *= mt;
                         hi[i] = pack_h2(w0, w1);
                         if (TERMS == 2) {
                             const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi[i]));
                             lo[i] = pack_h2(w0 - back.x, w1 - back.y);
                         }
                     }
-                    l = fmaf(sum, down, l);
+                    l = fmaf(sum, dn, l);
                     tmem_st8(ts + 8 * b, hi);
                     if (TERMS == 2) tmem_st8(ts + NP / 2 + 8 * b, lo);
                 }
@@ -777,7 +775,10 @@ __global__ void __launch_bounds__(32 * (4 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
             tmem_st_wait();
             tc_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[rt][j & 1]);
+            if (lane == 0) {
+                mbar_arrive(&p_full[rt][j & 1]);
+                mbar_arrive(&f_empty[st]);
+            }
         }
         // (one phase after the other: a parity says nothing about a phase two steps away. Inside the loop
         // the scores of step j imply the product of step j - 2)
@@ -827,50 +828,38 @@ __global__ void __launch_bounds__(32 * (4 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
         constexpr uint32_t CPR = HD / 16, N = NP * CPR / 128;  // 16-code pieces per row, per thread and operand
         const int32_t* table = a.b.table + (uint64_t)s * a.b.table_stride;
         const uint32_t lb = 31 - __clz(a.c.page_size / 16);  // log2 of the blocks of a page: 0, 1 or 2
-        auto page_of = [&](int32_t blk) {
-            if (blk >= b1) return -1;
-            const int32_t p = __ldg(table + ((uint32_t)blk >> lb));
-            if (p >= 0 && (uint32_t)p < a.c.n_pages) return p;
-            flag_error(a.err, DEV_ERR_POSITION);
-            return -1;
-        };
         // Codes travel ahead in a ring of their own: every thread copies the pieces that it will
-        // widen itself, and the scales that it will need, RAW steps ahead and asynchronously, so the
-        // producers never wait for one another. RAW + 1 steps ahead the page of each of the
-        // thread's pieces is looked up.
-        int32_t page[N], fpage = -1;  // fpage: of block pt of the step, for its factors
+        // widen itself, RAW steps ahead and asynchronously, so the producers never wait for one
+        // another. RAW + 1 steps ahead the page of each of the thread's pieces is looked up.
+        int32_t page[N];
+        uint64_t at[N];  // of the piece inside its page, for the first block of the page
+#pragma unroll
+        for (uint32_t i = 0; i < N; ++i) {
+            const uint32_t piece = pt + 128 * i, r = piece / CPR;
+            at[i] = (uint64_t)(h * a.c.page_size + r % 16) * HD + 16 * (piece % CPR);
+        }
         auto pages = [&](uint32_t j) {
 #pragma unroll
-            for (uint32_t i = 0; i < N; ++i) page[i] = page_of(b0 + (int32_t)(j * NB + (pt + 128 * i) / CPR / 16));
-            if (pt < NB) fpage = page_of(b0 + (int32_t)(j * NB + pt));
+            for (uint32_t i = 0; i < N; ++i) {
+                const int32_t blk = b0 + (int32_t)(j * NB + (pt + 128 * i) / CPR / 16);
+                page[i] = blk < b1 ? __ldg(table + ((uint32_t)blk >> lb)) : -1;
+            }
         };
-        uint32_t gone = 0;  // bits: this thread's pieces (and factors) of step j % RAW without a page
-        auto scale_at = [&](int32_t pg, uint32_t sub) { return (uint64_t)pg * a.c.scale_stride + (h << lb) + sub; };
+        uint32_t gone = 0;  // bits: this thread's pieces of step j % RAW that have no (valid) page
         auto fetch = [&](uint32_t j) {
             const uint32_t rs = j % RAW;
             uint8_t* raw = sraw + rs * (2 * NP * HD);
-            gone &= ~(((2u << N) - 1) << (rs * (N + 1)));
+            gone &= ~(((1u << N) - 1) << (rs * N));
 #pragma unroll
             for (uint32_t i = 0; i < N; ++i) {
-                const uint32_t piece = pt + 128 * i, r = piece / CPR, c = piece % CPR;
-                const uint32_t sub = (uint32_t)(b0 + (int32_t)(j * NB + r / 16)) & ((1u << lb) - 1);
-                if (page[i] >= 0) {
-                    const uint64_t at = (uint64_t)page[i] * a.c.page_stride +
-                                        (uint64_t)(h * a.c.page_size + sub * 16 + r % 16) * HD + 16 * c;
-                    cp_async16(raw + 16 * piece, a.c.k + at);
-                    cp_async16(raw + NP * HD + 16 * piece, a.c.v + at);
-                    cp_async4(&raw_sv[(rs * N + i) * 128 + pt], a.c.vs + scale_at(page[i], sub));
+                const uint32_t piece = pt + 128 * i;
+                const uint32_t sub = (uint32_t)(b0 + (int32_t)(j * NB + piece / CPR / 16)) & ((1u << lb) - 1);
+                if ((uint32_t)page[i] < a.c.n_pages) {
+                    const uint64_t o = (uint32_t)page[i] * a.c.page_stride + at[i] + sub * (16 * HD);
+                    cp_async16(raw + 16 * piece, a.c.k + o);
+                    cp_async16(raw + NP * HD + 16 * piece, a.c.v + o);
                 } else {
-                    gone |= 1u << (rs * (N + 1) + i);
-                }
-            }
-            if (pt < NB) {
-                const uint32_t sub = (uint32_t)(b0 + (int32_t)(j * NB + pt)) & ((1u << lb) - 1);
-                if (fpage >= 0) {
-                    cp_async4(&raw_f[(rs * NB + pt) * 2], a.c.ks + scale_at(fpage, sub));
-                    cp_async4(&raw_f[(rs * NB + pt) * 2 + 1], a.c.vs + scale_at(fpage, sub));
-                } else {
-                    gone |= 1u << (rs * (N + 1) + N);
+                    gone |= 1u << (rs * N + i);
                 }
             }
         };
@@ -883,49 +872,28 @@ __global__ void __launch_bounds__(32 * (4 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
             }
             cp_async_commit();
         }
+        auto widen = [&](uint8_t* panel, const uint8_t* raw, uint32_t none) {
+            uint4 w[N];
+#pragma unroll
+            for (uint32_t i = 0; i < N; ++i) w[i] = *reinterpret_cast<const uint4*>(raw + 16 * (pt + 128 * i));
+#pragma unroll
+            for (uint32_t i = 0; i < N; ++i) {
+                const uint32_t piece = pt + 128 * i;
+                codes_to_panel(panel, NP, piece / CPR, piece % CPR, w[i], none >> i & 1);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+        };
         for (uint32_t j = 0; j < steps; ++j) {  // (after an abort the loop runs out quickly: every wait gives up at once)
-            const uint32_t st = j % ST, rs = j % RAW, fs = j % FS;
+            const uint32_t st = j % ST, rs = j % RAW, none = gone >> (rs * N);
             cp_async_wait<(int)RAW - 1>();
             const uint8_t* raw = sraw + rs * (2 * NP * HD);
             uint8_t* dst = skv + st * 2 * kKv;
             if (j >= ST) bwait(&k_empty[st], (j / ST - 1) & 1, &abort_flag);
-            if (pt < NB) {
-                const bool hidden = gone >> (rs * (N + 1) + N) & 1;
-                const float sk = raw_f[(rs * NB + pt) * 2], sv = raw_f[(rs * NB + pt) * 2 + 1];
-                const uint32_t sb = __float_as_uint(sv);
-                const int eb = (int)((sb >> 23) & 0xffu);
-                const bool plain = eb > 0 && eb < 255, bad = eb == 255;
-                f_sk[fs][pt] = hidden ? 0.f : sk;
-                if (TERMS == 2) {
-                    f_mant[fs][pt] = plain ? __uint_as_float((sb & 0x807fffffu) | 0x3f800000u) : 1.f;
-                    f_down[fs][pt] = plain ? __uint_as_float((uint32_t)(254 - eb) << 23) : kZeroDown;
-                    f_e[fs][pt] = hidden ? -INFINITY : plain ? (float)(eb - 127) : bad ? __uint_as_float(0x7fc00000u) : kZeroExp;
-                } else {
-                    f_down[fs][pt] = plain ? __fdiv_rn(1.f, sv) : kZeroDown;
-                    f_e[fs][pt] = hidden ? -INFINITY : plain ? log2f(sv) : bad ? __uint_as_float(0x7fc00000u) : kZeroExp;
-                }
-            }
-#pragma unroll
-            for (uint32_t i = 0; i < N; ++i) {
-                const uint32_t piece = pt + 128 * i;
-                codes_to_panel(dst, NP, piece / CPR, piece % CPR, *reinterpret_cast<const uint4*>(raw + 16 * piece),
-                               gone >> (rs * (N + 1) + i) & 1);
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
+            widen(dst, raw, none);
             if (lane == 0) mbar_arrive(&k_full[st]);
-            if (pt == 0) mbar_arrive(&f_full[fs]);
             if (j >= ST) bwait(&v_empty[st], (j / ST - 1) & 1, &abort_flag);
-#pragma unroll
-            for (uint32_t i = 0; i < N; ++i) {
-                const uint32_t piece = pt + 128 * i;
-                // codes under a scale of 0 (or below the normal numbers) stand for 0
-                const bool none = (gone >> (rs * (N + 1) + i) & 1) || abs_bits(raw_sv[(rs * N + i) * 128 + pt]) < 0x00800000u;
-                codes_to_panel(dst + kKv, NP, piece / CPR, piece % CPR,
-                               *reinterpret_cast<const uint4*>(raw + NP * HD + 16 * piece), none);
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
+            widen(dst + kKv, raw + NP * HD, none);
             if (lane == 0) mbar_arrive(&v_full[st]);
             if (j + RAW < steps) {
                 fetch(j + RAW);
@@ -934,7 +902,44 @@ __global__ void __launch_bounds__(32 * (4 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
             cp_async_commit();
         }
         cp_async_wait<0>();
-    } else if (steps && elect_one()) {
+    } else if (warp == kSoftWarps + 5) {
+        // ---------------------------------------------------------------- the blocks' factors
+        // one lane per block, 32 / NB steps looked up together
+        const int32_t* table = a.b.table + (uint64_t)s * a.b.table_stride;
+        const uint32_t lb = 31 - __clz(a.c.page_size / 16);
+        for (uint32_t j0 = 0; j0 < steps; j0 += 32 / NB) {
+            const int32_t blk = b0 + (int32_t)(j0 * NB + lane);
+            const int32_t page = blk < b1 ? __ldg(table + ((uint32_t)blk >> lb)) : -1;
+            const bool hidden = (uint32_t)page >= a.c.n_pages;
+            if (hidden && blk < b1) flag_error(a.err, DEV_ERR_POSITION);
+            float sk = 0.f, sv = 0.f;
+            if (!hidden) {
+                const uint64_t at = (uint32_t)page * a.c.scale_stride + (h << lb) + ((uint32_t)blk & ((1u << lb) - 1));
+                sk = __ldg(a.c.ks + at);
+                sv = __ldg(a.c.vs + at);
+            }
+            // sv = mant 2^e (TERMS = 2), or e = log2 sv; zeros have mant 0 and an exponent that no maximum
+            // notices; a scale that is not finite makes the weights of the rows that see it so
+            const uint32_t sb = __float_as_uint(sv);
+            const int eb = (int)((sb >> 23) & 0xffu);
+            const bool plain = eb > 0 && eb < 255;
+            const float mant = eb == 0 ? 0.f : TERMS == 2 && plain ? __uint_as_float((sb & 0x807fffffu) | 0x3f800000u) : 1.f;
+            const float down = !plain ? kZeroDown : TERMS == 2 ? __uint_as_float((uint32_t)(254 - eb) << 23) : __fdiv_rn(1.f, sv);
+            const float e = hidden      ? -INFINITY
+                            : eb == 255 ? __uint_as_float(0x7fc00000u)
+                            : eb == 0   ? kZeroExp
+                            : TERMS == 2 ? (float)(eb - 127)
+                                         : log2f(sv);
+            for (uint32_t i = 0; i < 32 / NB && j0 + i < steps; ++i) {
+                const uint32_t j = j0 + i, fs = j % FS;
+                if (j >= FS) bwait(&f_empty[fs], (j / FS - 1) & 1, &abort_flag);
+                __syncwarp();
+                if (lane / NB == i) f_blk[fs][lane % NB] = make_float4(sk, e, down, mant);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&f_full[fs]);
+            }
+        }
+    } else if (warp == kSoftWarps + 4 && steps && elect_one()) {
         // ---------------------------------------------------------------- MMA
         bool ok = bwait(&q_full, 0, &abort_flag);
         auto scores = [&](uint32_t j) {
@@ -1024,7 +1029,7 @@ Shape shape_of(const Kv8Cache& c, const Kv8Batch& b, uint32_t heads, uint32_t ty
 template <class T, int HD> cudaError_t launch(const Plan& p, bool tiles, cudaStream_t s) {
     if (tiles) {
         constexpr int terms = sizeof(T) == 4 ? 2 : 1;
-        constexpr uint32_t smem = tile_smem(HD, terms), threads = 32 * (4 * role_of(HD, terms).rt + 5);
+        constexpr uint32_t smem = tile_smem(HD, terms), threads = 32 * (4 * role_of(HD, terms).rt + 6);
         static std::atomic<bool> opted[64];
         int dev = 0;
         cudaError_t e = cudaGetDevice(&dev);
