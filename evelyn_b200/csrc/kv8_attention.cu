@@ -542,6 +542,37 @@ __device__ __forceinline__ void tmem_st8(uint32_t t, const uint32_t* v) {
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// two f32 operations in one instruction
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    return (uint64_t)__float_as_uint(a) | (uint64_t)__float_as_uint(b) << 32;
+}
+__device__ __forceinline__ uint64_t pack2(uint32_t a, uint32_t b) { return (uint64_t)a | (uint64_t)b << 32; }
+__device__ __forceinline__ float lo2(uint64_t v) { return __uint_as_float((uint32_t)v); }
+__device__ __forceinline__ float hi2(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// 2^x of two values on the FMA pipe, x from -126 (below: as there) up to 127: the nearest whole number
+// n goes into the exponent, 2^(x - n) is a polynomial of degree 4 fitted on [-1/2, 1/2] for the smallest
+// relative error (2.6e-6, a 50th of the f16 rounding that follows).
+__device__ __forceinline__ uint64_t exp2_poly2(uint64_t x) {
+    x = pack2(fmaxf(lo2(x), -126.f), fmaxf(hi2(x), -126.f));
+    const uint64_t n = add2(x, pack2(12582912.f, 12582912.f));  // n in the low mantissa bits
+    const uint64_t r = add2(x, fma2(add2(n, pack2(-12582912.f, -12582912.f)), pack2(-1.f, -1.f), 0ull));
+    uint64_t y = fma2(pack2(0.009570101276f, 0.009570101276f), r, pack2(0.05591785908f, 0.05591785908f));
+    y = fma2(y, r, pack2(0.2402474433f, 0.2402474433f));
+    y = fma2(y, r, pack2(0.6931217909f, 0.6931217909f));
+    y = fma2(y, r, pack2(0.9999992847f, 0.9999992847f));
+    return pack2((uint32_t)y + ((uint32_t)n << 23), (uint32_t)(y >> 32) + ((uint32_t)(n >> 32) << 23));
+}
+
 // byte offset of 16-byte piece `p` (8 f16 values) of row r in panels of `rows` rows
 __device__ __forceinline__ uint32_t panel_at(uint32_t rows, uint32_t r, uint32_t p) {
     return (p >> 3) * (rows * 128u) + r * 128u + (((p & 7u) ^ (r & 7u)) << 4);
@@ -561,7 +592,7 @@ __device__ __forceinline__ void codes_to_panel(uint8_t* panel, uint32_t rows, ui
 }
 
 template <class T, int HD>
-__global__ void __launch_bounds__(32 * (4 * role_of(HD, sizeof(T) == 4 ? 2 : 1).rt + 6), 1)
+__global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).rt + 5), 1)
     kv8_tile_kernel(const __grid_constant__ Plan P) {
     constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
     constexpr Role R = role_of(HD, TERMS);
@@ -572,7 +603,7 @@ __global__ void __launch_bounds__(32 * (4 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
     extern __shared__ uint8_t raw_smem[];
     constexpr uint32_t FS = 8;  // steps of block factors
     __shared__ __align__(8) uint64_t k_full[ST], k_empty[ST], v_full[ST], v_empty[ST], f_full[FS], f_empty[FS];
-    __shared__ __align__(8) uint64_t s_full[RT][2], p_full[RT][2], o_done[RT], q_full, fin;
+    __shared__ __align__(8) uint64_t s_full[RT][2], p_full[RT][2], o_done[RT], q_full, fin[RT];
     __shared__ float4 f_blk[FS][NB];  // key scale, exponent of the value scale, 2^-exponent, mantissa
     __shared__ uint32_t tmem_base;
     __shared__ volatile int abort_flag;
@@ -602,9 +633,9 @@ __global__ void __launch_bounds__(32 * (4 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
         abort_flag = 0;
         for (uint32_t i = 0; i < ST; ++i) {
             mbar_init(&k_full[i], 4);
-            mbar_init(&k_empty[i], 1);
+            mbar_init(&k_empty[i], RT);
             mbar_init(&v_full[i], 4);
-            mbar_init(&v_empty[i], 1);
+            mbar_init(&v_empty[i], RT);
         }
         for (uint32_t i = 0; i < FS; ++i) {
             mbar_init(&f_full[i], 1);
@@ -617,9 +648,9 @@ __global__ void __launch_bounds__(32 * (4 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
             mbar_init(&p_full[i][0], 4);
             mbar_init(&p_full[i][1], 4);
             mbar_init(&o_done[i], 1);
+            mbar_init(&fin[i], 1);
         }
         mbar_init(&q_full, kSoftWarps);
-        mbar_init(&fin, 1);
         fence_barrier_init();
     }
     if (warp == kSoftWarps + 4) {
@@ -691,24 +722,72 @@ __global__ void __launch_bounds__(32 * (4 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
             if (!ok) break;
             tc_after();
             const uint32_t ts = to + HD + (j & 1) * NP;
+            const int32_t p0 = (b0 + (int32_t)(j * NB)) * 16;
+            const bool masked = __any_sync(0xffffffffu, p0 + (int32_t)NP - 1 > open || !live);
+            float f[NB], e[NB], down[NB], mant[NB];
+            bool far = false;  // a block far below the maximum, or one of zeros
+#pragma unroll
+            for (uint32_t b = 0; b < NB; ++b) {
+                const float4 w = f_blk[st][b];
+                f[b] = step * w.x;
+                e[b] = w.y, down[b] = w.z, mant[b] = w.w;
+                far |= e[b] < M - kFar || mant[b] == 0.f;
+            }
+            // ---- the usual step: nothing hidden, and the maximum still holds. The weights are made
+            // without looking for the maximum; their f16 pairs tell whether one passed 2^kSlack (or is
+            // not a number), and then the scores are read again below. A quarter of the exponentials
+            // runs on the FMA pipe: all of them on the special-function pipe would bound the step.
+            if (TERMS == 1 && j > 0 && !masked && !__any_sync(0xffffffffu, far)) {
+                uint32_t hi[NP / 2], top = 0;
+                float add = 0.f;
+#pragma unroll
+                for (uint32_t c = 0; c < NP; c += 32) {
+                    uint32_t v[32];
+                    tmem_ld32(ts + c, v);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (uint32_t b = c / 16; b < c / 16 + 2; ++b) {
+                        const uint64_t ff = pack2(f[b], f[b]), off = pack2(e[b] - M, e[b] - M);
+                        uint64_t sum = 0;
+#pragma unroll
+                        for (uint32_t i = 0; i < 8; ++i) {
+                            const uint64_t x = fma2(pack2(v[16 * b - c + 2 * i], v[16 * b - c + 2 * i + 1]), ff, off);
+                            const uint64_t w = i % 4 == 3 ? exp2_poly2(x) : pack2(exp2_fast(lo2(x)), exp2_fast(hi2(x)));
+                            sum = add2(sum, w);
+                            hi[8 * b + i] = pack_h2(lo2(w), hi2(w));
+                            top = __vmaxu2(top, hi[8 * b + i]);
+                        }
+                        add = fmaf(lo2(sum) + hi2(sum), down[b], add);
+                    }
+                }
+                // 0x5c00 is 2^8 in f16; an infinity or a NaN is above it
+                if (!__any_sync(0xffffffffu, (top & 0xffffu) > 0x5c00u || top >> 16 > 0x5c00u)) {
+                    l += add;
+#pragma unroll
+                    for (uint32_t b = 0; b < NB; ++b) tmem_st8(ts + 8 * b, hi + 8 * b);
+                    tmem_st_wait();
+                    tc_before();
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive(&p_full[rt][j & 1]);
+                        mbar_arrive(&f_empty[st]);
+                    }
+                    continue;
+                }
+            }
             uint32_t v[NP];
 #pragma unroll
             for (uint32_t c = 0; c < NP; c += 32) tmem_ld32(ts + c, *reinterpret_cast<uint32_t(*)[32]>(v + c));
             tmem_ld_wait();
-            const int32_t p0 = (b0 + (int32_t)(j * NB)) * 16;
-            const bool masked = __any_sync(0xffffffffu, p0 + (int32_t)NP - 1 > open || !live);
             if (masked) {
 #pragma unroll
                 for (uint32_t i = 0; i < NP; ++i)
                     if (p0 + (int32_t)i > last) v[i] = 0xff800000u;  // -infinity
             }
             // the largest score: of each block's products, then by the block's factor (not negative)
-            float mx = -INFINITY, f[NB], e[NB], down[NB], mant[NB];
+            float mx = -INFINITY;
 #pragma unroll
             for (uint32_t b = 0; b < NB; ++b) {
-                const float4 w = f_blk[st][b];
-                f[b] = step * w.x;
-                e[b] = w.y, down[b] = w.z, mant[b] = w.w;
                 float m = __uint_as_float(v[16 * b]);
 #pragma unroll
                 for (uint32_t i = 1; i < 16; ++i) m = fmaxf(m, __uint_as_float(v[16 * b + i]));
@@ -734,7 +813,7 @@ __global__ void __launch_bounds__(32 * (4 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
                     }
                 }
             }
-            bool far = false;
+            far = false;  // (the maximum may have moved)
 #pragma unroll
             for (uint32_t b = 0; b < NB; ++b) far |= (e[b] < M - kFar && e[b] != -INFINITY) || mant[b] == 0.f;
             auto weights = [&](auto rare) {  // rare: hidden positions, or a block far below the maximum
@@ -902,7 +981,7 @@ __global__ void __launch_bounds__(32 * (4 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
             cp_async_commit();
         }
         cp_async_wait<0>();
-    } else if (warp == kSoftWarps + 5) {
+    } else if (warp == kSoftWarps + 4 + RT) {
         // ---------------------------------------------------------------- the blocks' factors
         // one lane per block, 32 / NB steps looked up together
         const int32_t* table = a.b.table + (uint64_t)s * a.b.table_stride;
@@ -939,58 +1018,51 @@ __global__ void __launch_bounds__(32 * (4 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
                 if (lane == 0) mbar_arrive(&f_full[fs]);
             }
         }
-    } else if (warp == kSoftWarps + 4 && steps && elect_one()) {
-        // ---------------------------------------------------------------- MMA
+    } else if (warp < kSoftWarps + 4 + RT && steps && elect_one()) {
+        // ---------------------------------------------------------------- MMA: one thread per row tile, so that
+        // one tile's products run while the other waits for its weights
+        const uint32_t rt = warp - kSoftWarps - 4;
+        const uint32_t d = tm + rt * kTileCols, qb = smem_addr(sq + rt * TERMS * kQPart);
         bool ok = bwait(&q_full, 0, &abort_flag);
         auto scores = [&](uint32_t j) {
             const uint32_t st = j % ST;
-            ok = ok && bwait(&k_full[st], (j / ST) & 1, &abort_flag);
+            // the buffer holds the weights of step j - 2 until their product has ended (products of
+            // different shapes are not ordered by their issue)
+            ok = ok && (j < 2 || bwait(&o_done[rt], (j - 2) & 1, &abort_flag)) &&
+                 bwait(&k_full[st], (j / ST) & 1, &abort_flag);
             if (!ok) return;
             tc_after();
-            const uint32_t kb = smem_addr(skv + st * 2 * kKv);
+            const uint32_t kb = smem_addr(skv + st * 2 * kKv), ds = d + HD + (j & 1) * NP;
 #pragma unroll
-            for (uint32_t t = 0; t < RT; ++t) {
-                // the buffer holds the weights of step j - 2 until their product has ended (products of
-                // different shapes are not ordered by their issue)
-                ok = ok && (j < 2 || bwait(&o_done[t], (j - 2) & 1, &abort_flag));
-                if (!ok) return;
-                tc_after();
-                const uint32_t d = tm + t * kTileCols + HD + (j & 1) * NP;
-                const uint32_t qb = smem_addr(sq + t * TERMS * kQPart);
+            for (uint32_t x = 0; x < (uint32_t)TERMS; ++x)
 #pragma unroll
-                for (uint32_t x = 0; x < (uint32_t)TERMS; ++x)
-#pragma unroll
-                    for (uint32_t k = 0; k < HD / 16; ++k)
-                        mma_ss(d, swizzled_desc(qb + x * kQPart + (k / 4) * (kTileRows * 128) + (k % 4) * 32, 16),
-                               swizzled_desc(kb + (k / 4) * (NP * 128) + (k % 4) * 32, 16), f16_idesc(NP, false), x > 0 || k > 0);
-                mma_commit(&s_full[t][j & 1]);
-            }
+                for (uint32_t k = 0; k < HD / 16; ++k)
+                    mma_ss(ds, swizzled_desc(qb + x * kQPart + (k / 4) * (kTileRows * 128) + (k % 4) * 32, 16),
+                           swizzled_desc(kb + (k / 4) * (NP * 128) + (k % 4) * 32, 16), f16_idesc(NP, false), x > 0 || k > 0);
+            mma_commit(&s_full[rt][j & 1]);
             mma_commit(&k_empty[st]);
         };
         scores(0);
         for (uint32_t j = 0; j < steps && ok; ++j) {
             if (j + 1 < steps) scores(j + 1);
             const uint32_t st = j % ST, vb = smem_addr(skv + st * 2 * kKv + kKv);
-            ok = ok && bwait(&v_full[st], (j / ST) & 1, &abort_flag);
+            ok = ok && bwait(&v_full[st], (j / ST) & 1, &abort_flag) &&
+                 bwait(&p_full[rt][j & 1], (j >> 1) & 1, &abort_flag);
+            if (!ok) break;
+            tc_after();
+            const uint32_t pw = d + HD + (j & 1) * NP;
 #pragma unroll
-            for (uint32_t t = 0; t < RT; ++t) {
-                ok = ok && bwait(&p_full[t][j & 1], (j >> 1) & 1, &abort_flag);
-                if (!ok) break;
-                tc_after();
-                const uint32_t d = tm + t * kTileCols, p = d + HD + (j & 1) * NP;
+            for (uint32_t x = 0; x < (uint32_t)TERMS; ++x)
 #pragma unroll
-                for (uint32_t x = 0; x < (uint32_t)TERMS; ++x)
-#pragma unroll
-                    for (uint32_t k = 0; k < NP / 16; ++k)
-                        mma_ts(d, p + x * (NP / 2) + 8 * k, swizzled_desc(vb + k * 2048, NP * 128), f16_idesc(HD, true),
-                               j > 0 || x > 0 || k > 0);
-                mma_commit(&o_done[t]);
-            }
-            if (ok) mma_commit(&v_empty[st]);
+                for (uint32_t k = 0; k < NP / 16; ++k)
+                    mma_ts(d, pw + x * (NP / 2) + 8 * k, swizzled_desc(vb + k * 2048, NP * 128), f16_idesc(HD, true),
+                           j > 0 || x > 0 || k > 0);
+            mma_commit(&o_done[rt]);
+            mma_commit(&v_empty[st]);
         }
         if (!ok) {  // the MMAs in flight end before the tensor memory is freed
-            mma_commit(&fin);
-            mbar_wait(&fin, 0);
+            mma_commit(&fin[rt]);
+            mbar_wait(&fin[rt], 0);
         }
     }
     __syncwarp();
@@ -1029,7 +1101,7 @@ Shape shape_of(const Kv8Cache& c, const Kv8Batch& b, uint32_t heads, uint32_t ty
 template <class T, int HD> cudaError_t launch(const Plan& p, bool tiles, cudaStream_t s) {
     if (tiles) {
         constexpr int terms = sizeof(T) == 4 ? 2 : 1;
-        constexpr uint32_t smem = tile_smem(HD, terms), threads = 32 * (4 * role_of(HD, terms).rt + 6);
+        constexpr uint32_t smem = tile_smem(HD, terms), threads = 32 * (5 * role_of(HD, terms).rt + 5);
         static std::atomic<bool> opted[64];
         int dev = 0;
         cudaError_t e = cudaGetDevice(&dev);
