@@ -485,6 +485,17 @@ __device__ __forceinline__ bool bwait(uint64_t* bar, uint32_t parity, volatile i
     }
     return true;
 }
+// the same for a whole warp, which stays together
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    const uint64_t t0 = global_ns();
+    while (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity)))
+        if (__any_sync(0xffffffffu, *abort_flag || global_ns() - t0 > kWaitNs)) {
+            *abort_flag = 1;
+            return false;
+        }
+    return true;
+}
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
@@ -717,8 +728,7 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
         bool ok = true;
         for (uint32_t j = 0; j < steps && ok; ++j) {
             const uint32_t st = j % FS;
-            ok = bwait(&f_full[st], (j / FS) & 1, &abort_flag) && bwait(&s_full[rt][j & 1], (j >> 1) & 1, &abort_flag);
-            ok = __all_sync(0xffffffffu, ok);
+            ok = warp_wait(&f_full[st], (j / FS) & 1, &abort_flag) && warp_wait(&s_full[rt][j & 1], (j >> 1) & 1, &abort_flag);
             if (!ok) break;
             tc_after();
             const uint32_t ts = to + HD + (j & 1) * NP;
@@ -799,7 +809,7 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
                 l = rebase(l, M, m);
                 M = m;
                 if (j > 0) {
-                    ok = __all_sync(0xffffffffu, bwait(&o_done[rt], (j - 1) & 1, &abort_flag));
+                    ok = warp_wait(&o_done[rt], (j - 1) & 1, &abort_flag);
                     if (!ok) break;
                     tc_after();
 #pragma unroll 1
@@ -861,8 +871,8 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
         }
         // (one phase after the other: a parity says nothing about a phase two steps away. Inside the loop
         // the scores of step j imply the product of step j - 2)
-        if (steps > 1 && ok) ok = __all_sync(0xffffffffu, bwait(&o_done[rt], (steps - 2) & 1, &abort_flag));
-        if (steps && ok) ok = __all_sync(0xffffffffu, bwait(&o_done[rt], (steps - 1) & 1, &abort_flag));
+        if (steps > 1 && ok) ok = warp_wait(&o_done[rt], (steps - 2) & 1, &abort_flag);
+        if (steps && ok) ok = warp_wait(&o_done[rt], (steps - 1) & 1, &abort_flag);
         tc_after();
         if (ok) {
             const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);  // a row that sees nothing: zeros
@@ -968,10 +978,10 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
             cp_async_wait<(int)RAW - 1>();
             const uint8_t* raw = sraw + rs * (2 * NP * HD);
             uint8_t* dst = skv + st * 2 * kKv;
-            if (j >= ST) bwait(&k_empty[st], (j / ST - 1) & 1, &abort_flag);
+            if (j >= ST) warp_wait(&k_empty[st], (j / ST - 1) & 1, &abort_flag);
             widen(dst, raw, none);
             if (lane == 0) mbar_arrive(&k_full[st]);
-            if (j >= ST) bwait(&v_empty[st], (j / ST - 1) & 1, &abort_flag);
+            if (j >= ST) warp_wait(&v_empty[st], (j / ST - 1) & 1, &abort_flag);
             widen(dst + kKv, raw + NP * HD, none);
             if (lane == 0) mbar_arrive(&v_full[st]);
             if (j + RAW < steps) {
@@ -1011,7 +1021,7 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
                                          : log2f(sv);
             for (uint32_t i = 0; i < 32 / NB && j0 + i < steps; ++i) {
                 const uint32_t j = j0 + i, fs = j % FS;
-                if (j >= FS) bwait(&f_empty[fs], (j / FS - 1) & 1, &abort_flag);
+                if (j >= FS) warp_wait(&f_empty[fs], (j / FS - 1) & 1, &abort_flag);
                 __syncwarp();
                 if (lane / NB == i) f_blk[fs][lane % NB] = make_float4(sk, e, down, mant);
                 __syncwarp();
