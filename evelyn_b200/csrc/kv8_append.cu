@@ -8,11 +8,12 @@
 // call holds rint(x / scale), and one filled a token at a time is off by at most one more
 // rounding for each time that its scale rose.
 //
-// Layout: a warp owns one (block, kv head) of K or of V, so nothing else touches the block's
-// scale or codes and no atomics are needed. A lane holds four values of a row, as two pairs
+// Layout: a CTA of four warps owns one (block, kv head) of K or of V, so nothing else touches the
+// block's scale or codes and no atomics are needed; its rows are dealt to the warps and stay in
+// registers, the maximum meets in shared memory. A lane holds four values of a row, as two pairs
 // (NeoX rotation: dims 2u, 2u+1 and the same + rope_dim / 2; else four neighbours), so both
-// halves of a rotated pair sit in one lane. The rows of a block are all in flight before the
-// maximum is known. Bound: HBM (each new value read once, one byte written).
+// halves of a rotated pair sit in one lane. Query rows: a warp takes four heads of a token at a
+// time. Bound: HBM (each new value read once, one byte written).
 //
 // Norm: the sum of squares and its root are computed in 64 bits and rounded once, then x * r * w
 // in f32; rotation in f32, each product and sum rounded once. So codes and scales are the same
@@ -27,9 +28,10 @@ constexpr uint32_t kQHeads = 4;  // q heads a warp takes together
 
 struct Plan {
     Kv8AppendArgs a;
-    uint32_t tile;        // tokens whose blocks one warp looks for: 1 or 16
-    uint32_t kv_items;    // (tile, K or V, kv head)
-    uint32_t items;       // and (token, group of q heads) after them
+    uint32_t tile;        // tokens whose blocks one CTA looks for: 1 or 16
+    uint32_t kv_ctas;     // (tile, K or V, kv head)
+    uint32_t q_tokens;    // consecutive tokens of a warp
+    uint32_t q_items;     // (q_tokens tokens, group of q heads), a warp each, in the CTAs after those
     uint32_t q_groups, q_per;
 };
 
@@ -98,47 +100,49 @@ __device__ __forceinline__ Seq seq_of(const Kv8AppendArgs& a, int32_t t, uint32_
     return r;
 }
 
-// New rows of one block: positions base + (t - q0), t in [t, t + rows), of head h of K or V.
+// New rows of one block: positions base + (t - q0), tokens [t, t + rows), of head h of K or V.
+// Called by the whole CTA.
 template <class T, int HD, bool KEY>
-__device__ __forceinline__ void write_block(const Kv8AppendArgs& a, const Seq& sq, int32_t t, uint32_t rows,
-                                            uint32_t h, uint32_t lane) {
+__device__ __forceinline__ void write_block(const Kv8AppendArgs& a, const Seq& sq, int32_t t, uint32_t rows, uint32_t h,
+                                            uint32_t warp, uint32_t lane, uint32_t* red) {
     constexpr uint32_t W = HD == 64 ? 16 : 32;       // lanes per row
-    constexpr int P = 32 / W;                        // rows side by side
+    constexpr uint32_t P = 32 / W;                   // rows of a warp side by side
     constexpr int N = HD / (4 * W);                  // units per lane
-    constexpr int R = 16 / P;                        // passes over the block's rows
+    constexpr uint32_t S = P * kWarps, R = 16 / S;   // rows of the CTA side by side, passes
     const uint32_t pos = (uint32_t)(sq.base + (t - sq.q0)), row0 = pos % 16;
     const uint32_t pg = pos / a.c.page_size, blk = pos % a.c.page_size / 16;
-    const int32_t page = a.b.table[(uint64_t)sq.s * a.b.table_stride + pg];
-    if (page < 0 || (uint32_t)page >= a.c.n_pages) {
-        if (lane == 0) flag_error(a.err, DEV_ERR_POSITION);
-        return;
-    }
-    float* scale_at = (KEY ? a.c.ks : a.c.vs) + (uint64_t)page * a.c.scale_stride + h * (a.c.page_size / 16) + blk;
-    int8_t* codes = (KEY ? a.c.k : a.c.v) + (uint64_t)page * a.c.page_stride +
-                    ((uint64_t)h * a.c.page_size + blk * 16) * HD;
-    const float old = row0 ? *scale_at : 0.f;
+    const uint32_t sub = lane / W, u0 = lane % W, first = warp * P + sub;  // this lane's rows: first, first + S, ...
     const T* src = static_cast<const T*>(KEY ? a.k : a.v) + h * HD;
     const uint64_t stride = KEY ? a.k_stride : a.v_stride;
-    const uint32_t sub = lane / W, u0 = lane % W;
     Unit un[N];
 #pragma unroll
     for (int n = 0; n < N; ++n) un[n] = unit_of(u0 + n * W, KEY ? a.rope_dim : 0u, KEY && a.interleaved);
     float x[R][N][4];
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const uint32_t i = r * P + sub;
+    for (uint32_t r = 0; r < R; ++r) {
+        const uint32_t i = first + r * S;
         const T* p = src + (uint64_t)(t + (int32_t)min(i, rows - 1)) * stride;
+        if (r == 0 || r * S < rows)
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
-            if (!KEY) {
-                load4(p + un[n].lo, x[r][n]);
-            } else {
-                load2(p + un[n].lo, x[r][n][0], x[r][n][1]);
-                load2(p + un[n].hi, x[r][n][2], x[r][n][3]);
+            for (int n = 0; n < N; ++n) {
+                if (!KEY) {
+                    load4(p + un[n].lo, x[r][n]);
+                } else {
+                    load2(p + un[n].lo, x[r][n][0], x[r][n][1]);
+                    load2(p + un[n].hi, x[r][n][2], x[r][n][3]);
+                }
             }
-        }
-        if (r + 1 < R && (uint32_t)(r + 1) * P >= rows) break;
     }
+    const int32_t page = a.b.table[(uint64_t)sq.s * a.b.table_stride + pg];
+    const bool fine = (uint32_t)page < a.c.n_pages;
+    if (!fine) {
+        if (threadIdx.x == 0) flag_error(a.err, DEV_ERR_POSITION);
+        return;  // the whole CTA
+    }
+    float* scale_at = (KEY ? a.c.ks : a.c.vs) + (uint64_t)page * a.c.scale_stride + h * (a.c.page_size / 16) + blk;
+    int8_t* codes = (KEY ? a.c.k : a.c.v) + (uint64_t)page * a.c.page_stride +
+                    ((uint64_t)h * a.c.page_size + blk * 16) * HD;
+    const float old = row0 ? *scale_at : 0.f;
     float w[N][4];
     if (KEY && a.k_norm) {
 #pragma unroll
@@ -149,13 +153,12 @@ __device__ __forceinline__ void write_block(const Kv8AppendArgs& a, const Seq& s
     }
     uint32_t m = 0;
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        if ((uint32_t)r * P < rows) {
-            const uint32_t i = r * P + sub;
+    for (uint32_t r = 0; r < R; ++r) {
+        if (r * S < rows) {
             if (KEY) {
                 if (a.k_norm) norm_row<N>(x[r], w, HD, a.eps, W);
                 if (a.rope) {
-                    const float* tr = a.rope + (uint64_t)(pos + min(i, rows - 1)) * a.rope_dim;
+                    const float* tr = a.rope + (uint64_t)(pos + min(first + r * S, rows - 1)) * a.rope_dim;
 #pragma unroll
                     for (int n = 0; n < N; ++n)
                         if (un[n].turns)
@@ -169,6 +172,10 @@ __device__ __forceinline__ void write_block(const Kv8AppendArgs& a, const Seq& s
         }
     }
     m = __reduce_max_sync(0xffffffffu, m);
+    if (lane == 0) red[warp] = m;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t k = 0; k < kWarps; ++k) m = max(m, red[k]);
     const float fresh = scale_of(m);
     // a NaN on either side (a value that is not finite, now or earlier in this block) stays
     const float now = (fresh != fresh || old != old) ? __uint_as_float(0x7fc00000u) : fmaxf(old, fresh);
@@ -176,7 +183,7 @@ __device__ __forceinline__ void write_block(const Kv8AppendArgs& a, const Seq& s
     const bool live = now > 0.f;
     if (row0 && __float_as_uint(now) != __float_as_uint(old)) {  // the earlier rows follow the scale
         const float ratio = live ? __fdiv_rn(old, now) : 0.f;
-        for (uint32_t i = sub; i < row0; i += P)
+        for (uint32_t i = first; i < row0; i += S)
 #pragma unroll
             for (int n = 0; n < N; ++n) {
                 uint32_t* at = reinterpret_cast<uint32_t*>(codes + i * HD + 4 * (u0 + n * W));
@@ -187,10 +194,9 @@ __device__ __forceinline__ void write_block(const Kv8AppendArgs& a, const Seq& s
                 *at = pack4(q[0], q[1], q[2], q[3]);
             }
     }
-    if (lane == 0) *scale_at = now;
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const uint32_t i = r * P + sub;
+    for (uint32_t r = 0; r < R; ++r) {
+        const uint32_t i = first + r * S;
         if (i < rows) {
             int8_t* at = codes + (row0 + i) * HD;
 #pragma unroll
@@ -199,7 +205,7 @@ __device__ __forceinline__ void write_block(const Kv8AppendArgs& a, const Seq& s
 #pragma unroll
                 for (int j = 0; j < 4; ++j) q[j] = live ? code_bits(x[r][n][j], inv) : 0u;
                 const uint32_t c = pack4(q[0], q[1], q[2], q[3]);
-                if (!KEY) {
+                if (!KEY || un[n].hi == un[n].lo + 2) {
                     *reinterpret_cast<uint32_t*>(at + un[n].lo) = c;
                 } else {
                     *reinterpret_cast<uint16_t*>(at + un[n].lo) = (uint16_t)c;
@@ -208,6 +214,8 @@ __device__ __forceinline__ void write_block(const Kv8AppendArgs& a, const Seq& s
             }
         }
     }
+    __syncthreads();  // every warp has read the old scale (and red) by now
+    if (threadIdx.x == 0) *scale_at = now;
 }
 
 // q heads [h0, h0 + n) of token t: norm, rotation, one rounding to the output type.
@@ -264,21 +272,27 @@ __device__ __forceinline__ void write_q(const Kv8AppendArgs& a, uint32_t pos, in
     }
 }
 
-template <class T, int HD> __global__ void __launch_bounds__(32 * kWarps) kv8_append_kernel(const __grid_constant__ Plan p) {
-    const uint32_t lane = threadIdx.x & 31;
-    const uint32_t item = blockIdx.x * kWarps + (threadIdx.x >> 5);
-    if (item >= p.items) return;
+template <class T, int HD> __global__ void __launch_bounds__(32 * kWarps, 5) kv8_append_kernel(const __grid_constant__ Plan p) {
+    __shared__ uint32_t red[kWarps];
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const Kv8AppendArgs& a = p.a;
-    if (item >= p.kv_items) {
-        const uint32_t i = item - p.kv_items, h0 = i % p.q_groups * p.q_per;
-        const int32_t t = (int32_t)(i / p.q_groups);
-        const Seq sq = seq_of(a, t, lane);
-        if (sq.ok) write_q<T, HD>(a, (uint32_t)(sq.base + (t - sq.q0)), t, h0, min(p.q_per, a.heads - h0), lane);
+    if (blockIdx.x >= p.kv_ctas) {
+        const uint32_t item = (blockIdx.x - p.kv_ctas) * kWarps + warp;
+        if (item >= p.q_items) return;
+        const uint32_t h0 = item % p.q_groups * p.q_per;
+        const int32_t t0 = (int32_t)(item / p.q_groups * p.q_tokens), t1 = min(t0 + (int32_t)p.q_tokens, (int32_t)a.b.total);
+        Seq sq;
+        sq.q1 = t0;
+        for (int32_t t = t0; t < t1; ++t) {
+            if (t >= sq.q1 || t == t0) sq = seq_of(a, t, lane);
+            if (sq.ok) write_q<T, HD>(a, (uint32_t)(sq.base + (t - sq.q0)), t, h0, min(p.q_per, a.heads - h0), lane);
+            else sq.q1 = t;  // (look again at the next one)
+        }
         return;
     }
-    const uint32_t per = 2 * a.c.kv_heads, hk = item % per, h = hk >> 1;
-    const int32_t t0 = (int32_t)(item / per * p.tile), t1 = min(t0 + (int32_t)p.tile, (int32_t)a.b.total);
-    // the blocks whose first new token is in [t0, t1)
+    const uint32_t per = 2 * a.c.kv_heads, hk = blockIdx.x % per, h = hk >> 1;
+    const int32_t t0 = (int32_t)(blockIdx.x / per * p.tile), t1 = min(t0 + (int32_t)p.tile, (int32_t)a.b.total);
+    // the blocks whose first new token is in [t0, t1); every warp looks for itself and finds the same
     for (int32_t t = t0; t < t1;) {
         const Seq sq = seq_of(a, t, lane);
         if (!sq.ok) {
@@ -288,15 +302,15 @@ template <class T, int HD> __global__ void __launch_bounds__(32 * kWarps) kv8_ap
         const uint32_t pos = (uint32_t)(sq.base + (t - sq.q0)), row = pos % 16;
         const int32_t end = min(sq.q1, t + 16 - (int32_t)row);  // the block's new tokens end here
         if (row == 0 || t == sq.q0) {
-            if (hk & 1) write_block<T, HD, false>(a, sq, t, (uint32_t)(end - t), h, lane);
-            else write_block<T, HD, true>(a, sq, t, (uint32_t)(end - t), h, lane);
+            if (hk & 1) write_block<T, HD, false>(a, sq, t, (uint32_t)(end - t), h, warp, lane, red);
+            else write_block<T, HD, true>(a, sq, t, (uint32_t)(end - t), h, warp, lane, red);
         }
         t = end;
     }
 }
 
 template <class T> cudaError_t launch(const Plan& p, cudaStream_t s) {
-    const uint32_t grid = (p.items + kWarps - 1) / kWarps;
+    const uint32_t grid = p.kv_ctas + (p.q_items + kWarps - 1) / kWarps;
     if (p.a.c.head_dim == 64) kv8_append_kernel<T, 64><<<grid, 32 * kWarps, 0, s>>>(p);
     else if (p.a.c.head_dim == 128) kv8_append_kernel<T, 128><<<grid, 32 * kWarps, 0, s>>>(p);
     else kv8_append_kernel<T, 256><<<grid, 32 * kWarps, 0, s>>>(p);
@@ -308,17 +322,19 @@ template <class T> cudaError_t launch(const Plan& p, cudaStream_t s) {
 cudaError_t launch_kv8_append(const Kv8AppendArgs& a, cudaStream_t s) {
     Plan p;
     p.a = a;
-    // prompts: a warp covers 16 tokens, so nearly every warp finds one block; decoding: every
-    // token starts or continues a block of its own and gets its own warps
+    // prompts: a CTA covers 16 tokens, so nearly every CTA finds one block; decoding: every
+    // token starts or continues a block of its own and gets its own CTAs
     p.tile = (uint64_t)a.b.total >= 8ull * a.b.n_seqs ? 16 : 1;
     const uint64_t tiles = (a.b.total + p.tile - 1) / p.tile;
-    // few tokens: one q head per warp, for the shortest chain; many: four in flight
+    // few tokens: one q head per warp, for the shortest chain; many: four in flight, four tokens
+    // one after the other under one look at the sequence
     p.q_per = p.tile == 1 ? 1 : kQHeads;
+    p.q_tokens = p.tile == 1 ? 1 : 4;
     p.q_groups = a.q ? (a.heads + p.q_per - 1) / p.q_per : 0;
-    const uint64_t kv = tiles * 2 * a.c.kv_heads, items = kv + (uint64_t)a.b.total * p.q_groups;
-    if (items > 0x7fffffffull) return cudaErrorInvalidValue;
-    p.kv_items = (uint32_t)kv;
-    p.items = (uint32_t)items;
+    const uint64_t kv = tiles * 2 * a.c.kv_heads, q = (uint64_t)((a.b.total + p.q_tokens - 1) / p.q_tokens) * p.q_groups;
+    if (kv + q > 0x7fffffffull) return cudaErrorInvalidValue;
+    p.kv_ctas = (uint32_t)kv;
+    p.q_items = (uint32_t)q;
     switch (a.type) {
         case GGML_F32: return launch<float>(p, s);
         case GGML_F16: return launch<__half>(p, s);

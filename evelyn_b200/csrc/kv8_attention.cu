@@ -570,20 +570,6 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
-// 2^x of two values on the FMA pipe, x from -126 (below: as there) up to 127: the nearest whole number
-// n goes into the exponent, 2^(x - n) is a polynomial of degree 4 fitted on [-1/2, 1/2] for the smallest
-// relative error (2.6e-6, a 50th of the f16 rounding that follows).
-__device__ __forceinline__ uint64_t exp2_poly2(uint64_t x) {
-    x = pack2(fmaxf(lo2(x), -126.f), fmaxf(hi2(x), -126.f));
-    const uint64_t n = add2(x, pack2(12582912.f, 12582912.f));  // n in the low mantissa bits
-    const uint64_t r = add2(x, fma2(add2(n, pack2(-12582912.f, -12582912.f)), pack2(-1.f, -1.f), 0ull));
-    uint64_t y = fma2(pack2(0.009570101276f, 0.009570101276f), r, pack2(0.05591785908f, 0.05591785908f));
-    y = fma2(y, r, pack2(0.2402474433f, 0.2402474433f));
-    y = fma2(y, r, pack2(0.6931217909f, 0.6931217909f));
-    y = fma2(y, r, pack2(0.9999992847f, 0.9999992847f));
-    return pack2((uint32_t)y + ((uint32_t)n << 23), (uint32_t)(y >> 32) + ((uint32_t)(n >> 32) << 23));
-}
-
 // byte offset of 16-byte piece `p` (8 f16 values) of row r in panels of `rows` rows
 __device__ __forceinline__ uint32_t panel_at(uint32_t rows, uint32_t r, uint32_t p) {
     return (p >> 3) * (rows * 128u) + r * 128u + (((p & 7u) ^ (r & 7u)) << 4);
@@ -744,12 +730,11 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
                 far |= e[b] < M - kFar || mant[b] == 0.f;
             }
             // ---- the usual step: nothing hidden, and the maximum still holds. The weights are made
-            // without looking for the maximum; their f16 pairs tell whether one passed 2^kSlack (or is
-            // not a number), and then the scores are read again below. A quarter of the exponentials
-            // runs on the FMA pipe: all of them on the special-function pipe would bound the step.
+            // without looking for the maximum: their sum tells whether one may be too large for f16 (or is
+            // not a number), and then the scores are read again below.
             if (TERMS == 1 && j > 0 && !masked && !__any_sync(0xffffffffu, far)) {
-                uint32_t hi[NP / 2], top = 0;
-                float add = 0.f;
+                uint32_t hi[NP / 2];
+                float add = 0.f, tot = 0.f;
 #pragma unroll
                 for (uint32_t c = 0; c < NP; c += 32) {
                     uint32_t v[32];
@@ -762,16 +747,16 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
 #pragma unroll
                         for (uint32_t i = 0; i < 8; ++i) {
                             const uint64_t x = fma2(pack2(v[16 * b - c + 2 * i], v[16 * b - c + 2 * i + 1]), ff, off);
-                            const uint64_t w = i % 4 == 3 ? exp2_poly2(x) : pack2(exp2_fast(lo2(x)), exp2_fast(hi2(x)));
-                            sum = add2(sum, w);
-                            hi[8 * b + i] = pack_h2(lo2(w), hi2(w));
-                            top = __vmaxu2(top, hi[8 * b + i]);
+                            const float w0 = exp2_fast(lo2(x)), w1 = exp2_fast(hi2(x));
+                            sum = add2(sum, pack2(w0, w1));
+                            hi[8 * b + i] = pack_h2(w0, w1);
                         }
-                        add = fmaf(lo2(sum) + hi2(sum), down[b], add);
+                        const float s1 = lo2(sum) + hi2(sum);
+                        tot += s1;
+                        add = fmaf(s1, down[b], add);
                     }
                 }
-                // 0x5c00 is 2^8 in f16; an infinity or a NaN is above it
-                if (!__any_sync(0xffffffffu, (top & 0xffffu) > 0x5c00u || top >> 16 > 0x5c00u)) {
+                if (__all_sync(0xffffffffu, tot < 16384.f)) {
                     l += add;
 #pragma unroll
                     for (uint32_t b = 0; b < NB; ++b) tmem_st8(ts + 8 * b, hi + 8 * b);
