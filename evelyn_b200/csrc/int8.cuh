@@ -65,6 +65,15 @@ template <class T> __device__ __forceinline__ void store2(T* p, float a, float b
     }
 }
 
+template <class T> __device__ __forceinline__ void store4(T* p, const float (&x)[4]) {
+    if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+    } else {
+        T v[4] = {from_f32<T>(x[0]), from_f32<T>(x[1]), from_f32<T>(x[2]), from_f32<T>(x[3])};
+        *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(v);
+    }
+}
+
 // |x| as bits: unsigned order is the order of magnitudes, with the infinity above every
 // finite number and NaN above it, so one integer maximum finds both the largest magnitude
 // and whether all values are finite.

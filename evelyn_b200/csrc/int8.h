@@ -65,7 +65,7 @@ struct Kv8AppendArgs {
     float eps = 0.f;
     int32_t* err = nullptr;
 };
-cudaError_t launch_kv8_append(const Kv8AppendArgs& a, cudaStream_t s);
+cudaError_t launch_kv8_append(const Kv8AppendArgs& a, int sms, cudaStream_t s);
 
 struct Kv8AttnArgs {
     Kv8Cache c;

@@ -256,7 +256,7 @@ evl_status evl_kv8_append(const evl_kv8_cache* cache, const evl_kv8_batch* batch
         a.v_stride = v_stride;
         a.err = d_err;
         OnDeviceOf on(d_k);
-        cuda_check(launch_kv8_append(a, static_cast<cudaStream_t>(stream)), "kv8 append");
+        cuda_check(launch_kv8_append(a, sm_count(on.dev), static_cast<cudaStream_t>(stream)), "kv8 append");
     });
 }
 
