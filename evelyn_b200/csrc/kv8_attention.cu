@@ -17,14 +17,14 @@
 //   K: mma.sync m16n8k32 on the codes as they are. q is fixed point in three signed 8-bit limbs
 //      (22 bits below the row's largest magnitude), the integer products are exact, so a score
 //      is as good as an f32 dot product. The K order inside the product is permuted so that a
-//      lane's fragment is 16 neighbouring bytes of a row: codes go from HBM to registers to the
-//      tensor cores, with no shared memory and no conversion.
+//      lane's fragment is 16 neighbouring bytes of a row: the codes reach the tensor cores as they
+//      were copied, with no conversion.
 //   V: mma.sync m16n8k16 in f16: codes are exact in f16, the weights two f16 parts (22 bits).
 //      A lane loads 16 neighbouring dims of four positions and pairs positions with byte
 //      permutes; the weights move to the other operand's layout by two 8x8 transposes.
 //   The maximum is raised only when a score passes it by 2^8, so most blocks cost one vote.
-// A warp takes every 4th block of the CTA's chunk of positions, the next block's codes already
-// in flight in registers. The warps' partials meet in shared memory; a sequence of more than one
+// A warp takes every 4th block of the CTA's chunk of positions, the next blocks already on their way
+// into a ring of its own (asynchronous copies, each lane its own pieces: no barrier, no registers). The warps' partials meet in shared memory; a sequence of more than one
 // chunk leaves (O, M, l) in the workspace for kv8_join_kernel.
 // Bound: HBM, (2 head_dim + 1/2) bytes per position and kv head.
 #include <algorithm>
@@ -113,41 +113,80 @@ __device__ __forceinline__ Span span_of(const Kv8AttnArgs& a, uint32_t s) {
     return r;
 }
 
-// The codes and scales of one block of 16 positions for one lane.
-template <int HD> struct Block {
-    uint32_t k[HD / 64][2][4];                       // rows g, g + 8: 16 bytes at 64 c + 16 t
-    uint32_t v[HD <= 128 ? 1 : 2][4][HD < 128 ? 2 : 4];  // positions 2t, 2t+1, 2t+8, 2t+9: 16 (8) bytes of dims
-    float sk, sv;
-};
+// One block of 16 positions for one warp in shared memory: 16 (8) byte pieces, each in the place of the
+// lane that will use it, so a lane reads what it copied itself and the warp needs no barrier:
+// K rows g, g + 8 at 64 c + 16 t; V positions 2t, 2t+1, 2t+8, 2t+9 at 16 g (8 g); the two scales.
+constexpr uint32_t ring_bytes(int hd) { return 32u * hd + 256; }
+// blocks on their way per warp (a block in use besides): as many as leave room for three CTAs on an SM
+constexpr int ring_depth(int hd) { return hd == 64 ? 6 : hd == 128 ? 4 : 3; }
+constexpr uint32_t split_smem(int hd) { return kWarps * ring_depth(hd) * ring_bytes(hd); }
+
+template <int N> __device__ __forceinline__ void cp_async(void* dst, const void* src) {
+    if constexpr (N == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(dst)), "l"(src) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_addr(dst)), "l"(src), "n"(N) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
 template <int HD>
-__device__ __forceinline__ void load_block(Block<HD>& b, const Kv8Cache& c, int32_t page, uint32_t sub, uint32_t h,
-                                           uint32_t g, uint32_t t) {
+__device__ __forceinline__ void fetch_block(uint8_t* slot, const Kv8Cache& c, int32_t page, uint32_t sub, uint32_t h,
+                                            uint32_t lane) {
+    const uint32_t g = lane >> 2, t = lane & 3;
     const uint64_t row = (uint64_t)page * c.page_stride + ((uint64_t)h * c.page_size + sub * 16) * HD;
     const int8_t *k = c.k + row, *v = c.v + row;
-    const uint64_t sc = (uint64_t)page * c.scale_stride + h * (c.page_size / 16) + sub;
-    b.sk = __ldg(c.ks + sc);
-    b.sv = __ldg(c.vs + sc);
 #pragma unroll
     for (int i = 0; i < HD / 64; ++i)
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const uint4 w = ldg_nc(k + (g + 8 * r) * HD + 64 * i + 16 * t);
-            b.k[i][r][0] = w.x, b.k[i][r][1] = w.y, b.k[i][r][2] = w.z, b.k[i][r][3] = w.w;
-        }
+        for (int r = 0; r < 2; ++r) cp_async<16>(slot + (i * 2 + r) * 512 + lane * 16, k + (g + 8 * r) * HD + 64 * i + 16 * t);
+    slot += HD / 32 * 512;
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
         const int8_t* at = v + (2 * t + (p & 1) + (p >> 1) * 8) * HD;
         if constexpr (HD == 64) {
-            const uint2 w = __ldg(reinterpret_cast<const uint2*>(at + 8 * g));
+            cp_async<8>(slot + p * 256 + lane * 8, at + 8 * g);
+        } else {
+#pragma unroll
+            for (int i = 0; i < HD / 128; ++i) cp_async<16>(slot + (p * (HD / 128) + i) * 512 + lane * 16, at + 128 * i + 16 * g);
+        }
+    }
+    slot += HD * 16;
+    const uint64_t sc = (uint64_t)page * c.scale_stride + h * (c.page_size / 16) + sub;
+    cp_async<4>(slot + lane * 8, c.ks + sc);
+    cp_async<4>(slot + lane * 8 + 4, c.vs + sc);
+}
+// The codes and scales of one block for one lane.
+template <int HD> struct Block {
+    uint32_t k[HD / 64][2][4];
+    uint32_t v[HD <= 128 ? 1 : 2][4][HD < 128 ? 2 : 4];
+    float sk, sv;
+};
+template <int HD> __device__ __forceinline__ void read_block(Block<HD>& b, const uint8_t* slot, uint32_t lane) {
+#pragma unroll
+    for (int i = 0; i < HD / 64; ++i)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const uint4 w = *reinterpret_cast<const uint4*>(slot + (i * 2 + r) * 512 + lane * 16);
+            b.k[i][r][0] = w.x, b.k[i][r][1] = w.y, b.k[i][r][2] = w.z, b.k[i][r][3] = w.w;
+        }
+    slot += HD / 32 * 512;
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+        if constexpr (HD == 64) {
+            const uint2 w = *reinterpret_cast<const uint2*>(slot + p * 256 + lane * 8);
             b.v[0][p][0] = w.x, b.v[0][p][1] = w.y;
         } else {
 #pragma unroll
             for (int i = 0; i < HD / 128; ++i) {
-                const uint4 w = ldg_nc(at + 128 * i + 16 * g);
+                const uint4 w = *reinterpret_cast<const uint4*>(slot + (p * (HD / 128) + i) * 512 + lane * 16);
                 b.v[i][p][0] = w.x, b.v[i][p][1] = w.y, b.v[i][p][2] = w.z, b.v[i][p][3] = w.w;
             }
         }
     }
+    slot += HD * 16;
+    const float2 s = *reinterpret_cast<const float2*>(slot + lane * 8);
+    b.sk = s.x, b.sv = s.y;
 }
 
 template <class T, int HD>
@@ -157,8 +196,10 @@ __global__ void __launch_bounds__(32 * kWarps) kv8_split_kernel(const __grid_con
     constexpr int VC = HD <= 128 ? 1 : 2;        // V loads per position
     constexpr int MT = HD / 16;                  // 16-dim tiles of the output
     constexpr int LD = HD / 8 < 16 ? HD / 8 : 16;  // neighbouring dims of a lane's load
-    __shared__ float so[kWarps][kRows][HD];
+    constexpr int D = ring_depth(HD);
+    extern __shared__ __align__(16) uint8_t ring_smem[];
     __shared__ float2 sml[kWarps][kRows];
+    static_assert(split_smem(HD) >= kWarps * kRows * HD * 4, "the warps' partials lie over the rings");
     const Kv8AttnArgs& a = P.a;
     const uint32_t split = blockIdx.x, h = blockIdx.y % a.c.kv_heads, tile = blockIdx.y / a.c.kv_heads, s = blockIdx.z;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -175,6 +216,26 @@ __global__ void __launch_bounds__(32 * kWarps) kv8_split_kernel(const __grid_con
     const int32_t nblk = seen > 0 ? (seen + 15) / 16 : 0;
     const int32_t b0 = (int32_t)(split * P.chunk), b1 = min(nblk, b0 + (int32_t)P.chunk);
     if (b0 >= nblk && split > 0) return;  // (split 0 of an empty tile writes its zeros)
+
+    // ---- the warp's blocks b0 + warp, + kWarps, ...: D - 1 of them on their way, the pages of one more
+    // looked up
+    const int32_t* table = a.b.table + (uint64_t)s * a.b.table_stride;
+    const uint32_t lb = 31 - __clz(a.c.page_size / 16);  // log2 of the blocks of a page: 0, 1 or 2
+    uint8_t* ring = ring_smem + warp * (D * ring_bytes(HD));
+    auto page_of = [&](int32_t blk) { return blk < b1 ? __ldg(table + ((uint32_t)blk >> lb)) : -1; };
+    uint32_t bad = 0;  // bits: slots whose block has no valid page
+    bool bad_page = false;
+    int32_t ahead = b0 + (int32_t)warp, page = page_of(ahead);
+    auto fetch = [&](uint32_t slot) {
+        const bool fine = page >= 0 && (uint32_t)page < a.c.n_pages;
+        bad = fine ? bad & ~(1u << slot) : bad | 1u << slot;
+        if (fine) fetch_block<HD>(ring + slot * ring_bytes(HD), a.c, page, (uint32_t)ahead & ((1u << lb) - 1), h, lane);
+        cp_async_commit();
+        ahead += kWarps;
+        page = page_of(ahead);
+    };
+#pragma unroll
+    for (int i = 0; i < D - 1; ++i) fetch((uint32_t)i);
 
     // ---- q of row g: fixed point, m = q 2^sh, |m| <= 2^22, in three signed limbs
     uint32_t qb[3][KC][4];
@@ -236,20 +297,17 @@ __global__ void __launch_bounds__(32 * kWarps) kv8_split_kernel(const __grid_con
         for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
     float M[2] = {kNegBig, kNegBig}, l[2] = {0.f, 0.f};
 
-    const int32_t* table = a.b.table + (uint64_t)s * a.b.table_stride;
-    const uint32_t bpp = a.c.page_size / 16;
-    auto page_of = [&](int32_t blk) { return blk < b1 ? __ldg(table + (uint32_t)blk / bpp) : -1; };
-    auto fine = [&](int32_t page) { return page >= 0 && (uint32_t)page < a.c.n_pages; };
-    bool bad_page = false;
-    Block<HD> cur, nxt;
-    int32_t blk = b0 + (int32_t)warp;
-    int32_t page = page_of(blk), page1 = page_of(blk + kWarps);
-    if (fine(page)) load_block<HD>(cur, a.c, page, (uint32_t)blk % bpp, h, g, t);
-    for (; blk < b1; blk += kWarps) {
-        const bool have = fine(page);
-        page = page1;
-        page1 = page_of(blk + 2 * (int32_t)kWarps);
-        if (fine(page)) load_block<HD>(nxt, a.c, page, (uint32_t)(blk + kWarps) % bpp, h, g, t);
+    uint32_t slot = 0;
+    for (int32_t blk = b0 + (int32_t)warp; blk < b1; blk += kWarps) {
+        cp_async_wait<D - 2>();
+        const bool have = !(bad >> slot & 1);
+        Block<HD> cur;
+        if (have) read_block<HD>(cur, ring + slot * ring_bytes(HD), lane);
+        {
+            const uint32_t next = slot == 0 ? D - 1 : slot - 1;  // the slot that the block before left
+            fetch(next);
+        }
+        slot = slot + 1 == D ? 0 : slot + 1;
         if (have) {
             // ---- scores
             int acc[3][4];
@@ -347,11 +405,13 @@ __global__ void __launch_bounds__(32 * kWarps) kv8_split_kernel(const __grid_con
         } else {
             bad_page = true;
         }
-        cur = nxt;
     }
+    cp_async_wait<0>();
     if (bad_page && lane == 0) flag_error(a.err, DEV_ERR_POSITION);
 
-    // ---- the warps' partials
+    // ---- the warps' partials, over the rings
+    float(*so)[kRows][HD] = reinterpret_cast<float(*)[kRows][HD]>(ring_smem);
+    __syncthreads();
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         l[j] += __shfl_xor_sync(0xffffffffu, l[j], 4);
@@ -466,12 +526,6 @@ __host__ __device__ constexpr uint32_t tile_smem(int hd, int terms) {
            role_of(hd, terms).np * hd * (4 * role_of(hd, terms).stages + 2 * role_of(hd, terms).raw) + 1024;
 }
 static_assert(tile_smem(256, 2) <= 232448 && tile_smem(256, 1) <= 232448 && tile_smem(128, 1) <= 232448, "shared memory");
-
-__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(dst)), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 __device__ __forceinline__ bool bwait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
     if (mbar_try_wait(bar, parity)) return true;
@@ -930,8 +984,8 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
                 const uint32_t sub = (uint32_t)(b0 + (int32_t)(j * NB + piece / CPR / 16)) & ((1u << lb) - 1);
                 if ((uint32_t)page[i] < a.c.n_pages) {
                     const uint64_t o = (uint32_t)page[i] * a.c.page_stride + at[i] + sub * (16 * HD);
-                    cp_async16(raw + 16 * piece, a.c.k + o);
-                    cp_async16(raw + NP * HD + 16 * piece, a.c.v + o);
+                    cp_async<16>(raw + 16 * piece, a.c.k + o);
+                    cp_async<16>(raw + NP * HD + 16 * piece, a.c.v + o);
                 } else {
                     gone |= 1u << (rs * N + i);
                 }
@@ -1093,24 +1147,31 @@ Shape shape_of(const Kv8Cache& c, const Kv8Batch& b, uint32_t heads, uint32_t ty
     return r;
 }
 
+// the kernel's shared memory beyond the default, once per device (the attribute is the same for every call)
+template <auto kernel> cudaError_t opt_in(uint32_t smem) {
+    static std::atomic<bool> done[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    if (done[dev].load()) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e == cudaSuccess) done[dev] = true;
+    return e;
+}
+
 template <class T, int HD> cudaError_t launch(const Plan& p, bool tiles, cudaStream_t s) {
     if (tiles) {
         constexpr int terms = sizeof(T) == 4 ? 2 : 1;
         constexpr uint32_t smem = tile_smem(HD, terms), threads = 32 * (5 * role_of(HD, terms).rt + 5);
-        static std::atomic<bool> opted[64];
-        int dev = 0;
-        cudaError_t e = cudaGetDevice(&dev);
+        cudaError_t e = opt_in<kv8_tile_kernel<T, HD>>(smem);
         if (e != cudaSuccess) return e;
-        if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-        if (!opted[dev].load()) {
-            e = cudaFuncSetAttribute(kv8_tile_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-            if (e != cudaSuccess) return e;
-            opted[dev] = true;
-        }
         kv8_tile_kernel<T, HD><<<dim3(p.row_tiles * p.splits, p.a.c.kv_heads, p.a.b.n_seqs), threads, smem, s>>>(p);
     } else {
+        cudaError_t e = opt_in<kv8_split_kernel<T, HD>>(split_smem(HD));
+        if (e != cudaSuccess) return e;
         kv8_split_kernel<T, HD>
-            <<<dim3(p.splits, p.row_tiles * p.a.c.kv_heads, p.a.b.n_seqs), 32 * kWarps, 0, s>>>(p);
+            <<<dim3(p.splits, p.row_tiles * p.a.c.kv_heads, p.a.b.n_seqs), 32 * kWarps, split_smem(HD), s>>>(p);
     }
     if (p.splits > 1)
         kv8_join_kernel<T, HD><<<dim3((p.a.b.max_new + 3) / 4, p.a.heads, p.a.b.n_seqs), 128, 0, s>>>(p);
