@@ -456,28 +456,31 @@ __global__ void __launch_bounds__(32 * kWarps) kv8_split_kernel(const __grid_con
     }
 }
 
-// One warp per (token, head): the chunks' partials under their common maximum, in chunk order.
-template <class T, int HD> __global__ void __launch_bounds__(128) kv8_join_kernel(const __grid_constant__ Plan P) {
+// One CTA per (token, head): the chunks' partials under their common maximum. The warps deal the chunks
+// among themselves, each keeps the order of its own, and their sums are added in warp order.
+constexpr uint32_t kJoinWarps = 8;
+template <class T, int HD> __global__ void __launch_bounds__(32 * kJoinWarps) kv8_join_kernel(const __grid_constant__ Plan P) {
+    __shared__ float so[kJoinWarps][HD], sl[kJoinWarps];
     const Kv8AttnArgs& a = P.a;
-    const uint32_t lane = threadIdx.x & 31, head = blockIdx.y, s = blockIdx.z;
-    const int32_t i = (int32_t)(blockIdx.x * 4 + (threadIdx.x >> 5));
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, head = blockIdx.y, s = blockIdx.z;
+    const int32_t i = (int32_t)blockIdx.x;
     const Span sp = span_of(a, s);
     if (!sp.ok || i >= sp.n_new) return;
     const uint32_t h = head / P.group, row = (uint32_t)i * P.group + head % P.group, tile = row / P.tile_rows;
     const int32_t rows = sp.n_new * (int32_t)P.group;
     const int32_t seen = sp.base + (min((int32_t)((tile + 1) * P.tile_rows), rows) - 1) / (int32_t)P.group + 1;
     const uint32_t n = seen > 0 ? ((uint32_t)(seen + 15) / 16 + P.chunk - 1) / P.chunk : 1;
-    const uint64_t at = (((uint64_t)s * a.c.kv_heads + h) * P.row_tiles + tile) * P.splits;
+    const uint64_t at = ((((uint64_t)s * a.c.kv_heads + h) * P.row_tiles + tile) * P.splits) * P.tile_rows + row % P.tile_rows;
     float m = kNegBig;
-    for (uint32_t k = lane; k < n; k += 32) m = fmaxf(m, P.part_ml[(at + k) * P.tile_rows + row % P.tile_rows].x);
+    for (uint32_t k = lane; k < n; k += 32) m = fmaxf(m, P.part_ml[at + (uint64_t)k * P.tile_rows].x);
     m = warp_max(m);
     constexpr int N = HD / 64;
     float v[N][2], sum = 0.f;
 #pragma unroll
     for (int c = 0; c < N; ++c) v[c][0] = v[c][1] = 0.f;
 #pragma unroll 4
-    for (uint32_t k = 0; k < n; ++k) {
-        const uint64_t p = (at + k) * P.tile_rows + row % P.tile_rows;
+    for (uint32_t k = warp; k < n; k += kJoinWarps) {
+        const uint64_t p = at + (uint64_t)k * P.tile_rows;
         const float2 ml = P.part_ml[p];
         const float f = exp2_fast(ml.x - m);
         sum += rebase(ml.y, ml.x, m);
@@ -488,10 +491,21 @@ template <class T, int HD> __global__ void __launch_bounds__(128) kv8_join_kerne
             v[c][1] = fmaf(w.y, f, v[c][1]);
         }
     }
-    const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
-    T* out = static_cast<T*>(a.out) + (uint64_t)(sp.q0 + i) * a.out_stride + (uint64_t)head * HD;
 #pragma unroll
-    for (int c = 0; c < N; ++c) store2(out + 64 * c + 2 * lane, v[c][0] * inv, v[c][1] * inv);
+    for (int c = 0; c < N; ++c) *reinterpret_cast<float2*>(&so[warp][64 * c + 2 * lane]) = make_float2(v[c][0], v[c][1]);
+    if (lane == 0) sl[warp] = sum;
+    __syncthreads();
+    const uint32_t d = 2 * threadIdx.x;
+    if (d >= HD) return;
+    float2 o = make_float2(0.f, 0.f);
+    sum = 0.f;
+#pragma unroll
+    for (uint32_t w = 0; w < kJoinWarps; ++w) {
+        const float2 x = *reinterpret_cast<const float2*>(&so[w][d]);
+        o.x += x.x, o.y += x.y, sum += sl[w];
+    }
+    const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
+    store2(static_cast<T*>(a.out) + (uint64_t)(sp.q0 + i) * a.out_stride + (uint64_t)head * HD + d, o.x * inv, o.y * inv);
 }
 
 // ------------------------------------------------------------------ prompts
@@ -1174,7 +1188,7 @@ template <class T, int HD> cudaError_t launch(const Plan& p, bool tiles, cudaStr
             <<<dim3(p.splits, p.row_tiles * p.a.c.kv_heads, p.a.b.n_seqs), 32 * kWarps, split_smem(HD), s>>>(p);
     }
     if (p.splits > 1)
-        kv8_join_kernel<T, HD><<<dim3((p.a.b.max_new + 3) / 4, p.a.heads, p.a.b.n_seqs), 128, 0, s>>>(p);
+        kv8_join_kernel<T, HD><<<dim3(p.a.b.max_new, p.a.heads, p.a.b.n_seqs), 32 * kJoinWarps, 0, s>>>(p);
     return cudaGetLastError();
 }
 template <class T> cudaError_t by_dim(const Plan& p, bool tiles, cudaStream_t s) {
