@@ -19,7 +19,8 @@
 //      is as good as an f32 dot product. The K order inside the product is permuted so that a
 //      lane's fragment is 16 neighbouring bytes of a row: the codes reach the tensor cores as they
 //      were copied, with no conversion.
-//   V: mma.sync m16n8k16 in f16: codes are exact in f16, the weights two f16 parts (22 bits).
+//   V: mma.sync m16n8k16 in f16: codes are exact in f16, the weights two f16 parts (22 bits) for
+//      f32 outputs, one part for 16-bit outputs (half a step of 2^-11 each, as the prompt kernel).
 //      A lane loads 16 neighbouring dims of four positions and pairs positions with byte
 //      permutes; the weights move to the other operand's layout by two 8x8 transposes.
 //   The maximum is raised only when a score passes it by 2^8, so most blocks cost one vote.
@@ -196,6 +197,7 @@ __global__ void __launch_bounds__(32 * kWarps) kv8_split_kernel(const __grid_con
     constexpr int VC = HD <= 128 ? 1 : 2;        // V loads per position
     constexpr int MT = HD / 16;                  // 16-dim tiles of the output
     constexpr int LD = HD / 8 < 16 ? HD / 8 : 16;  // neighbouring dims of a lane's load
+    constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;  // f16 parts of a weight
     constexpr int D = ring_depth(HD);
     extern __shared__ __align__(16) uint8_t ring_smem[];
     __shared__ float2 sml[kWarps][kRows];
@@ -334,7 +336,8 @@ __global__ void __launch_bounds__(32 * kWarps) kv8_split_kernel(const __grid_con
             float x[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float d = fmaf((float)acc[2][j], 65536.f, fmaf((float)acc[1][j], 256.f, (float)acc[0][j]));
+                // (the two lower limbs together stay below 2^30)
+                const float d = fmaf((float)acc[2][j], 65536.f, (float)(acc[1][j] * 256 + acc[0][j]));
                 x[j] = fmaf(d, step[j & 1] * cur.sk, e);
             }
             if (blk * 16 + 15 > first_last) {
@@ -380,9 +383,11 @@ __global__ void __launch_bounds__(32 * kWarps) kv8_split_kernel(const __grid_con
                 const float p0 = w[2 * i] > 0.f ? w[2 * i] * mt[0] : 0.f;
                 const float p1 = w[2 * i + 1] > 0.f ? w[2 * i + 1] * mt[1] : 0.f;
                 const uint32_t hi = pack_h2(p0, p1);
-                const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi));
                 ph[i] = transpose8(hi);
-                pl[i] = transpose8(pack_h2(p0 - back.x, p1 - back.y));
+                if (TERMS == 2) {
+                    const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+                    pl[i] = transpose8(pack_h2(p0 - back.x, p1 - back.y));
+                }
             }
             // ---- O^T += V^T w^T: lane dims (128 i + 16 g) + 2 j, + 1 are rows g, g + 8 of tile j
 #pragma unroll
@@ -399,7 +404,7 @@ __global__ void __launch_bounds__(32 * kWarps) kv8_split_kernel(const __grid_con
                         const uint32_t a2 = codes_h2(hi, 0x4140), a3 = codes_h2(hi, 0x4342);
                         float(&d)[4] = o[(i * VW + q) * 2 + j];
                         mma_f16(d, a0, a1, a2, a3, ph[0], ph[1]);
-                        mma_f16(d, a0, a1, a2, a3, pl[0], pl[1]);
+                        if (TERMS == 2) mma_f16(d, a0, a1, a2, a3, pl[0], pl[1]);
                     }
                 }
         } else {

@@ -285,9 +285,8 @@ def _check(kv, lens, new, q, out, kind, scale=None):
     dim, at = q.shape[-1], 0
     scale = scale or 1 / np.sqrt(dim)
     eps = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}[kind]
-    # the prompt kernel holds the weights of 16-bit types in one f16 part (half a step: 2^-11)
-    heads = q.shape[1] // kv.k.shape[1]
-    weight_eps = 2.0 ** -11 if kind != "f32" and max(new) * heads >= 48 else 0.0
+    # the weights of 16-bit types are held in one f16 part (half a step: 2^-11)
+    weight_eps = 2.0 ** -11 if kind != "f32" else 0.0
     hq, ho = host(q), host(out).astype(np.float64)
     for s, (n, m) in enumerate(zip(lens, new)):
         k, v = (ref.values(a, b, kv.table[s], n) for a, b in ((kv.k, kv.ks), (kv.v, kv.vs)))
