@@ -6,15 +6,19 @@
 // row-major output is written in whole sectors without a transpose, and a product of few tokens
 // costs N = 16, not 128.
 //
-// One CTA works on tiles of 128 weight rows x NT tokens:
+// i8_gemm_kernel: one CTA works on tiles of 128 weight rows x NT tokens:
 //   warp 0     TMA producer: 128-byte K slices (128-byte swizzle) of both operands into a ring
 //              completing on mbarriers; ragged rows and a ragged K are zero-filled by TMA;
 //   warp 1     owns the tensor memory; one thread issues 4 MMAs (K = 32 each) per slice;
-//   warps 2-5  epilogue, one TMEM lane quadrant each; two accumulators, so a tile is written
-//              while the next one is multiplied.
+//   the others epilogue, one TMEM lane quadrant each (eight warps: two share a quadrant's columns);
+//              two accumulators, so a tile is written while the next one is multiplied.
 // With few tiles the K range is split over the CTAs of a cluster: the int32 partial tiles meet
 // through distributed shared memory, each CTA adding and writing its share of the columns, in
 // one launch, without a workspace, and exactly (integer sums).
+//
+// i8_gemm_pair_kernel: many tokens, 256 weight rows x 256 tokens on two CTAs that share their MMAs
+// (cta_group::2): each brings its own 128 weight rows and half of the tokens, so a slice costs each SM
+// 32 KB from L2 for 512 cycles of the tensor pipe where a CTA alone (128 x 256) needs 48 KB.
 //
 // Bound: few tokens -- HBM, every weight byte once; many tokens -- the tensor pipe.
 // Every wait is bounded; on a timeout the CTA records DEV_ERR_WAIT_TIMEOUT, lets its copies and
@@ -33,7 +37,6 @@ namespace {
 
 constexpr uint32_t kTileN = 128;                    // weight rows per tile (TMEM lanes)
 constexpr uint32_t kSlice = 128;                    // K values (bytes) per stage: one swizzle atom
-constexpr uint32_t kThreads = 192;
 constexpr uint32_t kMaxStages = 12;
 constexpr uint32_t kSmemCap = 200 * 1024;
 
@@ -43,6 +46,7 @@ struct Plan {
     uint32_t ntiles, mtiles;  // weight tiles, token tiles
     uint32_t slices;          // of K
     uint32_t split;           // CTAs (cluster) per tile
+    uint32_t group;           // token tiles that share a pass over the weight tiles
     uint32_t stages;
 };
 
@@ -57,9 +61,9 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, i
 __device__ __forceinline__ uint64_t smem_desc(uint32_t addr) {
     return (uint64_t)((addr & 0x3FFFFu) >> 4) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
-// kind::i8: signed 8-bit A and B, K-major, int32 D, M = 128
-__host__ __device__ constexpr uint32_t i8_idesc(uint32_t n) {
-    return (2u << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | ((128u >> 4) << 24);
+// kind::i8: signed 8-bit A and B, K-major, int32 D
+__host__ __device__ constexpr uint32_t i8_idesc(uint32_t n, uint32_t m = 128) {
+    return (2u << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | ((m >> 4) << 24);
 }
 __device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
@@ -96,22 +100,49 @@ __device__ __forceinline__ bool bwait(uint64_t* bar, uint32_t parity, volatile i
     return true;
 }
 
-// One output: token m, weight row n.
-template <class T>
-__device__ __forceinline__ void put(const I8GemmArgs& a, uint32_t m, uint32_t n, int32_t acc, float xs, float ws) {
-    float y = __fmul_rn(__fmul_rn(__int2float_rn(acc), xs), ws);
-    if (a.add) y = __fadd_rn(y, to_f32(static_cast<const T*>(a.add)[(uint64_t)m * a.add_stride + n]));
-    static_cast<T*>(a.y)[(uint64_t)m * a.y_stride + n] = from_f32<T>(y);
+// Tile number -> (weight tile, token tile): within a group of token tiles the tokens run fastest, so the
+// CTAs at work share few weight rows and the group's tokens stay in L2.
+__device__ __forceinline__ void tile_at(const Plan& P, uint32_t tile, uint32_t& nt, uint32_t& mt) {
+    const uint32_t per = P.group * P.ntiles, g = tile / per, r = tile % per;
+    const uint32_t here = min(P.group, P.mtiles - g * P.group);
+    nt = r / here;
+    mt = g * P.group + r % here;
 }
 
+// Outputs of weight row n for C tokens from m0, of which `count` exist. The sums' additions are read
+// before any output is written (they may share the buffer).
+template <class T, uint32_t C>
+__device__ __forceinline__ void put(const I8GemmArgs& a, uint32_t m0, uint32_t count, uint32_t n, const uint32_t (&acc)[C],
+                                    float ws) {
+    float add[C];
+    const T* ap = static_cast<const T*>(a.add) + (uint64_t)m0 * a.add_stride + n;
+    if (a.add) {
+#pragma unroll
+        for (uint32_t j = 0; j < C; ++j) add[j] = j < count ? to_f32(ap[j * a.add_stride]) : 0.f;
+    }
+    T* yp = static_cast<T*>(a.y) + (uint64_t)m0 * a.y_stride + n;
+#pragma unroll
+    for (uint32_t j = 0; j < C; ++j) {
+        if (j < count) {
+            float y = __fmul_rn(__fmul_rn(__int2float_rn((int32_t)acc[j]), __ldg(a.xs + m0 + j)), ws);
+            if (a.add) y = __fadd_rn(y, add[j]);
+            yp[j * a.y_stride] = from_f32<T>(y);
+        }
+    }
+}
+
+// epilogue warps of a tile of nt tokens
+__host__ __device__ constexpr uint32_t epi_warps(uint32_t nt) { return nt >= 128 ? 8 : 4; }
+__host__ __device__ constexpr uint32_t gemm_threads(uint32_t nt) { return 64 + 32 * epi_warps(nt); }
+
 template <uint32_t NT, class T>
-__global__ void __launch_bounds__(kThreads, 1) i8_gemm_kernel(const __grid_constant__ Plan P) {
+__global__ void __launch_bounds__(gemm_threads(NT), 1) i8_gemm_kernel(const __grid_constant__ Plan P) {
     namespace cg = cooperative_groups;
     extern __shared__ uint8_t raw_smem[];
     __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], d_full[2], d_empty[2], fin;
     __shared__ uint32_t tmem_base;
     __shared__ volatile int abort_flag;
-    constexpr uint32_t kStageBytes = (kTileN + NT) * kSlice;
+    constexpr uint32_t kStageBytes = (kTileN + NT) * kSlice, kEpi = epi_warps(NT), kThreads = gemm_threads(NT);
     constexpr uint32_t kCols = 2 * NT < 32 ? 32 : 2 * NT;  // two accumulators (a power of two)
     const I8GemmArgs& a = P.a;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -127,7 +158,7 @@ __global__ void __launch_bounds__(kThreads, 1) i8_gemm_kernel(const __grid_const
         }
         for (uint32_t i = 0; i < 2; ++i) {
             mbar_init(&d_full[i], 1);
-            mbar_init(&d_empty[i], 4);
+            mbar_init(&d_empty[i], kEpi);
         }
         mbar_init(&fin, 1);
         fence_barrier_init();
@@ -147,7 +178,9 @@ __global__ void __launch_bounds__(kThreads, 1) i8_gemm_kernel(const __grid_const
         if (lane == 0) {
             uint32_t n = 0;
             for (uint32_t tile = blockIdx.x / S; tile < tiles && !abort_flag; tile += gridDim.x / S) {
-                const int32_t w0 = (int32_t)(tile % P.ntiles * kTileN), x0 = (int32_t)(tile / P.ntiles * NT);
+                uint32_t nt, mt;
+                tile_at(P, tile, nt, mt);
+                const int32_t w0 = (int32_t)(nt * kTileN), x0 = (int32_t)(mt * NT);
                 for (uint32_t c = s0; c < s1; ++c, ++n) {
                     const uint32_t s = n % P.stages;
                     if (n >= P.stages && !bwait(&empty[s], (n / P.stages - 1) & 1, &abort_flag)) break;
@@ -186,36 +219,31 @@ __global__ void __launch_bounds__(kThreads, 1) i8_gemm_kernel(const __grid_const
             }
         }
     } else {
-        const uint32_t quad = warp & 3, r = quad * 32 + lane;
+        // columns of this warp: all, or half of them
+        constexpr uint32_t kHalf = NT / (kEpi / 4);
+        const uint32_t quad = warp & 3, r = quad * 32 + lane, c0 = (warp - 2) / 4 * kHalf;
         uint32_t it = 0;
         for (uint32_t tile = blockIdx.x / S; tile < tiles; tile += gridDim.x / S, ++it) {
-            const uint32_t n = tile % P.ntiles * kTileN + r, m0 = tile / P.ntiles * NT;
+            uint32_t nt, mt;
+            tile_at(P, tile, nt, mt);
+            const uint32_t n = nt * kTileN + r, m0 = mt * NT;
             const bool live = n < a.out;
             const float ws = live ? a.ws[n] : 0.f;
-            const uint32_t cols = min(NT, a.rows - m0);
+            const uint32_t cols = min(c0 + kHalf, a.rows - m0);
             bool ok = true;
             if (lane == 0) ok = bwait(&d_full[it & 1], (it / 2) & 1, &abort_flag);
             ok = __shfl_sync(0xffffffffu, (int)ok, 0);
             if (!ok) break;
             tc_after();
             const uint32_t at = tm + (it & 1) * NT + ((quad * 32) << 16);
-            if (S == 1) {
-                for (uint32_t c = 0; c < cols; c += 16) {
-                    uint32_t v[16];
-                    tmem_ld16(at + c, v);
-                    tmem_ld_wait();
-                    if (live) {
-#pragma unroll
-                        for (uint32_t j = 0; j < 16; ++j)
-                            if (c + j < cols) put<T>(a, m0 + c + j, n, (int32_t)v[j], a.xs[m0 + c + j], ws);
-                    }
-                }
-            } else {  // this CTA's partial tile for the cluster, over the ring (all slices are read)
-                int32_t* part = reinterpret_cast<int32_t*>(smem);
-                for (uint32_t c = 0; c < cols; c += 16) {
-                    uint32_t v[16];
-                    tmem_ld16(at + c, v);
-                    tmem_ld_wait();
+            int32_t* part = reinterpret_cast<int32_t*>(smem);  // (split: over the ring, whose slices are all read)
+            for (uint32_t c = c0; c < cols; c += 16) {
+                uint32_t v[16];
+                tmem_ld16(at + c, v);
+                tmem_ld_wait();
+                if (S == 1) {
+                    if (live) put<T, 16>(a, m0 + c, cols - c, n, v, ws);
+                } else {  // this CTA's partial tile for the cluster
 #pragma unroll
                     for (uint32_t j = 0; j < 16; ++j) part[(c + j) * kTileN + r] = (int32_t)v[j];
                 }
@@ -229,14 +257,16 @@ __global__ void __launch_bounds__(kThreads, 1) i8_gemm_kernel(const __grid_const
     if (S > 1) {
         cg::cluster_group cl = cg::this_cluster();
         cl.sync();
-        const uint32_t tile = blockIdx.x / S, n0 = tile % P.ntiles * kTileN, m0 = tile / P.ntiles * NT;
+        uint32_t nt, mt;
+        tile_at(P, blockIdx.x / S, nt, mt);
+        const uint32_t n0 = nt * kTileN, m0 = mt * NT;
         const uint32_t cols = min(NT, a.rows - m0);
         const int32_t* part = reinterpret_cast<const int32_t*>(smem);
         for (uint32_t i = rank * kThreads + tid; i < cols * kTileN && !abort_flag; i += S * kThreads) {
-            int32_t acc = 0;
-            for (uint32_t k = 0; k < S; ++k) acc += *cl.map_shared_rank(part + i, k);
+            uint32_t acc[1] = {0};
+            for (uint32_t k = 0; k < S; ++k) acc[0] += (uint32_t)*cl.map_shared_rank(part + i, k);
             const uint32_t m = m0 + i / kTileN, n = n0 + i % kTileN;
-            if (n < a.out) put<T>(a, m, n, acc, a.xs[m], a.ws[n]);
+            if (n < a.out) put<T, 1>(a, m, 1, n, acc, a.ws[n]);
         }
         cl.sync();  // the others read this CTA's tile until here
     }
@@ -245,6 +275,164 @@ __global__ void __launch_bounds__(kThreads, 1) i8_gemm_kernel(const __grid_const
     if (tid == 0 && abort_flag) flag_error(a.err, DEV_ERR_WAIT_TIMEOUT);
     if (warp == 1)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "r"(kCols) : "memory");
+}
+
+// ------------------------------------------------------------------ two CTAs, 256 x 256
+constexpr uint32_t kPairThreads = 320, kPairStage = 2 * 128 * kSlice, kPairStages = 6, kPairTokens = 256;
+
+// the address of a shared-memory object of this CTA in the cluster's CTA `rank`
+__device__ __forceinline__ uint32_t in_cta(const void* p, uint32_t rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr(p)), "r"(rank));
+    return r;
+}
+// a load into this CTA's shared memory that completes on a barrier of the pair's first CTA
+__device__ __forceinline__ void tma_load_pair(void* dst, const CUtensorMap* map, int32_t x, int32_t y, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+            smem_addr(dst)),
+        "l"(map), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void mma_i8_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+// arrive on `bar` of both CTAs once the MMAs issued so far have ended
+__device__ __forceinline__ void commit_pair(uint64_t* bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_addr(bar)),
+        "h"((uint16_t)3)
+        : "memory");
+}
+__device__ __forceinline__ void arrive_remote(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// one lane of a converged warp, in the form that tells the compiler so
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(p));
+    return p != 0;
+}
+
+template <class T>
+__global__ void __launch_bounds__(kPairThreads, 1) i8_gemm_pair_kernel(const __grid_constant__ Plan P) {
+    namespace cg = cooperative_groups;
+    extern __shared__ uint8_t raw_smem[];
+    // full: of the first CTA, for both; empty, d_full: of each; d_empty: of the first CTA, from both
+    __shared__ __align__(8) uint64_t full[kPairStages], empty[kPairStages], d_full[2], d_empty[2], fin;
+    __shared__ uint32_t tmem_base;
+    __shared__ volatile int abort_flag;
+    const I8GemmArgs& a = P.a;
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    cg::cluster_group cl = cg::this_cluster();
+    const uint32_t rank = cl.block_rank(), tiles = P.ntiles * P.mtiles, first = blockIdx.x / 2, stride = gridDim.x / 2;
+    uint8_t* smem = raw_smem + ((1024u - (smem_addr(raw_smem) & 1023u)) & 1023u);
+    if (tid == 0) {
+        abort_flag = 0;
+        for (uint32_t i = 0; i < kPairStages; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], 1);
+        }
+        for (uint32_t i = 0; i < 2; ++i) {
+            mbar_init(&d_full[i], 1);
+            mbar_init(&d_empty[i], 16);  // eight epilogue warps of each CTA
+        }
+        mbar_init(&fin, 1);
+        fence_barrier_init();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_base)),
+                     "r"(512)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_before();
+    __syncwarp();
+    cl.sync();  // barriers of both CTAs are there
+    tc_after();
+    const uint32_t tm = tmem_base;
+
+    if (warp == 0) {
+        if (elect_one()) {
+            uint32_t n = 0;
+            for (uint32_t tile = first; tile < tiles && !abort_flag; tile += stride) {
+                uint32_t nt, mt;
+                tile_at(P, tile, nt, mt);
+                const int32_t w0 = (int32_t)(nt * 256 + rank * 128), x0 = (int32_t)(mt * kPairTokens + rank * 128);
+                for (uint32_t c = 0; c < P.slices; ++c, ++n) {
+                    const uint32_t s = n % kPairStages;
+                    if (n >= kPairStages && !bwait(&empty[s], (n / kPairStages - 1) & 1, &abort_flag)) break;
+                    uint8_t* dst = smem + s * kPairStage;
+                    const uint32_t bar = in_cta(&full[s], 0);
+                    if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * kPairStage);
+                    tma_load_pair(dst, &P.wmap, (int32_t)(c * kSlice), w0, bar);
+                    tma_load_pair(dst + 128 * kSlice, &P.xmap, (int32_t)(c * kSlice), x0, bar);
+                }
+            }
+            if (abort_flag && rank == 0)  // copies in flight land before the CTAs leave
+                for (uint32_t s = 0; s < kPairStages && s < n; ++s) mbar_wait(&full[s], ((n - 1 - s) / kPairStages) & 1);
+        }
+    } else if (warp == 1) {
+        if (rank == 0 && elect_one()) {
+            uint32_t n = 0, it = 0;
+            for (uint32_t tile = first; tile < tiles && !abort_flag; tile += stride, ++it) {
+                const uint32_t acc = tm + (it & 1) * kPairTokens;
+                if (it >= 2 && !bwait(&d_empty[it & 1], (it / 2 - 1) & 1, &abort_flag)) break;
+                tc_after();
+                for (uint32_t c = 0; c < P.slices; ++c, ++n) {
+                    const uint32_t s = n % kPairStages;
+                    if (!bwait(&full[s], (n / kPairStages) & 1, &abort_flag)) break;
+                    tc_after();
+                    const uint32_t at = smem_addr(smem + s * kPairStage);
+                    const uint64_t da = smem_desc(at), db = smem_desc(at + 128 * kSlice);
+#pragma unroll
+                    for (uint32_t k = 0; k < kSlice / 32; ++k)
+                        mma_i8_pair(acc, da + 2 * k, db + 2 * k, i8_idesc(kPairTokens, 256), c > 0 || k > 0);
+                    commit_pair(&empty[s]);
+                }
+                commit_pair(&d_full[it & 1]);
+            }
+            if (abort_flag) {  // the MMAs in flight end before the tensor memory is freed
+                commit_pair(&fin);
+                mbar_wait(&fin, 0);
+            }
+        }
+    } else {
+        const uint32_t quad = warp & 3, r = quad * 32 + lane, c0 = (warp - 2) / 4 * 128;
+        uint32_t it = 0;
+        for (uint32_t tile = first; tile < tiles; tile += stride, ++it) {
+            uint32_t nt, mt;
+            tile_at(P, tile, nt, mt);
+            const uint32_t n = nt * 256 + rank * 128 + r, m0 = mt * kPairTokens, cols = min(c0 + 128, a.rows - m0);
+            const bool live = n < a.out;
+            const float ws = live ? a.ws[n] : 0.f;
+            bool ok = true;
+            if (lane == 0) ok = bwait(&d_full[it & 1], (it / 2) & 1, &abort_flag);
+            ok = __shfl_sync(0xffffffffu, (int)ok, 0);
+            if (!ok) break;
+            tc_after();
+            const uint32_t at = tm + (it & 1) * kPairTokens + ((quad * 32) << 16);
+            for (uint32_t c = c0; c < cols; c += 16) {
+                uint32_t v[16];
+                tmem_ld16(at + c, v);
+                tmem_ld_wait();
+                if (live) put<T, 16>(a, m0 + c, cols - c, n, v, ws);
+            }
+            tc_before();
+            __syncwarp();
+            if (lane == 0) arrive_remote(in_cta(&d_empty[it & 1], 0));
+        }
+    }
+    __syncwarp();
+    tc_before();
+    cl.sync();  // the pair's MMAs and copies have ended, nothing more arrives at the other's barriers
+    if (tid == 0 && abort_flag) flag_error(a.err, DEV_ERR_WAIT_TIMEOUT);
+    if (warp == 1)
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tm), "r"(512) : "memory");
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encoder() {
@@ -269,6 +457,39 @@ bool make_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, 
                                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// the kernel's shared memory beyond the default, once per device
+template <auto kernel> cudaError_t opt_in(uint32_t smem) {
+    static std::atomic<bool> done[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    if (done[dev].load()) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e == cudaSuccess) done[dev] = true;
+    return e;
+}
+
+// grid and shared memory of a launch in clusters of `cluster` CTAs
+template <auto kernel> cudaError_t go(const Plan& p, uint32_t grid, uint32_t threads, uint32_t smem, uint32_t cluster, cudaStream_t s) {
+    cudaError_t e = opt_in<kernel>(kSmemCap + 1024);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = cluster;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+constexpr uint32_t kGroup = 16;  // token tiles per pass over the weights
+
 template <uint32_t NT, class T> cudaError_t launch(Plan& p, int sms, cudaStream_t s) {
     const I8GemmArgs& a = p.a;
     constexpr uint32_t stage = (kTileN + NT) * kSlice;
@@ -277,45 +498,46 @@ template <uint32_t NT, class T> cudaError_t launch(Plan& p, int sms, cudaStream_
         return cudaErrorInvalidValue;
     p.ntiles = (a.out + kTileN - 1) / kTileN;
     p.mtiles = (a.rows + NT - 1) / NT;
-    p.slices = (a.cols + kSlice - 1) / kSlice;
+    p.group = kGroup;
     p.stages = std::min(kMaxStages, kSmemCap / stage);
     const uint64_t tiles = (uint64_t)p.ntiles * p.mtiles;
     if (tiles > 0x7fffffffull) return cudaErrorInvalidValue;
-    // split K while the tiles leave SMs free and every CTA keeps a few slices
-    p.split = 1;
-    while (p.split < 8 && tiles * p.split * 2 <= (uint64_t)sms && p.slices >= 4 * p.split) p.split *= 2;
+    // split K over as many CTAs as the SMs have room for, every CTA keeping four slices at least
+    p.split = (uint32_t)std::min<uint64_t>({8, std::max<uint64_t>(1, sms / tiles), std::max(1u, p.slices / 4)});
     // a cluster's partial tile lies over the ring
     const uint32_t smem = std::max(p.stages * stage, p.split > 1 ? NT * kTileN * 4 : 0u) + 1024;
-    static std::atomic<bool> opted[64];
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-    if (!opted[dev].load()) {
-        e = cudaFuncSetAttribute(i8_gemm_kernel<NT, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemCap + 1024);
-        if (e != cudaSuccess) return e;
-        opted[dev] = true;
-    }
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(p.split > 1 ? (uint32_t)tiles * p.split : (uint32_t)std::min<uint64_t>(tiles, sms));
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = p.split;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, i8_gemm_kernel<NT, T>, p);
+    const uint32_t grid = p.split > 1 ? (uint32_t)tiles * p.split : (uint32_t)std::min<uint64_t>(tiles, sms);
+    return go<i8_gemm_kernel<NT, T>>(p, grid, gemm_threads(NT), smem, p.split, s);
+}
+
+template <class T> cudaError_t launch_pair(Plan& p, int sms, cudaStream_t s) {
+    const I8GemmArgs& a = p.a;
+    if (!make_map(&p.wmap, a.w, a.out, a.cols, a.w_stride, 128) ||
+        !make_map(&p.xmap, a.x, a.rows, a.cols, a.x_stride, 128))
+        return cudaErrorInvalidValue;
+    p.ntiles = (a.out + 255) / 256;
+    p.mtiles = (a.rows + kPairTokens - 1) / kPairTokens;
+    p.group = kGroup;
+    p.split = 1;
+    p.stages = kPairStages;
+    const uint64_t tiles = (uint64_t)p.ntiles * p.mtiles;
+    if (tiles > 0x7fffffffull) return cudaErrorInvalidValue;
+    static_assert(kPairStages * kPairStage <= kSmemCap, "shared memory");
+    const uint32_t grid = 2 * (uint32_t)std::min<uint64_t>(tiles, sms / 2);
+    return go<i8_gemm_pair_kernel<T>>(p, grid, kPairThreads, kPairStages * kPairStage + 1024, 2, s);
 }
 
 template <class T> cudaError_t by_tokens(Plan& p, int sms, cudaStream_t s) {
-    if (p.a.rows <= 16) return launch<16, T>(p, sms, s);
-    if (p.a.rows <= 32) return launch<32, T>(p, sms, s);
-    if (p.a.rows <= 64) return launch<64, T>(p, sms, s);
-    if (p.a.rows <= 128) return launch<128, T>(p, sms, s);
-    return launch<256, T>(p, sms, s);
+    const uint64_t rows = p.a.rows, ntiles = (p.a.out + kTileN - 1) / kTileN;
+    p.slices = (p.a.cols + kSlice - 1) / kSlice;
+    auto tiles = [&](uint64_t nt) { return ntiles * ((rows + nt - 1) / nt); };
+    if (rows > 128 && tiles(256) / 2 >= (uint64_t)sms / 2) return launch_pair<T>(p, sms, s);
+    // fewer tiles than SMs: narrower ones
+    if (rows > 128 && tiles(256) >= (uint64_t)sms) return launch<256, T>(p, sms, s);
+    if (rows > 64 && (rows <= 128 || tiles(128) >= (uint64_t)sms)) return launch<128, T>(p, sms, s);
+    if (rows > 32) return launch<64, T>(p, sms, s);
+    if (rows > 16) return launch<32, T>(p, sms, s);
+    return launch<16, T>(p, sms, s);
 }
 
 }  // namespace
