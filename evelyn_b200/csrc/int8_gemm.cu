@@ -29,6 +29,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 
 #include "int8.cuh"
 
@@ -39,6 +40,7 @@ constexpr uint32_t kTileN = 128;                    // weight rows per tile (TME
 constexpr uint32_t kSlice = 128;                    // K values (bytes) per stage: one swizzle atom
 constexpr uint32_t kMaxStages = 12;
 constexpr uint32_t kSmemCap = 200 * 1024;
+constexpr uint32_t kTwoCtas = 32;                   // tokens of a tile up to which two CTAs share an SM
 
 struct Plan {
     CUtensorMap wmap, xmap;
@@ -129,6 +131,26 @@ __device__ __forceinline__ void put(const I8GemmArgs& a, uint32_t m0, uint32_t c
             yp[j * a.y_stride] = from_f32<T>(y);
         }
     }
+}
+
+// Outputs of token m for weight rows n .. n + 3, as far as they exist.
+template <class T> __device__ __forceinline__ void put_row(const I8GemmArgs& a, uint32_t m, uint32_t n, const uint32_t (&acc)[4]) {
+    const float xs = __ldg(a.xs + m);
+    const T* ap = static_cast<const T*>(a.add) + (uint64_t)m * a.add_stride + n;
+    T* yp = static_cast<T*>(a.y) + (uint64_t)m * a.y_stride + n;
+    float add[4], ws[4];
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) {
+        ws[j] = n + j < a.out ? __ldg(a.ws + n + j) : 0.f;
+        add[j] = a.add && n + j < a.out ? to_f32(ap[j]) : 0.f;
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j)
+        if (n + j < a.out) {
+            float y = __fmul_rn(__fmul_rn(__int2float_rn((int32_t)acc[j]), xs), ws[j]);
+            if (a.add) y = __fadd_rn(y, add[j]);
+            yp[j] = from_f32<T>(y);
+        }
 }
 
 // epilogue warps of a tile of nt tokens
@@ -262,11 +284,20 @@ __global__ void __launch_bounds__(gemm_threads(NT), 1) i8_gemm_kernel(const __gr
         const uint32_t n0 = nt * kTileN, m0 = mt * NT;
         const uint32_t cols = min(NT, a.rows - m0);
         const int32_t* part = reinterpret_cast<const int32_t*>(smem);
-        for (uint32_t i = rank * kThreads + tid; i < cols * kTileN && !abort_flag; i += S * kThreads) {
-            uint32_t acc[1] = {0};
-            for (uint32_t k = 0; k < S; ++k) acc[0] += (uint32_t)*cl.map_shared_rank(part + i, k);
-            const uint32_t m = m0 + i / kTileN, n = n0 + i % kTileN;
-            if (n < a.out) put<T, 1>(a, m, 1, n, acc, a.ws[n]);
+        // four neighbouring weight rows of a token per thread; every CTA's share is on its way before the
+        // first is added
+        for (uint32_t i = rank * kThreads + tid; i < cols * (kTileN / 4) && !abort_flag; i += S * kThreads) {
+            const uint32_t c = i / (kTileN / 4), r = i % (kTileN / 4) * 4;
+            int4 v[8];
+#pragma unroll
+            for (uint32_t k = 0; k < 8; ++k)
+                if (k < S) v[k] = *reinterpret_cast<const int4*>(cl.map_shared_rank(part + c * kTileN + r, k));
+            int4 sum = v[0];
+#pragma unroll
+            for (uint32_t k = 1; k < 8; ++k)
+                if (k < S) sum.x += v[k].x, sum.y += v[k].y, sum.z += v[k].z, sum.w += v[k].w;
+            const uint32_t acc[4] = {(uint32_t)sum.x, (uint32_t)sum.y, (uint32_t)sum.z, (uint32_t)sum.w};
+            put_row<T>(a, m0 + c, n0 + r, acc);
         }
         cl.sync();  // the others read this CTA's tile until here
     }
@@ -488,26 +519,93 @@ template <auto kernel> cudaError_t go(const Plan& p, uint32_t grid, uint32_t thr
     return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
+// Clusters of `cluster` CTAs that the device runs at once (a cluster stays inside one GPC, so this is less
+// than SMs / cluster); looked up once per device.
+template <auto kernel> uint32_t clusters_at_once(uint32_t threads, uint32_t smem, uint32_t cluster) {
+    static std::atomic<int> known[64][9];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64 || cluster > 8) return 0;
+    int n = known[dev][cluster].load();
+    if (!n) {
+        if (opt_in<kernel>(kSmemCap + 1024) != cudaSuccess) return 0;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(cluster);
+        cfg.blockDim = dim3(threads);
+        cfg.dynamicSmemBytes = smem;
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = cluster;
+        at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+        cfg.attrs = at;
+        cfg.numAttrs = 1;
+        if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) n = 0;
+        known[dev][cluster] = n ? n : -1;
+    }
+    return n > 0 ? (uint32_t)n : 0;
+}
+
 constexpr uint32_t kGroup = 16;  // token tiles per pass over the weights
 
-template <uint32_t NT, class T> cudaError_t launch(Plan& p, int sms, cudaStream_t s) {
+__host__ __device__ constexpr uint32_t stage_bytes(uint32_t nt) { return (kTileN + nt) * kSlice; }
+constexpr uint32_t ctas_per_sm(uint32_t nt) { return nt <= kTwoCtas ? 2 : 1; }
+constexpr uint32_t ring_stages(uint32_t nt) {
+    const uint32_t n = kSmemCap / ctas_per_sm(nt) / stage_bytes(nt);
+    return n < kMaxStages ? n : kMaxStages;
+}
+// the ring; a cluster's partial tile lies over it
+constexpr uint32_t gemm_smem(uint32_t nt) {
+    const uint32_t ring = ring_stages(nt) * stage_bytes(nt), part = nt * kTileN * 4;
+    return (ring > part ? ring : part) + 1024;
+}
+
+// How a product is cut: nt 0 is the pair kernel.
+struct Cut {
+    uint32_t nt = 0, split = 1;
+    double cost = 1e30;
+};
+// Estimated SM cycles, from what the kernels measured: a slice costs the tensor pipe 2 cycles per token
+// column, and L2 3.1 cycles per 128-byte row while all SMs load (fewer CTAs get up to twice that each);
+// a tile's outputs cost 60 cycles per column of an epilogue warp (100 with an addition; a split's
+// exchange 60 more), a launch 4000.
+double cost_of(uint32_t nt, uint64_t tiles, uint32_t split, uint32_t slices, bool add, int sms) {
+    const uint32_t pair = nt ? 1 : 2, cols = nt ? nt : 256, rows = nt ? kTileN + nt : 256;
+    const double slots = nt ? (double)sms * ctas_per_sm(nt) : sms / 2, units = (double)tiles * split;
+    const double busy = std::min(1.0, units * pair / ((double)sms * (nt ? ctas_per_sm(nt) : 1)));
+    const double share = nt ? ctas_per_sm(nt) : 1;  // CTAs that share an SM's pipes and bandwidth
+    const double load = 3.1 * rows * share * std::max(0.5, busy), mma = 2.0 * cols * share;
+    const double per = (double)slices / split * std::max(load, mma), out = ((add ? 100.0 : 60.0) + (split > 1 ? 60.0 : 0.0)) * cols / (cols >= 128 ? 2 : 1);
+    const double waves = std::ceil(units / slots);
+    // outputs of all tiles but the last are written behind the next tile's products
+    return 4000.0 + waves * per + out + (waves - 1) * std::max(0.0, out - per);
+}
+
+template <uint32_t NT, class T> void consider(Cut& best, const Plan& p, int sms) {
+    const uint64_t tiles = ((p.a.out + kTileN - 1) / kTileN) * (uint64_t)((p.a.rows + NT - 1) / NT);
+    if (NT > 16 && p.a.rows <= NT / 2) return;  // half of the columns would be empty
+    for (uint32_t k = 1; k <= 8; ++k) {
+        if (k > 1) {  // a split's clusters all run at once, every CTA with four slices at least
+            if (k * tiles > 2ull * sms || p.slices < 4 * k) break;
+            if (tiles > clusters_at_once<i8_gemm_kernel<NT, T>>(gemm_threads(NT), gemm_smem(NT), k)) continue;
+        }
+        const double c = cost_of(NT, tiles, k, p.slices, p.a.add != nullptr, sms);
+        if (c < best.cost) best.nt = NT, best.split = k, best.cost = c;
+    }
+}
+
+template <uint32_t NT, class T> cudaError_t launch(Plan& p, uint32_t split, int sms, cudaStream_t s) {
     const I8GemmArgs& a = p.a;
-    constexpr uint32_t stage = (kTileN + NT) * kSlice;
     if (!make_map(&p.wmap, a.w, a.out, a.cols, a.w_stride, kTileN) ||
         !make_map(&p.xmap, a.x, a.rows, a.cols, a.x_stride, NT))
         return cudaErrorInvalidValue;
     p.ntiles = (a.out + kTileN - 1) / kTileN;
     p.mtiles = (a.rows + NT - 1) / NT;
     p.group = kGroup;
-    p.stages = std::min(kMaxStages, kSmemCap / stage);
+    p.stages = ring_stages(NT);
+    p.split = split;
     const uint64_t tiles = (uint64_t)p.ntiles * p.mtiles;
     if (tiles > 0x7fffffffull) return cudaErrorInvalidValue;
-    // split K over as many CTAs as the SMs have room for, every CTA keeping four slices at least
-    p.split = (uint32_t)std::min<uint64_t>({8, std::max<uint64_t>(1, sms / tiles), std::max(1u, p.slices / 4)});
-    // a cluster's partial tile lies over the ring
-    const uint32_t smem = std::max(p.stages * stage, p.split > 1 ? NT * kTileN * 4 : 0u) + 1024;
-    const uint32_t grid = p.split > 1 ? (uint32_t)tiles * p.split : (uint32_t)std::min<uint64_t>(tiles, sms);
-    return go<i8_gemm_kernel<NT, T>>(p, grid, gemm_threads(NT), smem, p.split, s);
+    const uint32_t grid = split > 1 ? (uint32_t)tiles * split : (uint32_t)std::min<uint64_t>(tiles, (uint64_t)sms * ctas_per_sm(NT));
+    return go<i8_gemm_kernel<NT, T>>(p, grid, gemm_threads(NT), gemm_smem(NT), split, s);
 }
 
 template <class T> cudaError_t launch_pair(Plan& p, int sms, cudaStream_t s) {
@@ -528,16 +626,26 @@ template <class T> cudaError_t launch_pair(Plan& p, int sms, cudaStream_t s) {
 }
 
 template <class T> cudaError_t by_tokens(Plan& p, int sms, cudaStream_t s) {
-    const uint64_t rows = p.a.rows, ntiles = (p.a.out + kTileN - 1) / kTileN;
     p.slices = (p.a.cols + kSlice - 1) / kSlice;
-    auto tiles = [&](uint64_t nt) { return ntiles * ((rows + nt - 1) / nt); };
-    if (rows > 128 && tiles(256) / 2 >= (uint64_t)sms / 2) return launch_pair<T>(p, sms, s);
-    // fewer tiles than SMs: narrower ones
-    if (rows > 128 && tiles(256) >= (uint64_t)sms) return launch<256, T>(p, sms, s);
-    if (rows > 64 && (rows <= 128 || tiles(128) >= (uint64_t)sms)) return launch<128, T>(p, sms, s);
-    if (rows > 32) return launch<64, T>(p, sms, s);
-    if (rows > 16) return launch<32, T>(p, sms, s);
-    return launch<16, T>(p, sms, s);
+    Cut best;
+    consider<16, T>(best, p, sms);
+    consider<32, T>(best, p, sms);
+    consider<64, T>(best, p, sms);
+    consider<128, T>(best, p, sms);
+    consider<256, T>(best, p, sms);
+    if (p.a.rows > 128) {
+        const uint64_t tiles = (uint64_t)((p.a.out + 255) / 256) * ((p.a.rows + 255) / 256);
+        const double c = cost_of(0, tiles, 1, p.slices, p.a.add != nullptr, sms);
+        if (c < best.cost) best.nt = 0, best.cost = c;
+    }
+    switch (best.nt) {
+        case 0: return launch_pair<T>(p, sms, s);
+        case 16: return launch<16, T>(p, best.split, sms, s);
+        case 32: return launch<32, T>(p, best.split, sms, s);
+        case 64: return launch<64, T>(p, best.split, sms, s);
+        case 128: return launch<128, T>(p, best.split, sms, s);
+        default: return launch<256, T>(p, best.split, sms, s);
+    }
 }
 
 }  // namespace
