@@ -87,6 +87,19 @@ __device__ __forceinline__ void tmem_ld16(uint32_t t, uint32_t (&v)[16]) {
         : "r"(t)
         : "memory");
 }
+__device__ __forceinline__ void tmem_ld32(uint32_t t, uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
+          "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
+          "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(t)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ldc(uint32_t t, uint32_t (&v)[16]) { tmem_ld16(t, v); }
+__device__ __forceinline__ void tmem_ldc(uint32_t t, uint32_t (&v)[32]) { tmem_ld32(t, v); }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ bool bwait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
@@ -111,27 +124,32 @@ __device__ __forceinline__ void tile_at(const Plan& P, uint32_t tile, uint32_t& 
     mt = g * P.group + r % here;
 }
 
-// Outputs of weight row n for C tokens from m0, of which `count` exist. The sums' additions are read
-// before any output is written (they may share the buffer).
-template <class T, uint32_t C>
-__device__ __forceinline__ void put(const I8GemmArgs& a, uint32_t m0, uint32_t count, uint32_t n, const uint32_t (&acc)[C],
-                                    float ws) {
-    float add[C];
-    const T* ap = static_cast<const T*>(a.add) + (uint64_t)m0 * a.add_stride + n;
-    if (a.add) {
+// Outputs of weight row n for the tokens m0 + [c0, c1), accumulators at `at` + column: C columns at a time,
+// the next ones' additions on their way meanwhile (they may share y's buffer: each is read before its
+// own output is written, and no other output overlaps it).
+// (Loads have no conditions and are widened where they are used: a branch or a conversion beside
+// each would wait for it before the next is issued.)
+template <class T, uint32_t C> struct Outputs {
+    T add[C];
+    __device__ __forceinline__ void fetch(const I8GemmArgs& a, uint32_t m, uint32_t count, uint32_t n, bool live) {
+        if (!a.add || !live) return;
+        const T* p = static_cast<const T*>(a.add) + (uint64_t)m * a.add_stride + n;
 #pragma unroll
-        for (uint32_t j = 0; j < C; ++j) add[j] = j < count ? to_f32(ap[j * a.add_stride]) : 0.f;
+        for (uint32_t j = 0; j < C; ++j) add[j] = p[min(j, count - 1) * a.add_stride];
     }
-    T* yp = static_cast<T*>(a.y) + (uint64_t)m0 * a.y_stride + n;
+    __device__ __forceinline__ void put(const I8GemmArgs& a, uint32_t m, uint32_t count, uint32_t n, bool live,
+                                        const uint32_t (&acc)[C], float ws) const {
+        if (!live) return;
+        T* p = static_cast<T*>(a.y) + (uint64_t)m * a.y_stride + n;
 #pragma unroll
-    for (uint32_t j = 0; j < C; ++j) {
-        if (j < count) {
-            float y = __fmul_rn(__fmul_rn(__int2float_rn((int32_t)acc[j]), __ldg(a.xs + m0 + j)), ws);
-            if (a.add) y = __fadd_rn(y, add[j]);
-            yp[j * a.y_stride] = from_f32<T>(y);
-        }
+        for (uint32_t j = 0; j < C; ++j)
+            if (j < count) {
+                float y = __fmul_rn(__fmul_rn(__int2float_rn((int32_t)acc[j]), __ldg(a.xs + m + j)), ws);
+                if (a.add) y = __fadd_rn(y, to_f32(add[j]));
+                p[j * a.y_stride] = from_f32<T>(y);
+            }
     }
-}
+};
 
 // Outputs of token m for weight rows n .. n + 3, as far as they exist.
 template <class T> __device__ __forceinline__ void put_row(const I8GemmArgs& a, uint32_t m, uint32_t n, const uint32_t (&acc)[4]) {
@@ -252,6 +270,9 @@ __global__ void __launch_bounds__(gemm_threads(NT), 1) i8_gemm_kernel(const __gr
             const bool live = n < a.out;
             const float ws = live ? a.ws[n] : 0.f;
             const uint32_t cols = min(c0 + kHalf, a.rows - m0);
+            constexpr uint32_t C = NT <= kTwoCtas ? 16 : 32;  // (two CTAs share the SM's registers)
+            Outputs<T, C> out, next;
+            if (S == 1 && c0 < cols) out.fetch(a, m0 + c0, cols - c0, n, live);
             bool ok = true;
             if (lane == 0) ok = bwait(&d_full[it & 1], (it / 2) & 1, &abort_flag);
             ok = __shfl_sync(0xffffffffu, (int)ok, 0);
@@ -259,15 +280,17 @@ __global__ void __launch_bounds__(gemm_threads(NT), 1) i8_gemm_kernel(const __gr
             tc_after();
             const uint32_t at = tm + (it & 1) * NT + ((quad * 32) << 16);
             int32_t* part = reinterpret_cast<int32_t*>(smem);  // (split: over the ring, whose slices are all read)
-            for (uint32_t c = c0; c < cols; c += 16) {
-                uint32_t v[16];
-                tmem_ld16(at + c, v);
+            for (uint32_t c = c0; c < cols; c += C) {
+                uint32_t v[C];
+                tmem_ldc(at + c, v);
+                if (S == 1 && c + C < cols) next.fetch(a, m0 + c + C, cols - c - C, n, live);
                 tmem_ld_wait();
                 if (S == 1) {
-                    if (live) put<T, 16>(a, m0 + c, cols - c, n, v, ws);
+                    out.put(a, m0 + c, cols - c, n, live, v, ws);
+                    out = next;
                 } else {  // this CTA's partial tile for the cluster
 #pragma unroll
-                    for (uint32_t j = 0; j < 16; ++j) part[(c + j) * kTileN + r] = (int32_t)v[j];
+                    for (uint32_t j = 0; j < C; ++j) part[(c + j) * kTileN + r] = (int32_t)v[j];
                 }
             }
             tc_before();
@@ -441,17 +464,21 @@ __global__ void __launch_bounds__(kPairThreads, 1) i8_gemm_pair_kernel(const __g
             const uint32_t n = nt * 256 + rank * 128 + r, m0 = mt * kPairTokens, cols = min(c0 + 128, a.rows - m0);
             const bool live = n < a.out;
             const float ws = live ? a.ws[n] : 0.f;
+            Outputs<T, 32> out, next;
+            if (c0 < cols) out.fetch(a, m0 + c0, cols - c0, n, live);
             bool ok = true;
             if (lane == 0) ok = bwait(&d_full[it & 1], (it / 2) & 1, &abort_flag);
             ok = __shfl_sync(0xffffffffu, (int)ok, 0);
             if (!ok) break;
             tc_after();
             const uint32_t at = tm + (it & 1) * kPairTokens + ((quad * 32) << 16);
-            for (uint32_t c = c0; c < cols; c += 16) {
-                uint32_t v[16];
-                tmem_ld16(at + c, v);
+            for (uint32_t c = c0; c < cols; c += 32) {
+                uint32_t v[32];
+                tmem_ld32(at + c, v);
+                if (c + 32 < cols) next.fetch(a, m0 + c + 32, cols - c - 32, n, live);
                 tmem_ld_wait();
-                if (live) put<T, 16>(a, m0 + c, cols - c, n, v, ws);
+                out.put(a, m0 + c, cols - c, n, live, v, ws);
+                out = next;
             }
             tc_before();
             __syncwarp();
@@ -563,18 +590,18 @@ struct Cut {
     uint32_t nt = 0, split = 1;
     double cost = 1e30;
 };
-// Estimated SM cycles, from what the kernels measured: a slice costs the tensor pipe 2 cycles per token
-// column, and L2 3.1 cycles per 128-byte row while all SMs load (fewer CTAs get up to twice that each);
-// a tile's outputs cost 60 cycles per column of an epilogue warp (100 with an addition; a split's
-// exchange 60 more), a launch 4000.
+// Estimated SM cycles, the coefficients fitted to 105 shapes in every cut (1 to 1024 tokens, 578 to 24576
+// weight rows, 200 to 25600 columns; the chosen cut is 1.5 % slower than the best one on average, 13 % at
+// most): a slice costs L2 3.9 cycles per 128-byte row of the two operands or the tensor pipe 3.6 per token
+// column, whichever is more; outputs 45 per column of an epilogue warp, 40 more with an addition,
+// 30 more for a split's exchange; a launch 4000.
 double cost_of(uint32_t nt, uint64_t tiles, uint32_t split, uint32_t slices, bool add, int sms) {
-    const uint32_t pair = nt ? 1 : 2, cols = nt ? nt : 256, rows = nt ? kTileN + nt : 256;
-    const double slots = nt ? (double)sms * ctas_per_sm(nt) : sms / 2, units = (double)tiles * split;
-    const double busy = std::min(1.0, units * pair / ((double)sms * (nt ? ctas_per_sm(nt) : 1)));
+    const uint32_t cols = nt ? nt : 256, rows = nt ? kTileN + nt : 256;
     const double share = nt ? ctas_per_sm(nt) : 1;  // CTAs that share an SM's pipes and bandwidth
-    const double load = 3.1 * rows * share * std::max(0.5, busy), mma = 2.0 * cols * share;
-    const double per = (double)slices / split * std::max(load, mma), out = ((add ? 100.0 : 60.0) + (split > 1 ? 60.0 : 0.0)) * cols / (cols >= 128 ? 2 : 1);
-    const double waves = std::ceil(units / slots);
+    const double slots = nt ? sms * share : sms / 2;
+    const double per = (double)slices / split * share * std::max(3.9 * rows, 3.6 * cols);
+    const double out = (45.0 + (add ? 40.0 : 0.0) + (split > 1 ? 30.0 : 0.0)) * cols / (cols >= 128 ? 2 : 1);
+    const double waves = std::ceil((double)tiles * split / slots);
     // outputs of all tiles but the last are written behind the next tile's products
     return 4000.0 + waves * per + out + (waves - 1) * std::max(0.0, out - per);
 }
@@ -585,7 +612,9 @@ template <uint32_t NT, class T> void consider(Cut& best, const Plan& p, int sms)
     for (uint32_t k = 1; k <= 8; ++k) {
         if (k > 1) {  // a split's clusters all run at once, every CTA with four slices at least
             if (k * tiles > 2ull * sms || p.slices < 4 * k) break;
-            if (tiles > clusters_at_once<i8_gemm_kernel<NT, T>>(gemm_threads(NT), gemm_smem(NT), k)) continue;
+            // (the occupancy query counts one CTA per SM)
+            if (tiles > (uint64_t)ctas_per_sm(NT) * clusters_at_once<i8_gemm_kernel<NT, T>>(gemm_threads(NT), gemm_smem(NT), k))
+                continue;
         }
         const double c = cost_of(NT, tiles, k, p.slices, p.a.add != nullptr, sms);
         if (c < best.cost) best.nt = NT, best.split = k, best.cost = c;
