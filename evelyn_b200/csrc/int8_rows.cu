@@ -23,30 +23,55 @@ __device__ __forceinline__ uint32_t block_umax(uint32_t v, uint32_t* red) {
     return __reduce_max_sync(0xffffffffu, lane < warps ? red[lane] : 0u);
 }
 
-// One CTA per row, C chunks per thread in registers.
+// One CTA per row, C chunks per thread, kept as they were loaded: no load waits for a conversion or
+// stands behind a condition, so all are on their way together. The values after the last whole chunk
+// are one more per thread.
+template <class T> struct Chunk {
+    uint4 w[sizeof(T) / 2];  // kChunk values
+};
+template <class T> __device__ __forceinline__ void widen(const Chunk<T>& c, float (&v)[kChunk]) {
+    if constexpr (sizeof(T) == 4) {
+        const uint4 a = c.w[0], b = c.w[1];
+        v[0] = __uint_as_float(a.x), v[1] = __uint_as_float(a.y), v[2] = __uint_as_float(a.z), v[3] = __uint_as_float(a.w);
+        v[4] = __uint_as_float(b.x), v[5] = __uint_as_float(b.y), v[6] = __uint_as_float(b.z), v[7] = __uint_as_float(b.w);
+    } else {
+        unpack2(c.w[0].x, T{}, v[0], v[1]);
+        unpack2(c.w[0].y, T{}, v[2], v[3]);
+        unpack2(c.w[0].z, T{}, v[4], v[5]);
+        unpack2(c.w[0].w, T{}, v[6], v[7]);
+    }
+}
 template <class T, int C> __global__ void __launch_bounds__(1024) quantize_rows_kernel(const QuantRowsArgs a) {
     __shared__ uint32_t red[32];
     const uint64_t row = blockIdx.x;
     const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
     int8_t* codes = a.codes + row * a.code_stride;
     const uint32_t chunks = a.cols / kChunk, tail = a.cols % kChunk, nt = blockDim.x;
-    float v[C][kChunk];
-    uint32_t m = 0;
+    Chunk<T> raw[C];
+    T last{};
+    if (chunks) {
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+            const uint4* p = reinterpret_cast<const uint4*>(x + (uint64_t)min(threadIdx.x + i * nt, chunks - 1) * kChunk);
+#pragma unroll
+            for (uint32_t j = 0; j < sizeof(T) / 2; ++j) raw[i].w[j] = ldg_nc(p + j);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < C; ++i)
+#pragma unroll
+            for (uint32_t j = 0; j < sizeof(T) / 2; ++j) raw[i].w[j] = make_uint4(0, 0, 0, 0);
+    }
+    if (threadIdx.x < tail) last = x[(uint64_t)chunks * kChunk + threadIdx.x];
+    // (a thread past the end holds the last chunk again: the maximum is the same)
+    uint32_t m = threadIdx.x < tail ? abs_bits(to_f32(last)) : 0;
 #pragma unroll
     for (int i = 0; i < C; ++i) {
-        const uint32_t c = threadIdx.x + i * nt;
-        if (c < chunks) {
-            load8(x + (uint64_t)c * kChunk, v[i]);
-        } else {
-            const uint32_t left = c == chunks ? tail : 0;
+        float v[kChunk];
+        widen(raw[i], v);
 #pragma unroll
-            for (uint32_t j = 0; j < kChunk; ++j) v[i][j] = j < left ? to_f32(x[(uint64_t)c * kChunk + j]) : 0.f;
-        }
+        for (uint32_t j = 0; j < kChunk; ++j) m = max(m, abs_bits(v[j]));
     }
-#pragma unroll
-    for (int i = 0; i < C; ++i)
-#pragma unroll
-        for (uint32_t j = 0; j < kChunk; ++j) m = max(m, abs_bits(v[i][j]));
     m = block_umax(m, red);
     const float scale = scale_of(m), inv = inverse_of(scale);
     if (threadIdx.x == 0) a.scales[row] = scale;
@@ -54,18 +79,16 @@ template <class T, int C> __global__ void __launch_bounds__(1024) quantize_rows_
 #pragma unroll
     for (int i = 0; i < C; ++i) {
         const uint32_t c = threadIdx.x + i * nt;
+        if (c >= chunks) break;
+        float v[kChunk];
         uint32_t q[kChunk];
+        widen(raw[i], v);
 #pragma unroll
-        for (uint32_t j = 0; j < kChunk; ++j) q[j] = live ? code_bits(v[i][j], inv) : 0u;
-        if (c < chunks) {
-            *reinterpret_cast<uint2*>(codes + (uint64_t)c * kChunk) =
-                make_uint2(pack4(q[0], q[1], q[2], q[3]), pack4(q[4], q[5], q[6], q[7]));
-        } else if (c == chunks) {
-#pragma unroll
-            for (uint32_t j = 0; j < kChunk; ++j)
-                if (j < tail) codes[(uint64_t)c * kChunk + j] = (int8_t)q[j];
-        }
+        for (uint32_t j = 0; j < kChunk; ++j) q[j] = live ? code_bits(v[j], inv) : 0u;
+        *reinterpret_cast<uint2*>(codes + (uint64_t)c * kChunk) =
+            make_uint2(pack4(q[0], q[1], q[2], q[3]), pack4(q[4], q[5], q[6], q[7]));
     }
+    if (threadIdx.x < tail) codes[(uint64_t)chunks * kChunk + threadIdx.x] = live ? (int8_t)code_bits(to_f32(last), inv) : (int8_t)0;
 }
 
 // Rows that do not start on the boundaries of wide loads (an odd row length, a view), and rows
