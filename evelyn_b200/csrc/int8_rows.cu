@@ -6,6 +6,8 @@
 // bytes + one byte per value is all the traffic, so the kernel is bound by HBM. f32 throughout;
 // the products and the reciprocal are each rounded once, so the codes do not depend on the
 // launch shape.
+#include <atomic>
+
 #include "int8.cuh"
 
 namespace evl {
@@ -91,10 +93,98 @@ template <class T, int C> __global__ void __launch_bounds__(1024) quantize_rows_
     if (threadIdx.x < tail) codes[(uint64_t)chunks * kChunk + threadIdx.x] = live ? (int8_t)code_bits(to_f32(last), inv) : (int8_t)0;
 }
 
-// Rows that do not start on the boundaries of wide loads (an odd row length, a view), and rows
-// too long for registers: values one by one, neighbouring threads on neighbouring values, the
-// row read a second time from L2.
-template <class T> __global__ void __launch_bounds__(512) quantize_rows_plain_kernel(const QuantRowsArgs a) {
+// Rows that do not start on the boundaries of wide loads (an odd row length, a view), and rows too long
+// for registers: the row is staged in shared memory in the 16-byte granules of its global addresses
+// (asynchronous copies; the values before the first and after the last whole granule one by one, the
+// rest of those granules zero). The maximum is taken granule by granule; eight values of a chunk come
+// from the two (f32: three) granules that hold them, moved by the row's offset.
+template <class T> __global__ void __launch_bounds__(512) quantize_rows_staged_kernel(const QuantRowsArgs a) {
+    extern __shared__ __align__(16) uint8_t row_smem[];
+    __shared__ uint32_t red[32];
+    constexpr uint32_t ES = sizeof(T), NW = kChunk * ES / 4;  // words of a chunk
+    const uint64_t row = blockIdx.x;
+    const uint8_t* x = reinterpret_cast<const uint8_t*>(static_cast<const T*>(a.x) + row * a.x_stride);
+    int8_t* codes = a.codes + row * a.code_stride;
+    const uint32_t sh = (uint32_t)(reinterpret_cast<uintptr_t>(x) & 15), bytes = a.cols * ES;
+    const uint32_t g0 = sh ? 1 : 0, g1 = (sh + bytes) / 16;       // whole granules [g0, g1)
+    const uint32_t granules = (sh + bytes + 15) / 16 + 2;         // with two of zeros, which a last chunk may reach into
+    const uint32_t tid = threadIdx.x, nt = blockDim.x;
+    for (uint32_t g = tid; g < granules; g += nt) {
+        if (g >= g0 && g < g1)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(row_smem + 16 * g)), "l"(x + 16 * g - sh) : "memory");
+        else
+            *reinterpret_cast<uint4*>(row_smem + 16 * g) = make_uint4(0, 0, 0, 0);
+    }
+    asm volatile("cp.async.commit_group;\ncp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
+    // the values of a first and a last granule that are not whole
+    const uint32_t head = g0 ? min(16 - sh, bytes) / ES : 0;               // elements before the first whole granule
+    const uint32_t from = max(head, g1 > g0 ? (16 * g1 - sh) / ES : head);  // and from here on
+    if (tid < head) reinterpret_cast<T*>(row_smem + sh)[tid] = reinterpret_cast<const T*>(x)[tid];
+    if (from + tid < a.cols) reinterpret_cast<T*>(row_smem + sh)[from + tid] = reinterpret_cast<const T*>(x)[from + tid];
+    __syncthreads();
+    uint32_t m = 0;
+    for (uint32_t g = tid; g < granules; g += nt) {
+        const uint4 w = *reinterpret_cast<const uint4*>(row_smem + 16 * g);
+        const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (ES == 4) {
+                m = max(m, v[j] & 0x7fffffffu);
+            } else {
+                float p, q;
+                unpack2(v[j], T{}, p, q);
+                m = max(m, max(abs_bits(p), abs_bits(q)));
+            }
+        }
+    }
+    m = block_umax(m, red);
+    const float scale = scale_of(m), inv = inverse_of(scale);
+    if (tid == 0) a.scales[row] = scale;
+    const bool live = scale > 0.f;
+    const bool wide = (reinterpret_cast<uintptr_t>(codes) & 7) == 0;
+    const uint32_t chunks = (a.cols + kChunk - 1) / kChunk, bits = 8 * (sh & 3);
+    for (uint32_t c = tid; c < chunks; c += nt) {
+        uint32_t w[NW + 4], v[NW];
+#pragma unroll
+        for (uint32_t j = 0; j < NW + 4; j += 4) {
+            const uint4 g = *reinterpret_cast<const uint4*>(row_smem + c * (kChunk * ES) + 4 * j);
+            w[j] = g.x, w[j + 1] = g.y, w[j + 2] = g.z, w[j + 3] = g.w;
+        }
+        auto move = [&](auto at) {
+#pragma unroll
+            for (uint32_t j = 0; j < NW; ++j) v[j] = __funnelshift_r(w[at + j], j + at + 1 < NW + 4 ? w[at + j + 1] : 0u, bits);
+        };
+        switch (sh >> 2) {  // (the same for the whole row)
+            case 0: move(std::integral_constant<uint32_t, 0>{}); break;
+            case 1: move(std::integral_constant<uint32_t, 1>{}); break;
+            case 2: move(std::integral_constant<uint32_t, 2>{}); break;
+            default: move(std::integral_constant<uint32_t, 3>{}); break;
+        }
+        float f[kChunk];
+        uint32_t q[kChunk];
+#pragma unroll
+        for (uint32_t j = 0; j < kChunk; j += 4 / ES) {
+            if constexpr (ES == 4) f[j] = __uint_as_float(v[j]);
+            else unpack2(v[j / 2], T{}, f[j], f[j + 1]);
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < kChunk; ++j) q[j] = live ? code_bits(f[j], inv) : 0u;
+        const uint32_t left = a.cols - c * kChunk;
+        if (wide && left >= kChunk) {
+            *reinterpret_cast<uint2*>(codes + (uint64_t)c * kChunk) =
+                make_uint2(pack4(q[0], q[1], q[2], q[3]), pack4(q[4], q[5], q[6], q[7]));
+        } else {
+#pragma unroll
+            for (uint32_t j = 0; j < kChunk; ++j)
+                if (j < left) codes[(uint64_t)c * kChunk + j] = (int8_t)q[j];
+        }
+    }
+}
+
+// Rows that do not fit into shared memory: values one by one, neighbouring threads on neighbouring values,
+// the row read a second time from L2.
+template <class T> __global__ void __launch_bounds__(512) quantize_rows_long_kernel(const QuantRowsArgs a) {
     __shared__ uint32_t red[32];
     const uint64_t row = blockIdx.x;
     const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
@@ -111,13 +201,34 @@ template <class T> __global__ void __launch_bounds__(512) quantize_rows_plain_ke
         codes[c] = live ? (int8_t)code_bits(to_f32(x[c]), inv) : (int8_t)0;
 }
 
+// shared memory of a staged row, and the most that a CTA may have
+inline uint64_t staged_bytes(uint64_t row_bytes) { return row_bytes + 16 + 48; }
+constexpr uint32_t kStagedCap = 200 * 1024;
+template <auto kernel> cudaError_t opt_in(uint32_t smem) {
+    static std::atomic<bool> done[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    if (done[dev].load()) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e == cudaSuccess) done[dev] = true;
+    return e;
+}
+
 template <class T> cudaError_t launch(const QuantRowsArgs& a, int sms, cudaStream_t s) {
     const bool aligned = (reinterpret_cast<uintptr_t>(a.x) & 15) == 0 && (a.x_stride * sizeof(T)) % 16 == 0 &&
                          (reinterpret_cast<uintptr_t>(a.codes) & 7) == 0 && a.code_stride % 8 == 0;
     const uint32_t chunks = (a.cols + kChunk - 1) / kChunk;
     if (!aligned || chunks > 4 * 1024) {
-        const uint32_t nt = a.cols >= 4096 ? 512 : a.cols >= 512 ? 128 : 32;
-        quantize_rows_plain_kernel<T><<<a.rows, nt, 0, s>>>(a);
+        const uint64_t smem = staged_bytes((uint64_t)a.cols * sizeof(T));
+        const uint32_t nt = a.cols >= 8192 ? 512 : a.cols >= 1024 ? 256 : 64;
+        if (smem > kStagedCap) {
+            quantize_rows_long_kernel<T><<<a.rows, 512, 0, s>>>(a);
+        } else {
+            if (const cudaError_t e = opt_in<quantize_rows_staged_kernel<T>>(kStagedCap)) return e;
+            quantize_rows_staged_kernel<T><<<a.rows, nt, (uint32_t)smem, s>>>(a);
+        }
         return cudaGetLastError();
     }
     // few rows: as many threads as chunks, so that a row is one load deep; many rows: four

@@ -41,7 +41,8 @@ def same(a, b):
 # ------------------------------------------------------------------ rows
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("rows,cols,pad", [(1, 1, 0), (1, 4096, 0), (3, 17, 0), (5, 64, 8), (2, 1000, 24), (33, 5003, 5),
-                                           (400, 4096, 0), (301, 8200, 8), (2, 16384, 0), (2, 40000, 0), (1, 12288, 0)])
+                                           (400, 4096, 0), (301, 8200, 8), (2, 16384, 0), (2, 40000, 0), (1, 12288, 0), (9, 7, 0), (40, 23, 2),
+                                           (16, 1023, 0), (3, 110001, 0), (17, 8, 1), (8, 2047, 4)])
 def test_quantize_rows(kind, rows, cols, pad):
     t = gu.torch()
     rng = np.random.default_rng(rows * 31 + cols)
@@ -56,7 +57,25 @@ def test_quantize_rows(kind, rows, cols, pad):
     assert np.all(host(codes)[:, cols:] == 99)  # what lies between the rows is left alone
 
 
-@pytest.mark.parametrize("cols", [64, 333, 40000])
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("at", range(9))
+@pytest.mark.parametrize("cols", [1, 5, 8, 16, 41, 300])
+def test_quantize_rows_at_every_offset(kind, at, cols):
+    """Views that start anywhere in a 16-byte granule, full of larger values around them."""
+    t = gu.torch()
+    rng = np.random.default_rng(at * 7 + cols)
+    x = np.full((5, cols + 24), 1e4, np.float32)
+    x[:, at:at + cols] = rng.standard_normal((5, cols))
+    dx = dev(x, kind)[:, at:at + cols]
+    codes = t.full((5, cols + 5), 99, dtype=t.int8, device="cuda:0")
+    scales = gu.empty_f32(5)
+    int8.quantize_rows(dx, codes[:, at % 4:at % 4 + cols], scales)
+    want, ws = ref.quantize_rows(host(dx))
+    assert same(host(scales), ws) and np.array_equal(host(codes)[:, at % 4:at % 4 + cols], want)
+    assert np.all(host(codes)[:, :at % 4] == 99) and np.all(host(codes)[:, at % 4 + cols:] == 99)
+
+
+@pytest.mark.parametrize("cols", [64, 333, 40000, 110000])
 def test_quantize_rows_special_values(cols):
     x = np.random.default_rng(1).standard_normal((9, cols)).astype(np.float32)
     x[0] = 0
