@@ -526,8 +526,11 @@ template <class T, int HD> __global__ void __launch_bounds__(32 * kJoinWarps) kv
 //   4 softmax warps   per row tile, one row per thread: scores to registers, running maximum,
 //                     weights to f16 over the scores' own columns. O is rescaled (read, multiplied,
 //                     written back) only when a score passes the row's maximum by 2^8.
-// q is scaled by a power of two per row and held in one f16 part (16-bit inputs: exact) or two
-// (f32 inputs, TERMS = 2; then P is also two parts, two products each). The block scales enter as
+// 16-bit inputs (TERMS = 1): q is scaled by a power of two per row and held in one f16 part, exactly;
+// the weights are one f16 part. f32 inputs (TERMS = 2): q is fixed point in three 8-bit limbs and the
+// scores are integer products (kind::i8) of the codes as they are, summed exactly -- the f32 sums of
+// kind::f16 are cut off, not rounded, and over long sums that shows; the weights are two f16 parts
+// with a product each. The block scales enter as
 // in the kernel above; the value scale as an added log2 where one rounding of the weights follows
 // anyway (TERMS = 1).
 // Bound: the exponentials (16 a clock and SM) and the tensor pipe, about equally.
@@ -540,9 +543,14 @@ struct Role {  // per (HD, TERMS): row tiles, positions per step, stages of f16 
 __host__ __device__ constexpr Role role_of(int hd, int terms) {
     return hd == 256 ? (terms == 2 ? Role{1, 32, 2, 2} : Role{1, 32, 3, 3}) : terms == 2 ? Role{1, 64, 2, 4} : Role{2, 64, 2, 4};
 }
+// bytes of one part of a row tile's q (f16; or an 8-bit limb), of a stage's K
+__host__ __device__ constexpr uint32_t q_part(int hd, int terms) { return kTileRows * hd * (terms == 2 ? 1 : 2); }
+__host__ __device__ constexpr uint32_t q_parts(int terms) { return terms == 2 ? 3 : 1; }
+__host__ __device__ constexpr uint32_t k_stage(int hd, int terms) { return role_of(hd, terms).np * hd * (terms == 2 ? 1 : 2); }
 __host__ __device__ constexpr uint32_t tile_smem(int hd, int terms) {
-    return role_of(hd, terms).rt * terms * kTileRows * hd * 2 +
-           role_of(hd, terms).np * hd * (4 * role_of(hd, terms).stages + 2 * role_of(hd, terms).raw) + 1024;
+    return role_of(hd, terms).rt * q_parts(terms) * q_part(hd, terms) +
+           role_of(hd, terms).stages * (k_stage(hd, terms) + role_of(hd, terms).np * hd * 2) +
+           role_of(hd, terms).raw * role_of(hd, terms).np * hd * 2 + 1024;
 }
 static_assert(tile_smem(256, 2) <= 232448 && tile_smem(256, 1) <= 232448 && tile_smem(128, 1) <= 232448, "shared memory");
 
@@ -586,6 +594,25 @@ __device__ __forceinline__ uint64_t swizzled_desc(uint32_t addr, uint32_t lbo) {
     return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
            (1ull << 46) | (2ull << 61);
 }
+// K-major 8-bit operand: rows of 128 bytes as above, or (64 dims) of 64 bytes with the 64-byte swizzle
+template <int HD> __device__ __forceinline__ uint64_t bytes_desc(uint32_t addr) {
+    constexpr uint64_t group = HD == 64 ? 512 : 1024, mode = HD == 64 ? 4 : 2;
+    return (uint64_t)((addr & 0x3FFFFu) >> 4) | (1ull << 16) | ((group >> 4) << 32) | (1ull << 46) | (mode << 61);
+}
+// byte offset of 16-byte piece `p` of row r in such panels of `rows` rows
+template <int HD> __device__ __forceinline__ uint32_t bytes_at(uint32_t rows, uint32_t r, uint32_t p) {
+    if constexpr (HD == 64) return r * 64u + ((p ^ ((r >> 1) & 3u)) << 4);
+    else return (p >> 3) * (rows * 128u) + r * 128u + (((p & 7u) ^ (r & 7u)) << 4);
+}
+__host__ __device__ constexpr uint32_t i8_idesc(uint32_t n) {
+    return (2u << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | ((kTileRows >> 4) << 24);
+}
+__device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
 __host__ __device__ constexpr uint32_t f16_idesc(uint32_t n, bool b_mn_major) {
     return (1u << 4) | ((b_mn_major ? 1u : 0u) << 16) | ((n >> 3) << 17) | ((kTileRows >> 4) << 24);
 }
@@ -609,6 +636,14 @@ __device__ __forceinline__ void tmem_ld32(uint32_t t, uint32_t (&v)[32]) {
           "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
           "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
           "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(t)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t t, uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
         : "r"(t)
         : "memory");
 }
@@ -667,8 +702,10 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
     constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
     constexpr Role R = role_of(HD, TERMS);
     constexpr uint32_t RT = R.rt, NP = R.np, ST = R.stages, RAW = R.raw, NB = NP / 16;
-    constexpr uint32_t kQPart = kTileRows * HD * 2;   // one f16 part of a row tile's q
-    constexpr uint32_t kKv = NP * HD * 2;             // K (or V) of a stage
+    constexpr uint32_t kQPart = q_part(HD, TERMS), kQParts = q_parts(TERMS);
+    constexpr uint32_t kK = k_stage(HD, TERMS), kV = NP * HD * 2, kStage = kK + kV;  // K and V of a stage
+    constexpr uint32_t kSCols = TERMS == 2 ? 3 * NP : NP;  // tensor memory columns of a score buffer
+    static_assert(RT * (HD + 2 * kSCols) <= 512 && (RT == 1 || HD + 2 * kSCols <= 256), "tensor memory");
     constexpr uint32_t kSoftWarps = 4 * RT, kTileCols = RT == 2 ? 256 : 512;  // tensor memory columns per row tile
     extern __shared__ uint8_t raw_smem[];
     constexpr uint32_t FS = 8;  // steps of block factors
@@ -696,9 +733,9 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
     const uint32_t steps = b1 > b0 ? (uint32_t)(b1 - b0 + (int32_t)NB - 1) / NB : 0;
 
     uint8_t* smem = raw_smem + ((1024u - (smem_addr(raw_smem) & 1023u)) & 1023u);
-    uint8_t* sq = smem;                                  // [RT][TERMS] q panels
-    uint8_t* skv = smem + RT * TERMS * kQPart;           // [ST][K | V] f16 panels
-    uint8_t* sraw = skv + ST * 2 * kKv;                  // [RAW][K | V] codes, 16 bytes per thread and piece
+    uint8_t* sq = smem;                                  // [RT] q panels
+    uint8_t* skv = smem + RT * kQParts * kQPart;         // [ST][K | V] panels
+    uint8_t* sraw = skv + ST * kStage;                  // [RAW][K | V] codes, 16 bytes per thread and piece
     if (tid == 0) {
         abort_flag = 0;
         for (uint32_t i = 0; i < ST; ++i) {
@@ -753,27 +790,44 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
                 for (int i = 0; i < 8; ++i) m = max(m, abs_bits(v[i]));
             }
             const bool bad = m >= 0x7f800000u;
-            const int sh = min(100, 10 - ((int)(m >> 23) - 126));  // largest magnitude just under 2^10
+            // largest magnitude just under 2^10 (f16) or 2^22 (limbs)
+            const int sh = min(100, (TERMS == 2 ? 22 : 10) - ((int)(m >> 23) - 126));
             const float up = copysignf(exp2f((float)sh), a.scale);  // (so that the factor is not negative)
             step = bad ? __uint_as_float(0x7fc00000u) : exp2f((float)-sh) * fabsf(a.scale) * 1.4426950408889634f;
-            uint8_t* panel = sq + rt * TERMS * kQPart;
+            uint8_t* panel = sq + rt * kQParts * kQPart;
+            if constexpr (TERMS == 1) {
 #pragma unroll 4
-            for (int d = 0; d < HD; d += 8) {
-                float v[8];
-                load8(q + d, v);
-                uint32_t hi[4], lo[4];
+                for (int d = 0; d < HD; d += 8) {
+                    float v[8];
+                    load8(q + d, v);
+                    uint32_t hi[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float x = bad ? 0.f : v[2 * i] * up, y = bad ? 0.f : v[2 * i + 1] * up;
-                    hi[i] = pack_h2(x, y);
-                    if (TERMS == 2) {
-                        const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi[i]));
-                        lo[i] = pack_h2(x - back.x, y - back.y);
-                    }
+                    for (int i = 0; i < 4; ++i) hi[i] = pack_h2(bad ? 0.f : v[2 * i] * up, bad ? 0.f : v[2 * i + 1] * up);
+                    *reinterpret_cast<uint4*>(panel + panel_at(kTileRows, lr, d / 8)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
                 }
-                const uint32_t at = panel_at(kTileRows, lr, d / 8);
-                *reinterpret_cast<uint4*>(panel + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                if (TERMS == 2) *reinterpret_cast<uint4*>(panel + kQPart + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            } else {
+#pragma unroll 1
+                for (int d = 0; d < HD; d += 16) {
+                    uint32_t w[3][4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        float v[4];
+                        uint32_t lb[3][4];
+                        load4(q + d + 4 * k, v);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int x = bad ? 0 : __float2int_rn(v[i] * up);
+                            const int l0 = (int)(int8_t)x, x1 = (x - l0) >> 8, l1 = (int)(int8_t)x1, l2 = (x1 - l1) >> 8;
+                            lb[0][i] = (uint32_t)l0, lb[1][i] = (uint32_t)l1, lb[2][i] = (uint32_t)l2;
+                        }
+#pragma unroll
+                        for (int i = 0; i < 3; ++i) w[i][k] = pack4(lb[i][0], lb[i][1], lb[i][2], lb[i][3]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 3; ++i)
+                        *reinterpret_cast<uint4*>(panel + i * kQPart + bytes_at<HD>(kTileRows, lr, d / 16)) =
+                            make_uint4(w[i][0], w[i][1], w[i][2], w[i][3]);
+                }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
@@ -790,7 +844,7 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
             ok = warp_wait(&f_full[st], (j / FS) & 1, &abort_flag) && warp_wait(&s_full[rt][j & 1], (j >> 1) & 1, &abort_flag);
             if (!ok) break;
             tc_after();
-            const uint32_t ts = to + HD + (j & 1) * NP;
+            const uint32_t ts = to + HD + (j & 1) * kSCols;
             const int32_t p0 = (b0 + (int32_t)(j * NB)) * 16;
             const bool masked = __any_sync(0xffffffffu, p0 + (int32_t)NP - 1 > open || !live);
             float f[NB], e[NB], down[NB], mant[NB];
@@ -844,9 +898,23 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
                 }
             }
             uint32_t v[NP];
+            if constexpr (TERMS == 1) {
 #pragma unroll
-            for (uint32_t c = 0; c < NP; c += 32) tmem_ld32(ts + c, *reinterpret_cast<uint32_t(*)[32]>(v + c));
-            tmem_ld_wait();
+                for (uint32_t c = 0; c < NP; c += 32) tmem_ld32(ts + c, *reinterpret_cast<uint32_t(*)[32]>(v + c));
+                tmem_ld_wait();
+            } else {
+#pragma unroll
+                for (uint32_t c = 0; c < NP; c += 16) {
+                    uint32_t l0[16], l1[16], l2[16];
+                    tmem_ld16(ts + c, l0);
+                    tmem_ld16(ts + NP + c, l1);
+                    tmem_ld16(ts + 2 * NP + c, l2);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (uint32_t i = 0; i < 16; ++i)  // (the two lower limbs together stay below 2^30)
+                        v[c + i] = __float_as_uint(fmaf((float)(int)l2[i], 65536.f, (float)((int)l1[i] * 256 + (int)l0[i])));
+                }
+            }
             if (masked) {
 #pragma unroll
                 for (uint32_t i = 0; i < NP; ++i)
@@ -1031,16 +1099,28 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
         };
+        auto copy = [&](uint8_t* panel, const uint8_t* raw, uint32_t none) {  // the codes as they are
+#pragma unroll
+            for (uint32_t i = 0; i < N; ++i) {
+                const uint32_t piece = pt + 128 * i;
+                const uint4 w = *reinterpret_cast<const uint4*>(raw + 16 * piece);
+                *reinterpret_cast<uint4*>(panel + bytes_at<HD>(NP, piece / CPR, piece % CPR)) =
+                    none >> i & 1 ? make_uint4(0, 0, 0, 0) : w;
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+        };
         for (uint32_t j = 0; j < steps; ++j) {  // (after an abort the loop runs out quickly: every wait gives up at once)
             const uint32_t st = j % ST, rs = j % RAW, none = gone >> (rs * N);
             cp_async_wait<(int)RAW - 1>();
             const uint8_t* raw = sraw + rs * (2 * NP * HD);
-            uint8_t* dst = skv + st * 2 * kKv;
+            uint8_t* dst = skv + st * kStage;
             if (j >= ST) warp_wait(&k_empty[st], (j / ST - 1) & 1, &abort_flag);
-            widen(dst, raw, none);
+            if (TERMS == 1) widen(dst, raw, none);
+            else copy(dst, raw, none);
             if (lane == 0) mbar_arrive(&k_full[st]);
             if (j >= ST) warp_wait(&v_empty[st], (j / ST - 1) & 1, &abort_flag);
-            widen(dst + kKv, raw + NP * HD, none);
+            widen(dst + kK, raw + NP * HD, none);
             if (lane == 0) mbar_arrive(&v_full[st]);
             if (j + RAW < steps) {
                 fetch(j + RAW);
@@ -1090,7 +1170,7 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
         // ---------------------------------------------------------------- MMA: one thread per row tile, so that
         // one tile's products run while the other waits for its weights
         const uint32_t rt = warp - kSoftWarps - 4;
-        const uint32_t d = tm + rt * kTileCols, qb = smem_addr(sq + rt * TERMS * kQPart);
+        const uint32_t d = tm + rt * kTileCols, qb = smem_addr(sq + rt * kQParts * kQPart);
         bool ok = bwait(&q_full, 0, &abort_flag);
         auto scores = [&](uint32_t j) {
             const uint32_t st = j % ST;
@@ -1100,25 +1180,32 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
                  bwait(&k_full[st], (j / ST) & 1, &abort_flag);
             if (!ok) return;
             tc_after();
-            const uint32_t kb = smem_addr(skv + st * 2 * kKv), ds = d + HD + (j & 1) * NP;
-#pragma unroll
-            for (uint32_t x = 0; x < (uint32_t)TERMS; ++x)
+            const uint32_t kb = smem_addr(skv + st * kStage), ds = d + HD + (j & 1) * kSCols;
+            if constexpr (TERMS == 1) {
 #pragma unroll
                 for (uint32_t k = 0; k < HD / 16; ++k)
-                    mma_ss(ds, swizzled_desc(qb + x * kQPart + (k / 4) * (kTileRows * 128) + (k % 4) * 32, 16),
-                           swizzled_desc(kb + (k / 4) * (NP * 128) + (k % 4) * 32, 16), f16_idesc(NP, false), x > 0 || k > 0);
+                    mma_ss(ds, swizzled_desc(qb + (k / 4) * (kTileRows * 128) + (k % 4) * 32, 16),
+                           swizzled_desc(kb + (k / 4) * (NP * 128) + (k % 4) * 32, 16), f16_idesc(NP, false), k > 0);
+            } else {
+#pragma unroll
+                for (uint32_t x = 0; x < 3; ++x)
+#pragma unroll
+                    for (uint32_t k = 0; k < HD / 32; ++k)
+                        mma_i8(ds + x * NP, bytes_desc<HD>(qb + x * kQPart + (k / 4) * (kTileRows * 128) + (k % 4) * 32),
+                               bytes_desc<HD>(kb + (k / 4) * (NP * 128) + (k % 4) * 32), i8_idesc(NP), k > 0);
+            }
             mma_commit(&s_full[rt][j & 1]);
             mma_commit(&k_empty[st]);
         };
         scores(0);
         for (uint32_t j = 0; j < steps && ok; ++j) {
             if (j + 1 < steps) scores(j + 1);
-            const uint32_t st = j % ST, vb = smem_addr(skv + st * 2 * kKv + kKv);
+            const uint32_t st = j % ST, vb = smem_addr(skv + st * kStage + kK);
             ok = ok && bwait(&v_full[st], (j / ST) & 1, &abort_flag) &&
                  bwait(&p_full[rt][j & 1], (j >> 1) & 1, &abort_flag);
             if (!ok) break;
             tc_after();
-            const uint32_t pw = d + HD + (j & 1) * NP;
+            const uint32_t pw = d + HD + (j & 1) * kSCols;
 #pragma unroll
             for (uint32_t x = 0; x < (uint32_t)TERMS; ++x)
 #pragma unroll
