@@ -1242,10 +1242,13 @@ Shape shape_of(const Kv8Cache& c, const Kv8Batch& b, uint32_t heads, uint32_t ty
     r.tile_rows = r.tiles ? role.rt * kTileRows : kRows;
     r.row_tiles = (uint32_t)((rows + r.tile_rows - 1) / r.tile_rows);
     const uint32_t blocks = std::max(1u, (b.max_len + 15) / 16);
-    // chunks of positions: enough CTAs for three on every SM (the prompt kernel: one), each with
-    // at least 8 blocks (two per warp; the prompt kernel: 32, eight steps)
+    // chunks of positions: enough CTAs for three on every SM (the prompt kernel: one; one row tile of 256
+    // dims: two, as many as run at once -- 32768 positions over 4 kv heads 25 us against 34 with three;
+    // several row tiles read the same pages, and three measured better: 29 against 37), each with at
+    // least 8 blocks (two per warp; the prompt kernel: 32, eight steps). More chunks measured slower: a
+    // CTA's fixed cost is about 4 us.
     const uint64_t tiles = (uint64_t)b.n_seqs * c.kv_heads * r.row_tiles;
-    const uint64_t want = std::max<uint64_t>(1, (r.tiles ? 1ull : 3ull) * sms / std::max<uint64_t>(1, tiles));
+    const uint64_t want = std::max<uint64_t>(1, (r.tiles ? 1ull : c.head_dim == 256 && r.row_tiles == 1 ? 2ull : 3ull) * sms / std::max<uint64_t>(1, tiles));
     r.chunk = std::max(r.tiles ? 32u : 8u, (uint32_t)((blocks + want - 1) / want));
     r.chunk = (r.chunk + 3) / 4 * 4;
     r.splits = (blocks + r.chunk - 1) / r.chunk;
