@@ -10,8 +10,9 @@
 A layer of a decode or prompt step runs them one after the other: quantise, the q / k / v
 product, append, attention, quantise, the output product with the residual added.
 
-Arguments are tensors in device memory: any object with ``data_ptr()``, ``dtype``, ``shape`` and
-``stride()`` (PyTorch's, for one). Outputs are written into the tensors given. ``stream`` is a
+Arguments are tensors in device memory, those of a call on one device: any object with
+``data_ptr()``, ``dtype``, ``shape``, ``stride()`` and, to have that checked, ``device``
+(PyTorch's, for one). Outputs are written into the tensors given. ``stream`` is a
 CUDA stream handle (an integer; 0 is the device's default stream): a caller working on another
 stream passes that one. Calls are asynchronous and allocate nothing, so they can be captured into
 a graph. Arguments that do not fit raise EvelynError (InvalidInput, Unsupported); ``err``, an int32
@@ -42,14 +43,15 @@ def _kind(t) -> int:
         return _kinds.setdefault(t.dtype, _TYPES[name])
 
 
-# What the checks of a call found, by the types, shapes and strides of its tensors (never by
-# their addresses): a call whose tensors are laid out like an earlier one's is not checked again.
+# What the checks of a call found, by the types, shapes, strides and devices of its tensors
+# (never by their addresses): a call whose tensors are laid out like an earlier one's is not checked again.
 _plans: dict = {}
 _MOST_PLANS = 4096
+_MOST_TOTALS = 64  # descriptors that a batch keeps
 
 
 def _layout(*tensors) -> tuple:
-    return tuple([None if t is None else (t.dtype, t.shape, t.stride()) for t in tensors])
+    return tuple([None if t is None else (t.dtype, t.shape, t.stride(), getattr(t, "device", None)) for t in tensors])
 
 
 def _planned(key: tuple, plan):
@@ -62,6 +64,14 @@ def _planned(key: tuple, plan):
 def _need(ok: bool, msg: str):
     if not ok:
         raise EvelynError(1, msg)
+
+
+def _device_of(*tensors, known=()):
+    """The device that all of them are on (None for objects that name none)."""
+    found = {d for d in known if d is not None}
+    found.update(t.device for t in tensors if getattr(t, "device", None) is not None)
+    _need(len(found) <= 1, f"the tensors of a call must be on one device, not on {sorted(map(str, found))}")
+    return found.pop() if found else None
 
 
 def _named(t, name: str, what: str):
@@ -89,12 +99,10 @@ def _ptr(t) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
-def _err(err) -> Optional[int]:
-    if err is None:
-        return None
-    _named(err, "int32", "err")
-    _need(err.numel() >= 1, "err must hold one value")
-    return err.data_ptr()
+def _check_err(err):
+    if err is not None:
+        _named(err, "int32", "err")
+        _need(err.numel() >= 1, "err must hold one value")
 
 
 def quantize_rows(x, codes, scales, stream: int = 0) -> None:
@@ -103,6 +111,7 @@ def quantize_rows(x, codes, scales, stream: int = 0) -> None:
     key = ("rows", _layout(x, codes, scales))
     plan = _plans.get(key)
     if plan is None:
+        _device_of(x, codes, scales)
         kind, xs, cs = _kind(x), _rows(x, "x"), _rows(codes, "codes")
         rows, cols = x.shape
         _named(codes, "int8", "codes")
@@ -117,9 +126,11 @@ def quantize_rows(x, codes, scales, stream: int = 0) -> None:
 def matmul(x, x_scales, w, w_scales, y, add=None, err=None, stream: int = 0) -> None:
     """y [rows][out] = (x [rows][cols] @ w [out][cols]^T) * x_scales[:, None] * w_scales (+ add),
     x and w int8 with rows on 16-byte boundaries, int32 sums (evl_i8_matmul)."""
-    key = ("matmul", _layout(x, x_scales, w, w_scales, y, add))
+    key = ("matmul", _layout(x, x_scales, w, w_scales, y, add, err))
     plan = _plans.get(key)
     if plan is None:
+        _device_of(x, x_scales, w, w_scales, y, add, err)
+        _check_err(err)
         kind, xst, wst, yst = _kind(y), _rows(x, "x"), _rows(w, "w"), _rows(y, "y")
         rows, cols = x.shape
         out = w.shape[0]
@@ -139,7 +150,7 @@ def matmul(x, x_scales, w, w_scales, y, add=None, err=None, stream: int = 0) -> 
     kind, xst, wst, yst, ast, rows, out, cols = plan
     _check(runtime.lib().evl_i8_matmul(x.data_ptr(), xst, x_scales.data_ptr(), rows, w.data_ptr(), wst,
                                        w_scales.data_ptr(), out, cols, kind, _ptr(add), ast, y.data_ptr(), yst,
-                                       _err(err), stream))
+                                       _ptr(err), stream))
 
 
 class Kv8Cache:
@@ -157,6 +168,7 @@ class Kv8Cache:
             _named(t, name, what)
         self.kv_heads, self.head_dim, self.page_size, self.n_pages = heads, dim, page, pages
         self._tensors = (k, v, k_scales, v_scales)
+        self._device = _device_of(*self._tensors)
         self._c = _Kv8Cache(C.sizeof(_Kv8Cache), heads, dim, page, pages, 0, k.data_ptr(), v.data_ptr(),
                             k_scales.data_ptr(), v_scales.data_ptr(), stride, sstride)
         self._ref = C.byref(self._c)
@@ -180,6 +192,7 @@ class Kv8Batch:
         self.n_seqs, self.max_new, self.max_len = n, int(max_new), int(max_len)
         self._width = page_table.shape[1]
         self._tensors = (page_table, cu, lens)
+        self._device = _device_of(*self._tensors)
         self._fields = (self.max_new, self.max_len, tstride, page_table.data_ptr(), cu.data_ptr(), lens.data_ptr())
         self._by_total: dict = {}  # number of tokens -> the C descriptor of such a call
 
@@ -187,6 +200,8 @@ class Kv8Batch:
         _need(self.max_len <= self._width * page_size, "max_len passes the page table's rows")
         ref = self._by_total.get(total)
         if ref is None:
+            if len(self._by_total) >= _MOST_TOTALS:
+                self._by_total.clear()
             ref = C.byref(_Kv8Batch(C.sizeof(_Kv8Batch), self.n_seqs, total, *self._fields))
             self._by_total[total] = ref
         return ref
@@ -203,16 +218,19 @@ def kv8_append(cache: Kv8Cache, batch: Kv8Batch, k, v, q=None, q_out=None, rope=
     """Appends k, v [tokens][kv heads][head dim] to the cache and makes q [tokens][heads][head dim]
     ready into q_out (evl_kv8_append): an RMS norm per head with q_norm / k_norm [head dim]
     float32, then the rotation by rope [positions][rope dim / 2][2] float32 (cos, sin)."""
-    key = ("append", cache.kv_heads, cache.head_dim, interleaved, _layout(k, v, q, q_out, rope, q_norm, k_norm))
+    key = ("append", cache.kv_heads, cache.head_dim, cache._device, batch._device,
+           _layout(k, v, q, q_out, rope, q_norm, k_norm, err))
     plan = _plans.get(key)
     if plan is None:
+        _device_of(k, v, q, q_out, rope, q_norm, k_norm, err, known=(cache._device, batch._device))
+        _check_err(err)
         plan = _planned(key, _append_plan(cache, k, v, q, q_out, rope, q_norm, k_norm))
     total, kind, kst, vst, qst, ost, heads, rl, rd = plan
     prep = None
     if rope is not None or q_norm is not None or k_norm is not None:
         prep = C.byref(_Kv8Prep(_PREP_BYTES, rd, int(interleaved), rl, _ptr(rope), _ptr(q_norm), _ptr(k_norm), eps, 0))
     _check(runtime.lib().evl_kv8_append(cache._ref, batch._of(total, cache.page_size), prep, kind, k.data_ptr(), kst,
-                                        v.data_ptr(), vst, _ptr(q), qst, heads, _ptr(q_out), ost, _err(err), stream))
+                                        v.data_ptr(), vst, _ptr(q), qst, heads, _ptr(q_out), ost, _ptr(err), stream))
 
 
 _PREP_BYTES = C.sizeof(_Kv8Prep)
@@ -253,19 +271,22 @@ def kv8_attention(cache: Kv8Cache, batch: Kv8Batch, q, out, scale: float = 0.0, 
     """out [tokens][heads][head dim] = attention of q over the cache, each token up to its own
     position (evl_kv8_attention); scale 0 is 1 / sqrt(head dim). workspace: a device buffer of
     kv8_attention_workspace bytes, 256-byte aligned."""
-    key = ("attention", cache.head_dim, _layout(q, out, workspace))
+    key = ("attention", cache.head_dim, cache._device, batch._device, _layout(q, out, workspace, err))
     plan = _plans.get(key)
     if plan is None:
+        _device_of(q, out, workspace, err, known=(cache._device, batch._device))
+        _check_err(err)
         total, kind = q.shape[0], _kind(q)
         heads, qst = _heads(q, total, cache.head_dim, "q")
         oh, ost = _heads(out, total, cache.head_dim, "out")
         _need(oh == heads and out.dtype == q.dtype, "out must have the shape and type of q")
         size = 0
         if workspace is not None:
-            _need(workspace.numel() <= 1 or workspace.stride()[-1] == 1, "workspace must be contiguous")
+            _need(len(workspace.shape) == 1 and (workspace.shape[0] <= 1 or workspace.stride()[0] == 1),
+                  "workspace must be one contiguous dimension")
             size = workspace.numel() * workspace.element_size()
         plan = _planned(key, (total, kind, heads, qst, ost, size))
     total, kind, heads, qst, ost, size = plan
     _check(runtime.lib().evl_kv8_attention(cache._ref, batch._of(total, cache.page_size), kind, q.data_ptr(), qst, heads,
                                            scale, out.data_ptr(), ost, workspace.data_ptr() if size else None, size,
-                                           _err(err), stream))
+                                           _ptr(err), stream))

@@ -301,7 +301,9 @@ evl_status evl_i8_matmul(const int8_t* d_x, uint64_t x_stride, const float* d_x_
  *   its scale:  d_k_scales[p * scale_stride + h * (page_size / 16) + r / 16]
  * and the same for d_v. head_dim 64, 128 or 256; page_size 16, 32 or 64; page_stride (bytes)
  * a multiple of 16, the code buffers 16-byte aligned. A block's first append sets its codes
- * and scale, so pages need no initial value. */
+ * and scale, so pages need no initial value. Scales are 0 or positive (NaN: a block that held
+ * a value that is not finite); a caller that writes them itself keeps to that, and a
+ * subnormal value scale counts as 0. */
 typedef struct evl_kv8_cache {
     uint32_t struct_size; /* sizeof(evl_kv8_cache) */
     uint32_t kv_heads, head_dim, page_size, n_pages, reserved;
@@ -366,8 +368,11 @@ evl_status evl_kv8_attention_workspace_bytes(const evl_kv8_cache* cache, const e
  * head h / (heads / kv_heads). d_q and d_out [total][heads][head_dim] of `type`, tokens q_stride /
  * out_stride elements apart, 16-byte aligned, strides multiples of 16 bytes. heads a multiple of
  * kv_heads. scale 0: 1 / sqrt(head_dim). A row that sees no position gives zeros; a query row that
- * holds an infinity or a NaN gives NaN. Rows of d_out that belong to no sequence are left as they
- * were. d_workspace: evl_kv8_attention_workspace_bytes, 256-byte aligned, needing no initial
+ * holds an infinity or a NaN gives NaN. Scores are held in f32 with the base-2 exponent of the
+ * value scale added, so they are good to 2^-24 of their size, and beyond 1e38 in magnitude to
+ * nothing. Rows of d_out that belong to no sequence are left as they were. One kernel serves all
+ * sequences of a call, chosen by max_new: a batch that mixes prompts with single tokens gives
+ * the same sums but is faster as two calls. d_workspace: evl_kv8_attention_workspace_bytes, 256-byte aligned, needing no initial
  * value; calls that may overlap in time need one each. */
 evl_status evl_kv8_attention(const evl_kv8_cache* cache, const evl_kv8_batch* batch, uint32_t type, const void* d_q,
                              uint64_t q_stride, uint32_t heads, float scale, void* d_out, uint64_t out_stride,

@@ -166,3 +166,49 @@ def test_plain_forms_agree_with_their_definition():
     ref.append(codes, scales, np.array([[2, 0, 3]]), [40], [40], rows)
     got = ref.values(codes, scales, np.array([2, 0, 3]), 40)
     assert np.abs(got - rows).max() <= 0.5001 * np.abs(rows).max() / 127
+
+
+class On(Fake):
+    """The same with a device."""
+
+    def __init__(self, shape, device, dtype="float32", **k):
+        super().__init__(shape, dtype, **k)
+        self.device = device
+
+
+def test_tensors_of_one_call_are_on_one_device():
+    a, b = "cuda:0", "cuda:1"
+
+    def cache(scales=a):
+        return int8.Kv8Cache(On((4, 2, 16, 64), a, "int8"), On((4, 2, 16, 64), a, "int8"), On((4, 2, 1), scales), On((4, 2, 1), scales))
+
+    def batch(lens=a, all=a):
+        return int8.Kv8Batch(On((2, 4), all, "int32"), On((3,), all, "int32"), On((2,), lens, "int32"), 2, 64)
+
+    bad = lambda fn, *x, **k: refused("InvalidInput", "one device", fn, *x, **k)  # noqa: E731
+    bad(int8.quantize_rows, On((2, 32), a), On((2, 32), "cpu", "int8"), On((2,), a))
+    bad(int8.matmul, On((2, 32), a, "int8"), On((2,), a), On((8, 32), b, "int8"), On((8,), a), On((2, 8), a))
+    bad(int8.matmul, On((2, 32), a, "int8"), On((2,), a), On((8, 32), a, "int8"), On((8,), a), On((2, 8), a),
+        err=On((1,), "cpu", "int32"))
+    bad(cache, scales="cpu")
+    bad(batch, lens=b)
+    rows = On((3, 2, 64), a)
+    bad(int8.kv8_append, cache(), batch(), rows, On((3, 2, 64), b))
+    bad(int8.kv8_append, cache(), batch(b, b), rows, rows)
+    bad(int8.kv8_append, cache(), batch(), rows, rows, rope=On((64, 32, 2), "cpu"))
+    bad(int8.kv8_attention, cache(), batch(), rows, On((3, 2, 64), "cpu"))
+    bad(int8.kv8_attention, cache(), batch(b, b), rows, rows)
+    bad(int8.kv8_attention, cache(), batch(), rows, rows, workspace=On((512,), b, "uint8"))
+
+
+def test_workspace_is_one_run_of_memory():
+    for shape, stride in (((8, 64), (128, 1)), ((512,), (2,))):
+        refused("InvalidInput", "workspace", int8.kv8_attention, _kv(), _batch(), _rows(heads=4), _rows(heads=4),
+                workspace=Fake(shape, "uint8", stride=stride))
+
+
+def test_a_batch_keeps_few_descriptors():
+    b = _batch()
+    for total in range(1, 1000):
+        b._of(total, 16)
+    assert len(b._by_total) <= 64
