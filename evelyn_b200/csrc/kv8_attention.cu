@@ -683,12 +683,12 @@ __device__ __forceinline__ uint32_t panel_at(uint32_t rows, uint32_t r, uint32_t
     return (p >> 3) * (rows * 128u) + r * 128u + (((p & 7u) ^ (r & 7u)) << 4);
 }
 // 16 codes to f16, two 16-byte pieces
-__device__ __forceinline__ void codes_to_panel(uint8_t* panel, uint32_t rows, uint32_t r, uint32_t c, uint4 w, bool zero) {
+__device__ __forceinline__ void codes_to_panel(uint8_t* panel, uint32_t rows, uint32_t r, uint32_t c, uint4 w) {
     uint32_t h[8];
     const uint32_t in[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const uint32_t b = zero ? 0x80808080u : in[i] ^ 0x80808080u;
+        const uint32_t b = in[i] ^ 0x80808080u;
         h[2 * i] = codes_h2(b, 0x4140);
         h[2 * i + 1] = codes_h2(b, 0x4342);
     }
@@ -708,8 +708,8 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
     static_assert(RT * (HD + 2 * kSCols) <= 512 && (RT == 1 || HD + 2 * kSCols <= 256), "tensor memory");
     constexpr uint32_t kSoftWarps = 4 * RT, kTileCols = RT == 2 ? 256 : 512;  // tensor memory columns per row tile
     extern __shared__ uint8_t raw_smem[];
-    constexpr uint32_t FS = 8;  // steps of block factors
-    __shared__ __align__(8) uint64_t k_full[ST], k_empty[ST], v_full[ST], v_empty[ST], f_full[FS], f_empty[FS];
+    constexpr uint32_t FG = 8, FS = 2 * FG;  // steps of block factors handed over together, and kept
+    __shared__ __align__(8) uint64_t k_full[ST], k_empty[ST], v_full[ST], v_empty[ST], f_full[2], f_empty[2], c_full[RAW], c_empty[RAW];
     __shared__ __align__(8) uint64_t s_full[RT][2], p_full[RT][2], o_done[RT], q_full, fin[RT];
     __shared__ float4 f_blk[FS][NB];  // key scale, exponent of the value scale, 2^-exponent, mantissa
     __shared__ uint32_t tmem_base;
@@ -731,22 +731,27 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
     const int32_t b0 = (int32_t)(split * P.chunk), b1 = min(nblk, b0 + (int32_t)P.chunk);
     if (b0 >= nblk && split > 0) return;
     const uint32_t steps = b1 > b0 ? (uint32_t)(b1 - b0 + (int32_t)NB - 1) / NB : 0;
+    const uint32_t used = ((uint32_t)nrow + kTileRows - 1) / kTileRows;  // row tiles that hold rows; the others' warps rest
 
     uint8_t* smem = raw_smem + ((1024u - (smem_addr(raw_smem) & 1023u)) & 1023u);
     uint8_t* sq = smem;                                  // [RT] q panels
     uint8_t* skv = smem + RT * kQParts * kQPart;         // [ST][K | V] panels
-    uint8_t* sraw = skv + ST * kStage;                  // [RAW][K | V] codes, 16 bytes per thread and piece
+    uint8_t* sraw = skv + ST * kStage;                  // [RAW][K | V] codes, block after block
     if (tid == 0) {
         abort_flag = 0;
         for (uint32_t i = 0; i < ST; ++i) {
             mbar_init(&k_full[i], 4);
-            mbar_init(&k_empty[i], RT);
+            mbar_init(&k_empty[i], used);
             mbar_init(&v_full[i], 4);
-            mbar_init(&v_empty[i], RT);
+            mbar_init(&v_empty[i], used);
         }
-        for (uint32_t i = 0; i < FS; ++i) {
+        for (uint32_t i = 0; i < RAW; ++i) {
+            mbar_init(&c_full[i], 1);
+            mbar_init(&c_empty[i], 4);
+        }
+        for (uint32_t i = 0; i < 2; ++i) {
             mbar_init(&f_full[i], 1);
-            mbar_init(&f_empty[i], kSoftWarps);
+            mbar_init(&f_empty[i], 4 * used);
         }
         for (uint32_t i = 0; i < RT; ++i) {
             mbar_init(&s_full[i][0], 1);
@@ -757,7 +762,7 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
             mbar_init(&o_done[i], 1);
             mbar_init(&fin[i], 1);
         }
-        mbar_init(&q_full, kSoftWarps);
+        mbar_init(&q_full, 4 * used);
         fence_barrier_init();
     }
     if (warp == kSoftWarps + 4) {
@@ -771,7 +776,7 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
     tc_after();
     const uint32_t tm = tmem_base;
 
-    if (warp < kSoftWarps) {
+    if (warp < 4 * used) {
         // ---------------------------------------------------------------- softmax: one row per thread
         const uint32_t rt = warp >> 2, quad = warp & 3, lr = quad * 32 + lane;
         const int32_t row = r0 + (int32_t)(rt * kTileRows + lr);
@@ -833,20 +838,35 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
             __syncwarp();
             if (lane == 0) mbar_arrive(&q_full);
         }
-        const int32_t last = live ? sp.base + tok : -1;
+        const int32_t last = sp.base + tok;  // (lanes past the last row do its work again and write nothing)
+        const bool idle = r0 + (int32_t)(rt * kTileRows + quad * 32) >= rows;  // the whole warp
         // no row of this warp hides a position before this one
         const int32_t open = sp.base + min(r0 + (int32_t)(rt * kTileRows + quad * 32), rows - 1) / (int32_t)P.group;
         const uint32_t to = tm + rt * kTileCols + ((quad * 32) << 16);  // O, then the score buffers
         float M = kNegBig, l = 0.f;
         bool ok = true;
         for (uint32_t j = 0; j < steps && ok; ++j) {
-            const uint32_t st = j % FS;
-            ok = warp_wait(&f_full[st], (j / FS) & 1, &abort_flag) && warp_wait(&s_full[rt][j & 1], (j >> 1) & 1, &abort_flag);
+            const uint32_t st = j % FS, fg = j / FG % 2;
+            if (j % FG == 0) ok = warp_wait(&f_full[fg], (j / FG / 2) & 1, &abort_flag);
+            ok = ok && warp_wait(&s_full[rt][j & 1], (j >> 1) & 1, &abort_flag);
             if (!ok) break;
             tc_after();
+            auto done = [&] {
+                tmem_st_wait();
+                tc_before();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&p_full[rt][j & 1]);
+                    if (j % FG == FG - 1) mbar_arrive(&f_empty[fg]);
+                }
+            };
+            if (idle) {  // (what these rows add up goes nowhere)
+                done();
+                continue;
+            }
             const uint32_t ts = to + HD + (j & 1) * kSCols;
             const int32_t p0 = (b0 + (int32_t)(j * NB)) * 16;
-            const bool masked = __any_sync(0xffffffffu, p0 + (int32_t)NP - 1 > open || !live);
+            const bool masked = p0 + (int32_t)NP - 1 > open;
             float f[NB], e[NB], down[NB], mant[NB];
             bool far = false;  // a block far below the maximum, or one of zeros
 #pragma unroll
@@ -862,38 +882,32 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
             if (TERMS == 1 && j > 0 && !masked && !__any_sync(0xffffffffu, far)) {
                 uint32_t hi[NP / 2];
                 float add = 0.f, tot = 0.f;
+                uint32_t v[2][16];
+                tmem_ld16(ts, v[0]);
+                tmem_ld_wait();
 #pragma unroll
-                for (uint32_t c = 0; c < NP; c += 32) {
-                    uint32_t v[32];
-                    tmem_ld32(ts + c, v);
-                    tmem_ld_wait();
+                for (uint32_t b = 0; b < NB; ++b) {  // the next block's scores on their way meanwhile
+                    if (b + 1 < NB) tmem_ld16(ts + 16 * (b + 1), v[(b + 1) & 1]);
+                    const uint32_t(&x)[16] = v[b & 1];
+                    const uint64_t ff = pack2(f[b], f[b]), off = pack2(e[b] - M, e[b] - M);
+                    uint64_t sum = 0;
 #pragma unroll
-                    for (uint32_t b = c / 16; b < c / 16 + 2; ++b) {
-                        const uint64_t ff = pack2(f[b], f[b]), off = pack2(e[b] - M, e[b] - M);
-                        uint64_t sum = 0;
-#pragma unroll
-                        for (uint32_t i = 0; i < 8; ++i) {
-                            const uint64_t x = fma2(pack2(v[16 * b - c + 2 * i], v[16 * b - c + 2 * i + 1]), ff, off);
-                            const float w0 = exp2_fast(lo2(x)), w1 = exp2_fast(hi2(x));
-                            sum = add2(sum, pack2(w0, w1));
-                            hi[8 * b + i] = pack_h2(w0, w1);
-                        }
-                        const float s1 = lo2(sum) + hi2(sum);
-                        tot += s1;
-                        add = fmaf(s1, down[b], add);
+                    for (uint32_t i = 0; i < 8; ++i) {
+                        const uint64_t y = fma2(pack2(x[2 * i], x[2 * i + 1]), ff, off);
+                        const float w0 = exp2_fast(lo2(y)), w1 = exp2_fast(hi2(y));
+                        sum = add2(sum, pack2(w0, w1));
+                        hi[8 * b + i] = pack_h2(w0, w1);
                     }
+                    const float s1 = lo2(sum) + hi2(sum);
+                    tot += s1;
+                    add = fmaf(s1, down[b], add);
+                    if (b + 1 < NB) tmem_ld_wait();
                 }
                 if (__all_sync(0xffffffffu, tot < 16384.f)) {
                     l += add;
 #pragma unroll
                     for (uint32_t b = 0; b < NB; ++b) tmem_st8(ts + 8 * b, hi + 8 * b);
-                    tmem_st_wait();
-                    tc_before();
-                    __syncwarp();
-                    if (lane == 0) {
-                        mbar_arrive(&p_full[rt][j & 1]);
-                        mbar_arrive(&f_empty[st]);
-                    }
+                    done();
                     continue;
                 }
             }
@@ -987,13 +1001,7 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
             };
             if (masked || __any_sync(0xffffffffu, far)) weights(std::true_type{});
             else weights(std::false_type{});
-            tmem_st_wait();
-            tc_before();
-            __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(&p_full[rt][j & 1]);
-                mbar_arrive(&f_empty[st]);
-            }
+            done();
         }
         // (one phase after the other: a parity says nothing about a phase two steps away. Inside the loop
         // the scores of step j imply the product of step j - 2)
@@ -1037,114 +1045,89 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
                 }
             }
         }
+    } else if (warp < kSoftWarps) {
     } else if (warp < kSoftWarps + 4) {
         // ---------------------------------------------------------------- producers
         const uint32_t pt = tid - 32 * kSoftWarps;  // 0..127
         constexpr uint32_t CPR = HD / 16, N = NP * CPR / 128;  // 16-code pieces per row, per thread and operand
-        const int32_t* table = a.b.table + (uint64_t)s * a.b.table_stride;
-        const uint32_t lb = 31 - __clz(a.c.page_size / 16);  // log2 of the blocks of a page: 0, 1 or 2
-        // Codes travel ahead in a ring of their own: every thread copies the pieces that it will
-        // widen itself, RAW steps ahead and asynchronously, so the producers never wait for one
-        // another. RAW + 1 steps ahead the page of each of the thread's pieces is looked up.
-        int32_t page[N];
-        uint64_t at[N];  // of the piece inside its page, for the first block of the page
-#pragma unroll
-        for (uint32_t i = 0; i < N; ++i) {
-            const uint32_t piece = pt + 128 * i, r = piece / CPR;
-            at[i] = (uint64_t)(h * a.c.page_size + r % 16) * HD + 16 * (piece % CPR);
-        }
-        auto pages = [&](uint32_t j) {
-#pragma unroll
-            for (uint32_t i = 0; i < N; ++i) {
-                const int32_t blk = b0 + (int32_t)(j * NB + (pt + 128 * i) / CPR / 16);
-                page[i] = blk < b1 ? __ldg(table + ((uint32_t)blk >> lb)) : -1;
-            }
-        };
-        uint32_t gone = 0;  // bits: this thread's pieces of step j % RAW that have no (valid) page
-        auto fetch = [&](uint32_t j) {
-            const uint32_t rs = j % RAW;
-            uint8_t* raw = sraw + rs * (2 * NP * HD);
-            gone &= ~(((1u << N) - 1) << (rs * N));
-#pragma unroll
-            for (uint32_t i = 0; i < N; ++i) {
-                const uint32_t piece = pt + 128 * i;
-                const uint32_t sub = (uint32_t)(b0 + (int32_t)(j * NB + piece / CPR / 16)) & ((1u << lb) - 1);
-                if ((uint32_t)page[i] < a.c.n_pages) {
-                    const uint64_t o = (uint32_t)page[i] * a.c.page_stride + at[i] + sub * (16 * HD);
-                    cp_async<16>(raw + 16 * piece, a.c.k + o);
-                    cp_async<16>(raw + NP * HD + 16 * piece, a.c.v + o);
-                } else {
-                    gone |= 1u << (rs * N + i);
-                }
-            }
-        };
-        pages(0);
-#pragma unroll
-        for (uint32_t j = 0; j < RAW; ++j) {
-            if (j < steps) {
-                fetch(j);
-                pages(j + 1);
-            }
-            cp_async_commit();
-        }
-        auto widen = [&](uint8_t* panel, const uint8_t* raw, uint32_t none) {
+        // Piece of a thread: row and 16-code column. Eight neighbouring lanes take two rows of four columns, so
+        // that the f16 pieces that they write lie in eight different 16-byte columns of the banks.
+        auto row_of = [](uint32_t p) { return CPR == 4 ? p / 4 : p / (2 * CPR) * 2 + (p >> 2 & 1); };
+        auto col_of = [](uint32_t p) { return CPR == 4 ? p % 4 : (p & 3) | (p % (2 * CPR) >> 3) << 2; };
+        auto piece = [&](uint32_t i) { return pt + 128 * i; };
+        auto code_at = [&](uint32_t i) { return row_of(piece(i)) * HD + 16 * col_of(piece(i)); };
+        // (blocks without a valid page were not copied: whatever codes lie there have weight 0)
+        auto widen = [&](uint8_t* panel, const uint8_t* raw) {
             uint4 w[N];
 #pragma unroll
-            for (uint32_t i = 0; i < N; ++i) w[i] = *reinterpret_cast<const uint4*>(raw + 16 * (pt + 128 * i));
+            for (uint32_t i = 0; i < N; ++i) w[i] = *reinterpret_cast<const uint4*>(raw + code_at(i));
 #pragma unroll
-            for (uint32_t i = 0; i < N; ++i) {
-                const uint32_t piece = pt + 128 * i;
-                codes_to_panel(panel, NP, piece / CPR, piece % CPR, w[i], none >> i & 1);
-            }
+            for (uint32_t i = 0; i < N; ++i) codes_to_panel(panel, NP, row_of(piece(i)), col_of(piece(i)), w[i]);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
         };
-        auto copy = [&](uint8_t* panel, const uint8_t* raw, uint32_t none) {  // the codes as they are
+        auto copy = [&](uint8_t* panel, const uint8_t* raw) {  // the codes as they are
 #pragma unroll
-            for (uint32_t i = 0; i < N; ++i) {
-                const uint32_t piece = pt + 128 * i;
-                const uint4 w = *reinterpret_cast<const uint4*>(raw + 16 * piece);
-                *reinterpret_cast<uint4*>(panel + bytes_at<HD>(NP, piece / CPR, piece % CPR)) =
-                    none >> i & 1 ? make_uint4(0, 0, 0, 0) : w;
-            }
+            for (uint32_t i = 0; i < N; ++i)
+                *reinterpret_cast<uint4*>(panel + bytes_at<HD>(NP, row_of(piece(i)), col_of(piece(i)))) =
+                    *reinterpret_cast<const uint4*>(raw + code_at(i));
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
         };
         for (uint32_t j = 0; j < steps; ++j) {  // (after an abort the loop runs out quickly: every wait gives up at once)
-            const uint32_t st = j % ST, rs = j % RAW, none = gone >> (rs * N);
-            cp_async_wait<(int)RAW - 1>();
+            const uint32_t st = j % ST, rs = j % RAW;
             const uint8_t* raw = sraw + rs * (2 * NP * HD);
             uint8_t* dst = skv + st * kStage;
+            warp_wait(&c_full[rs], (j / RAW) & 1, &abort_flag);
             if (j >= ST) warp_wait(&k_empty[st], (j / ST - 1) & 1, &abort_flag);
-            if (TERMS == 1) widen(dst, raw, none);
-            else copy(dst, raw, none);
+            if (TERMS == 1) widen(dst, raw);
+            else copy(dst, raw);
             if (lane == 0) mbar_arrive(&k_full[st]);
             if (j >= ST) warp_wait(&v_empty[st], (j / ST - 1) & 1, &abort_flag);
-            widen(dst + kK, raw + NP * HD, none);
-            if (lane == 0) mbar_arrive(&v_full[st]);
-            if (j + RAW < steps) {
-                fetch(j + RAW);
-                pages(j + RAW + 1);
+            widen(dst + kK, raw + NP * HD);
+            if (lane == 0) {
+                mbar_arrive(&v_full[st]);
+                mbar_arrive(&c_empty[rs]);
             }
-            cp_async_commit();
         }
-        cp_async_wait<0>();
     } else if (warp == kSoftWarps + 4 + RT) {
-        // ---------------------------------------------------------------- the blocks' factors
-        // one lane per block, 32 / NB steps looked up together
+        // ---------------------------------------------------------------- the blocks: their factors and codes
+        // one lane per block, 32 / NB steps looked up together; a block's codes are one run of memory for
+        // K and one for V, each copied by its lane
+        constexpr uint32_t LS = 32 / NB;
+        static_assert(LS % FG == 0, "whole groups of factors");
         const int32_t* table = a.b.table + (uint64_t)s * a.b.table_stride;
-        const uint32_t lb = 31 - __clz(a.c.page_size / 16);
-        for (uint32_t j0 = 0; j0 < steps; j0 += 32 / NB) {
+        const uint32_t lb = 31 - __clz(a.c.page_size / 16);  // log2 of the blocks of a page: 0, 1 or 2
+        uint32_t n = 0;  // steps whose copies were issued
+        bool ok = true;
+        for (uint32_t j0 = 0; j0 < steps && ok; j0 += LS) {
             const int32_t blk = b0 + (int32_t)(j0 * NB + lane);
             const int32_t page = blk < b1 ? __ldg(table + ((uint32_t)blk >> lb)) : -1;
+            const uint32_t sub = (uint32_t)blk & ((1u << lb) - 1);
             const bool hidden = (uint32_t)page >= a.c.n_pages;
             if (hidden && blk < b1) flag_error(a.err, DEV_ERR_POSITION);
             float sk = 0.f, sv = 0.f;
             if (!hidden) {
-                const uint64_t at = (uint32_t)page * a.c.scale_stride + (h << lb) + ((uint32_t)blk & ((1u << lb) - 1));
+                const uint64_t at = (uint32_t)page * a.c.scale_stride + (h << lb) + sub;
                 sk = __ldg(a.c.ks + at);
                 sv = __ldg(a.c.vs + at);
             }
+            const uint64_t code = hidden ? 0 : (uint32_t)page * a.c.page_stride + (uint64_t)(h * a.c.page_size + 16 * sub) * HD;
+            auto copies = [&](uint32_t j) {
+                const uint32_t rs = j % RAW, i = j - j0;
+                if (j >= RAW) ok = warp_wait(&c_empty[rs], (j / RAW - 1) & 1, &abort_flag);
+                if (!ok) return;
+                const bool mine = lane / NB == i && !hidden;
+                const uint32_t count = __popc(__ballot_sync(0xffffffffu, mine));
+                if (lane == 0) mbar_arrive_expect_tx(&c_full[rs], count * (2 * 16 * HD));
+                __syncwarp();
+                if (mine) {
+                    uint8_t* dst = sraw + rs * (2 * NP * HD) + lane % NB * (16 * HD);
+                    tma_load_1d(dst, a.c.k + code, 16 * HD, &c_full[rs]);
+                    tma_load_1d(dst + NP * HD, a.c.v + code, 16 * HD, &c_full[rs]);
+                }
+                ++n;
+            };
             // sv = mant 2^e (TERMS = 2), or e = log2 sv; zeros have mant 0 and an exponent that no maximum
             // notices; a scale that is not finite makes the weights of the rows that see it so
             const uint32_t sb = __float_as_uint(sv);
@@ -1157,16 +1140,19 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
                             : eb == 0   ? kZeroExp
                             : TERMS == 2 ? (float)(eb - 127)
                                          : log2f(sv);
-            for (uint32_t i = 0; i < 32 / NB && j0 + i < steps; ++i) {
-                const uint32_t j = j0 + i, fs = j % FS;
-                if (j >= FS) warp_wait(&f_empty[fs], (j / FS - 1) & 1, &abort_flag);
+            for (uint32_t g = 0; g < LS / FG && j0 + g * FG < steps && ok; ++g) {
+                const uint32_t grp = j0 / FG + g;
+                if (grp >= 2) ok = warp_wait(&f_empty[grp % 2], (grp / 2 - 1) & 1, &abort_flag);
                 __syncwarp();
-                if (lane / NB == i) f_blk[fs][lane % NB] = make_float4(sk, e, down, mant);
+                if (lane / NB / FG == g) f_blk[(j0 + lane / NB) % FS][lane % NB] = make_float4(sk, e, down, mant);
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&f_full[fs]);
+                if (lane == 0) mbar_arrive(&f_full[grp % 2]);
+                for (uint32_t i = 0; i < FG && j0 + g * FG + i < steps && ok; ++i) copies(j0 + g * FG + i);
             }
         }
-    } else if (warp < kSoftWarps + 4 + RT && steps && elect_one()) {
+        if (!ok)  // copies in flight land before the CTA leaves
+            for (uint32_t i = 0; i < RAW && i < n; ++i) mbar_wait(&c_full[i], ((n - 1 - i) / RAW) & 1);
+    } else if (warp < kSoftWarps + 4 + used && steps && elect_one()) {
         // ---------------------------------------------------------------- MMA: one thread per row tile, so that
         // one tile's products run while the other waits for its weights
         const uint32_t rt = warp - kSoftWarps - 4;
