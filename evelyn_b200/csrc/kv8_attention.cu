@@ -852,6 +852,9 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
             if (!ok) break;
             tc_after();
             auto done = [&] {
+                // The last products are waited for behind the loop, where a parity cannot tell them from those two
+                // steps before: the step before the last has to be seen to end while the last one still needs this warp
+                if (j > 0 && j + 1 == steps) ok = warp_wait(&o_done[rt], (j - 1) & 1, &abort_flag);
                 tmem_st_wait();
                 tc_before();
                 __syncwarp();
@@ -1003,9 +1006,6 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
             else weights(std::false_type{});
             done();
         }
-        // (one phase after the other: a parity says nothing about a phase two steps away. Inside the loop
-        // the scores of step j imply the product of step j - 2)
-        if (steps > 1 && ok) ok = warp_wait(&o_done[rt], (steps - 2) & 1, &abort_flag);
         if (steps && ok) ok = warp_wait(&o_done[rt], (steps - 1) & 1, &abort_flag);
         tc_after();
         if (ok) {
@@ -1023,8 +1023,9 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
 #pragma unroll
                     for (int i = 0; i < 32; ++i) o[i] = 0;
                 }
-                if (!live) continue;
-                if (P.splits > 1) {
+                __syncwarp();
+                if (!live) {
+                } else if (P.splits > 1) {
 #pragma unroll
                     for (int i = 0; i < 32; i += 4)
                         *reinterpret_cast<uint4*>(P.part_o + slot * HD + c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
@@ -1043,6 +1044,7 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
                         *reinterpret_cast<uint4*>(out + c + i) = *reinterpret_cast<uint4*>(y);
                     }
                 }
+                __syncwarp();
             }
         }
     } else if (warp < kSoftWarps) {

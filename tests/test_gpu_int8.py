@@ -576,6 +576,28 @@ def test_outputs_do_not_depend_on_the_batch_they_run_in():
         assert np.array_equal(host(getattr(whole, d))[rows], host(getattr(parts, d))[rows])
 
 
+def test_calls_on_several_streams_at_once():
+    """Prompts of few steps on four streams, each with its own output and workspace: nothing waits in vain
+    for a product that has already ended, and the results are those of a call alone."""
+    t = gu.torch()
+    rng = np.random.default_rng(15)
+    lens, new = [200, 90, 130], [30, 90, 12]
+    kv = Kv(rng, 2, 128, 32, lens)
+    q = t.randn(sum(new), 8, 128, generator=t.Generator("cuda:0").manual_seed(3), device="cuda:0").to(t.bfloat16)
+    want = host(_attend(kv, lens, new, q, "bf16"))
+    b = kv.batch(lens, new)
+    streams = [t.cuda.Stream() for _ in range(4)]
+    outs = [t.full(q.shape, 7.0, dtype=q.dtype, device="cuda:0") for _ in streams]
+    spaces = [t.empty(max(1, int8.kv8_attention_workspace(kv.cache, b, q)), dtype=t.uint8, device="cuda:0") for _ in streams]
+    t.cuda.synchronize()
+    for _ in range(100):
+        for s, o, w in zip(streams, outs, spaces):
+            int8.kv8_attention(kv.cache, b, q, o, workspace=w, err=kv.err, stream=s.cuda_stream)
+    t.cuda.synchronize()
+    assert int(kv.err) == 0
+    assert all(same(host(o), want) for o in outs)
+
+
 def test_calls_of_no_tokens():
     t = gu.torch()
     kv = Kv(np.random.default_rng(2), 1, 64, 16, [16])
