@@ -535,7 +535,14 @@ template <class T, int HD> __global__ void __launch_bounds__(32 * kJoinWarps) kv
 // anyway (TERMS = 1).
 // Bound: the exponentials (16 a clock and SM) and the tensor pipe, about equally.
 constexpr uint32_t kTileRows = 128;
-constexpr uint32_t kTileMin = 48;  // rows per (sequence, kv head) from which it is used
+// Rows per (sequence, kv head) from which it may be used, and the blocks of 16 positions times tiles of eight rows
+// that each warp of the other kernel would then have to take. Measured over 64 to 256 dims, 16 to 64
+// rows, 300 to 16000 positions of 1 to 64 sequences: 1.2 % over the better kernel's time on average, 26 % at
+// most; on either side of the rule, 32 rows over 4099 positions of 9 sequences with 2 kv heads of
+// 256 dims: 30 us against 51; 32 rows over 600 positions of 2 sequences with 8 of 128: 13.1 against 12.3.
+// (f32 up to 128 dims has one row tile and twice the products, and its rows pay later.)
+__host__ __device__ constexpr uint32_t tile_min(int hd, int terms) { return terms == 2 && hd <= 128 ? 48 : 24; }
+constexpr uint64_t kTileWork = 3;
 
 struct Role {  // per (HD, TERMS): row tiles, positions per step, stages of f16 panels, of codes
     uint32_t rt, np, stages, raw;
@@ -705,12 +712,14 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
     constexpr uint32_t kQPart = q_part(HD, TERMS), kQParts = q_parts(TERMS);
     constexpr uint32_t kK = k_stage(HD, TERMS), kV = NP * HD * 2, kStage = kK + kV;  // K and V of a stage
     constexpr uint32_t kSCols = TERMS == 2 ? 3 * NP : NP;  // tensor memory columns of a score buffer
-    static_assert(RT * (HD + 2 * kSCols) <= 512 && (RT == 1 || HD + 2 * kSCols <= 256), "tensor memory");
+    // log2 of a row tile's score buffers: as many as its share of the tensor memory holds beside O, up to four
+    constexpr uint32_t kMostBuffers = HD + 4 * kSCols <= 512 ? 2 : 1, kShared = RT == 1 ? kMostBuffers : 1;
+    static_assert(RT * (HD + (kSCols << kShared)) <= 512 && (RT == 1 || HD + 2 * kSCols <= 256), "tensor memory");
     constexpr uint32_t kSoftWarps = 4 * RT, kTileCols = RT == 2 ? 256 : 512;  // tensor memory columns per row tile
     extern __shared__ uint8_t raw_smem[];
     constexpr uint32_t FG = 8, FS = 2 * FG;  // steps of block factors handed over together, and kept
     __shared__ __align__(8) uint64_t k_full[ST], k_empty[ST], v_full[ST], v_empty[ST], f_full[2], f_empty[2], c_full[RAW], c_empty[RAW];
-    __shared__ __align__(8) uint64_t s_full[RT][2], p_full[RT][2], o_done[RT], q_full, fin[RT];
+    __shared__ __align__(8) uint64_t s_full[RT][4], p_full[RT][4], o_done[RT][4], q_full, fin[RT];
     __shared__ float4 f_blk[FS][NB];  // key scale, exponent of the value scale, 2^-exponent, mantissa
     __shared__ uint32_t tmem_base;
     __shared__ volatile int abort_flag;
@@ -732,6 +741,7 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
     if (b0 >= nblk && split > 0) return;
     const uint32_t steps = b1 > b0 ? (uint32_t)(b1 - b0 + (int32_t)NB - 1) / NB : 0;
     const uint32_t used = ((uint32_t)nrow + kTileRows - 1) / kTileRows;  // row tiles that hold rows; the others' warps rest
+    const uint32_t lsb = RT == 2 && used == 1 ? kMostBuffers : kShared, nsb = 1u << lsb;  // score buffers of a row tile
 
     uint8_t* smem = raw_smem + ((1024u - (smem_addr(raw_smem) & 1023u)) & 1023u);
     uint8_t* sq = smem;                                  // [RT] q panels
@@ -754,12 +764,13 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
             mbar_init(&f_empty[i], 4 * used);
         }
         for (uint32_t i = 0; i < RT; ++i) {
-            mbar_init(&s_full[i][0], 1);
-            mbar_init(&s_full[i][1], 1);
-            // (one per buffer: a warp may finish the next step's weights before another has this one's)
-            mbar_init(&p_full[i][0], 4);
-            mbar_init(&p_full[i][1], 4);
-            mbar_init(&o_done[i], 1);
+            // (one of each per score buffer: a warp may finish the next step's weights before another has this
+            // one's, and a parity tells only neighbouring phases apart)
+            for (uint32_t k = 0; k < 4; ++k) {
+                mbar_init(&s_full[i][k], 1);
+                mbar_init(&p_full[i][k], 4);
+                mbar_init(&o_done[i][k], 1);
+            }
             mbar_init(&fin[i], 1);
         }
         mbar_init(&q_full, 4 * used);
@@ -848,18 +859,15 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
         for (uint32_t j = 0; j < steps && ok; ++j) {
             const uint32_t st = j % FS, fg = j / FG % 2;
             if (j % FG == 0) ok = warp_wait(&f_full[fg], (j / FG / 2) & 1, &abort_flag);
-            ok = ok && warp_wait(&s_full[rt][j & 1], (j >> 1) & 1, &abort_flag);
+            ok = ok && warp_wait(&s_full[rt][j % nsb], (j >> lsb) & 1, &abort_flag);
             if (!ok) break;
             tc_after();
             auto done = [&] {
-                // The last products are waited for behind the loop, where a parity cannot tell them from those two
-                // steps before: the step before the last has to be seen to end while the last one still needs this warp
-                if (j > 0 && j + 1 == steps) ok = warp_wait(&o_done[rt], (j - 1) & 1, &abort_flag);
                 tmem_st_wait();
                 tc_before();
                 __syncwarp();
                 if (lane == 0) {
-                    mbar_arrive(&p_full[rt][j & 1]);
+                    mbar_arrive(&p_full[rt][j % nsb]);
                     if (j % FG == FG - 1) mbar_arrive(&f_empty[fg]);
                 }
             };
@@ -867,7 +875,7 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
                 done();
                 continue;
             }
-            const uint32_t ts = to + HD + (j & 1) * kSCols;
+            const uint32_t ts = to + HD + j % nsb * kSCols;
             const int32_t p0 = (b0 + (int32_t)(j * NB)) * 16;
             const bool masked = p0 + (int32_t)NP - 1 > open;
             float f[NB], e[NB], down[NB], mant[NB];
@@ -952,7 +960,7 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
                 l = rebase(l, M, m);
                 M = m;
                 if (j > 0) {
-                    ok = warp_wait(&o_done[rt], (j - 1) & 1, &abort_flag);
+                    ok = warp_wait(&o_done[rt][(j - 1) % nsb], ((j - 1) >> lsb) & 1, &abort_flag);
                     if (!ok) break;
                     tc_after();
 #pragma unroll 1
@@ -1006,7 +1014,7 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
             else weights(std::false_type{});
             done();
         }
-        if (steps && ok) ok = warp_wait(&o_done[rt], (steps - 1) & 1, &abort_flag);
+        if (steps && ok) ok = warp_wait(&o_done[rt][(steps - 1) % nsb], ((steps - 1) >> lsb) & 1, &abort_flag);
         tc_after();
         if (ok) {
             const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);  // a row that sees nothing: zeros
@@ -1162,13 +1170,13 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
         bool ok = bwait(&q_full, 0, &abort_flag);
         auto scores = [&](uint32_t j) {
             const uint32_t st = j % ST;
-            // the buffer holds the weights of step j - 2 until their product has ended (products of
+            // the buffer holds the weights of step j - nsb until their product has ended (products of
             // different shapes are not ordered by their issue)
-            ok = ok && (j < 2 || bwait(&o_done[rt], (j - 2) & 1, &abort_flag)) &&
+            ok = ok && (j < nsb || bwait(&o_done[rt][j % nsb], ((j >> lsb) - 1) & 1, &abort_flag)) &&
                  bwait(&k_full[st], (j / ST) & 1, &abort_flag);
             if (!ok) return;
             tc_after();
-            const uint32_t kb = smem_addr(skv + st * kStage), ds = d + HD + (j & 1) * kSCols;
+            const uint32_t kb = smem_addr(skv + st * kStage), ds = d + HD + j % nsb * kSCols;
             if constexpr (TERMS == 1) {
 #pragma unroll
                 for (uint32_t k = 0; k < HD / 16; ++k)
@@ -1182,7 +1190,7 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
                         mma_i8(ds + x * NP, bytes_desc<HD>(qb + x * kQPart + (k / 4) * (kTileRows * 128) + (k % 4) * 32),
                                bytes_desc<HD>(kb + (k / 4) * (NP * 128) + (k % 4) * 32), i8_idesc(NP), k > 0);
             }
-            mma_commit(&s_full[rt][j & 1]);
+            mma_commit(&s_full[rt][j % nsb]);
             mma_commit(&k_empty[st]);
         };
         scores(0);
@@ -1190,17 +1198,17 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
             if (j + 1 < steps) scores(j + 1);
             const uint32_t st = j % ST, vb = smem_addr(skv + st * kStage + kK);
             ok = ok && bwait(&v_full[st], (j / ST) & 1, &abort_flag) &&
-                 bwait(&p_full[rt][j & 1], (j >> 1) & 1, &abort_flag);
+                 bwait(&p_full[rt][j % nsb], (j >> lsb) & 1, &abort_flag);
             if (!ok) break;
             tc_after();
-            const uint32_t pw = d + HD + (j & 1) * kSCols;
+            const uint32_t pw = d + HD + j % nsb * kSCols;
 #pragma unroll
             for (uint32_t x = 0; x < (uint32_t)TERMS; ++x)
 #pragma unroll
                 for (uint32_t k = 0; k < NP / 16; ++k)
                     mma_ts(d, pw + x * (NP / 2) + 8 * k, swizzled_desc(vb + k * 2048, NP * 128), f16_idesc(HD, true),
                            j > 0 || x > 0 || k > 0);
-            mma_commit(&o_done[rt]);
+            mma_commit(&o_done[rt][j % nsb]);
             mma_commit(&v_empty[st]);
         }
         if (!ok) {  // the MMAs in flight end before the tensor memory is freed
@@ -1224,20 +1232,22 @@ struct Shape {
 Shape shape_of(const Kv8Cache& c, const Kv8Batch& b, uint32_t heads, uint32_t type, int sms) {
     Shape r;
     r.group = heads / c.kv_heads;
+    const int terms = type == GGML_F32 ? 2 : 1;
     const uint64_t rows = (uint64_t)std::max(1u, b.max_new) * r.group;
-    r.tiles = rows >= kTileMin;
-    const Role role = role_of((int)c.head_dim, type == GGML_F32 ? 2 : 1);
+    const uint32_t blocks = std::max(1u, (b.max_len + 15) / 16);
+    r.tiles = rows >= tile_min((int)c.head_dim, terms) &&
+              (double)b.n_seqs * c.kv_heads * blocks * ((rows + kRows - 1) / kRows) >= (double)kTileWork * 3 * kWarps * sms;
+    const Role role = role_of((int)c.head_dim, terms);
     r.tile_rows = r.tiles ? role.rt * kTileRows : kRows;
     r.row_tiles = (uint32_t)((rows + r.tile_rows - 1) / r.tile_rows);
-    const uint32_t blocks = std::max(1u, (b.max_len + 15) / 16);
     // chunks of positions: enough CTAs for three on every SM (the prompt kernel: one; one row tile of 256
     // dims: two, as many as run at once -- 32768 positions over 4 kv heads 25 us against 34 with three;
     // several row tiles read the same pages, and three measured better: 29 against 37), each with at
-    // least 8 blocks (two per warp; the prompt kernel: 32, eight steps). More chunks measured slower: a
+    // least 8 blocks (two per warp, two steps of the prompt kernel). More chunks measured slower: a
     // CTA's fixed cost is about 4 us.
     const uint64_t tiles = (uint64_t)b.n_seqs * c.kv_heads * r.row_tiles;
     const uint64_t want = std::max<uint64_t>(1, (r.tiles ? 1ull : c.head_dim == 256 && r.row_tiles == 1 ? 2ull : 3ull) * sms / std::max<uint64_t>(1, tiles));
-    r.chunk = std::max(r.tiles ? 32u : 8u, (uint32_t)((blocks + want - 1) / want));
+    r.chunk = std::max(8u, (uint32_t)((blocks + want - 1) / want));
     r.chunk = (r.chunk + 3) / 4 * 4;
     r.splits = (blocks + r.chunk - 1) / r.chunk;
     r.slots = tiles * r.splits;

@@ -156,6 +156,24 @@ def test_matmul_residual_in_place_and_tall():
 
 
 # ------------------------------------------------------------------ the cache
+# Sequences without positions or tokens that every batch gets besides, so that its size lets few
+# rows take the prompt kernel too.
+_EMPTY = [0]
+
+
+@pytest.fixture(params=[0, 1800], ids=["alone", "wide"])
+def width(request):
+    _EMPTY[0] = request.param
+    yield
+    _EMPTY[0] = 0
+
+
+def _with_empty(table, cu, lens):
+    n = _EMPTY[0]
+    return (np.concatenate([table, np.full((n, table.shape[1]), -5, np.int32)]),
+            np.concatenate([cu, np.full(n, cu[-1], np.int32)]), np.concatenate([lens, np.zeros(n, np.int32)]))
+
+
 class Kv:
     """A cache with its host mirror, and sequences of given lengths in scattered pages."""
 
@@ -182,7 +200,8 @@ class Kv:
 
     def batch(self, lens, new, slack=0):
         cu = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
-        return int8.Kv8Batch(dev(self.table), dev(cu), dev(np.asarray(lens, np.int32)), max(1, max(new)) + slack,
+        table, cu, at = _with_empty(self.table, cu, np.asarray(lens, np.int32))
+        return int8.Kv8Batch(dev(table), dev(cu), dev(at), max(1, max(new)) + slack,
                              max(lens) + min(slack, self.table.shape[1] * self.k.shape[2] - max(lens)))
 
     def same(self):
@@ -318,6 +337,7 @@ def _check(kv, lens, new, q, out, kind, scale=None):
     return at
 
 
+@pytest.mark.usefixtures("width")
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("dim,page", [(64, 16), (128, 32), (256, 64)])
 @pytest.mark.parametrize("heads,hk", [(1, 1), (6, 2), (8, 1), (20, 1), (4, 4)])
@@ -331,6 +351,7 @@ def test_attention_tokens(kind, dim, page, heads, hk, lens, new):
     assert np.all(host(out)[n:] == 7.0) and int(kv.err) == 0
 
 
+@pytest.mark.usefixtures("width")
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("dim,page", [(64, 32), (128, 16), (256, 32)])
 @pytest.mark.parametrize("heads,hk,lens,new", [(4, 2, [5], [5]), (2, 2, [40, 33, 300], [3, 33, 2]), (8, 1, [200], [70]),
@@ -344,6 +365,7 @@ def test_attention_many_tokens(kind, dim, page, heads, hk, lens, new):
     assert int(kv.err) == 0
 
 
+@pytest.mark.usefixtures("width")
 @pytest.mark.parametrize("lens,new", [([20001, 9], [1, 1]), ([2100, 70], [50, 64])])
 @pytest.mark.parametrize("scale", [0.3, -0.2])
 def test_attention_long_and_scaled(lens, new, scale):
@@ -353,6 +375,20 @@ def test_attention_long_and_scaled(lens, new, scale):
     _check(kv, lens, new, q, _attend(kv, lens, new, q, "f32", scale=scale), "f32", scale=np.float32(scale))
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("heads,new", [(8, [30, 4]), (16, [40, 1])])
+def test_attention_drafts_over_many_positions(kind, dim, heads, new):
+    """Positions split over CTAs of the prompt kernel, one row tile and two."""
+    rng = np.random.default_rng(dim + heads)
+    lens = [3001, 500]
+    kv = Kv(rng, 2, dim, 32, lens)
+    q = dev(rng.standard_normal((sum(new), heads, dim)).astype(np.float32) * 2, kind)
+    _check(kv, lens, new, q, _attend(kv, lens, new, q, kind), kind)
+    assert int(kv.err) == 0
+
+
+@pytest.mark.usefixtures("width")
 def test_attention_strided_views():
     """q and out inside larger rows, pages inside a pool that holds other layers."""
     t = gu.torch()
@@ -370,6 +406,7 @@ def test_attention_strided_views():
     assert not host(out[:, :4]).any() and not host(out[:, 8:]).any()
 
 
+@pytest.mark.usefixtures("width")
 @pytest.mark.parametrize("kind", ["f32", "f16"])
 @pytest.mark.parametrize("new", [4, 13])
 def test_attention_scales_of_any_size(kind, new):
@@ -388,6 +425,7 @@ def test_attention_scales_of_any_size(kind, new):
         _check(kv, [n], [new], q, _attend(kv, [n], [new], q, kind), kind)
 
 
+@pytest.mark.usefixtures("width")
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
 @pytest.mark.parametrize("n", [40, 90])
 def test_attention_ignores_what_it_does_not_see(kind, n):
@@ -414,6 +452,7 @@ def test_attention_ignores_what_it_does_not_see(kind, n):
         assert np.isnan(got[see:, 0]).all() and np.isfinite(got[:see]).all() and np.isfinite(got[:, 1]).all()
 
 
+@pytest.mark.usefixtures("width")
 @pytest.mark.parametrize("n", [3, 30])
 def test_attention_queries_that_are_not_finite(n):
     rng = np.random.default_rng(13)
@@ -431,6 +470,7 @@ def test_attention_queries_that_are_not_finite(n):
     assert same(got[fine], want[fine])
 
 
+@pytest.mark.usefixtures("width")
 @pytest.mark.parametrize("many", [False, True])
 def test_attention_skips_what_is_out_of_range(many):
     """(many: max_new large enough for the prompt kernel)"""
@@ -439,10 +479,11 @@ def test_attention_skips_what_is_out_of_range(many):
     kv.table[1, 2] = kv.k.shape[0] + 7
     t = gu.torch()
     q = dev(rng.standard_normal((3, 2, 64)).astype(np.float32))
-    b = int8.Kv8Batch(dev(kv.table), dev(np.arange(4, dtype=np.int32)), dev(np.array([64, 64, 65], np.int32)), 1, 64)
+    lists = _with_empty(kv.table, np.arange(4, dtype=np.int32), np.array([64, 64, 65], np.int32))
+    b = int8.Kv8Batch(*map(dev, lists), 1, 64)
     if many:  # three sequences of one token in a launch for up to 60
         q = dev(rng.standard_normal((60, 2, 64)).astype(np.float32))
-        b = int8.Kv8Batch(dev(kv.table), dev(np.arange(4, dtype=np.int32)), dev(np.array([64, 64, 65], np.int32)), 60, 64)
+        b = int8.Kv8Batch(*map(dev, lists), 60, 64)
     out = t.full(q.shape, 7.0, device="cuda:0")
     ws = t.empty(int8.kv8_attention_workspace(kv.cache, b, q) + 256, dtype=t.uint8, device="cuda:0")
     int8.kv8_attention(kv.cache, b, q, out, workspace=ws, err=kv.err)
@@ -513,6 +554,7 @@ class Layer:
         assert int(kv.err) == 0
 
 
+@pytest.mark.usefixtures("width")
 def test_layer_prompt_then_steps():
     """A ragged prompt, then decode steps, through all operators, every stage checked."""
     t = gu.torch()
@@ -530,6 +572,7 @@ def test_layer_prompt_then_steps():
         lens = [n + m for n, m in zip(lens, new)]
 
 
+@pytest.mark.usefixtures("width")
 def test_layer_captured_and_replayed_on_another_stream():
     """One decode step captured into a graph; the lengths, the tokens and the pages' contents move
     on between replays through the same buffers."""
@@ -576,6 +619,7 @@ def test_outputs_do_not_depend_on_the_batch_they_run_in():
         assert np.array_equal(host(getattr(whole, d))[rows], host(getattr(parts, d))[rows])
 
 
+@pytest.mark.usefixtures("width")
 def test_calls_on_several_streams_at_once():
     """Prompts of few steps on four streams, each with its own output and workspace: nothing waits in vain
     for a product that has already ended, and the results are those of a call alone."""
