@@ -25,9 +25,15 @@
 //      permutes; the weights move to the other operand's layout by two 8x8 transposes.
 //   The maximum is raised only when a score passes it by 2^8, so most blocks cost one vote.
 // A warp takes every 4th block of the CTA's chunk of positions, the next blocks already on their way
-// into a ring of its own (asynchronous copies, each lane its own pieces: no barrier, no registers). The warps' partials meet in shared memory; a sequence of more than one
-// chunk leaves (O, M, l) in the workspace for kv8_join_kernel.
-// Bound: HBM, (2 head_dim + 1/2) bytes per position and kv head.
+// into a ring of its own (asynchronous copies, each lane its own pieces: no barrier, no registers). The
+// warps' partials meet in shared memory; a sequence of more than one chunk leaves (O, M, l) in the workspace for
+// kv8_join_kernel.
+// Bound: HBM, (2 head_dim + 1/2) bytes per position and kv head. Measured (32 heads, 8 kv heads of 128 dims):
+// 131071 positions of one sequence, f32, 65 us = 4.1 TB/s, 62 % of a copy's rate; 32 sequences of up to
+// 2100, bf16, 33 us = 3.1 TB/s; 517 positions 8.1 us. What holds it: about 370 instructions a block and
+// warp, a quarter of them V's widening, issued by three warps a scheduler (issue 46 % busy, all waiting
+// in turn on the ring, the products and the exponentials), and about 4 us from a CTA's start to its first
+// product and from its last one to the join.
 #include <algorithm>
 #include <atomic>
 
@@ -516,24 +522,33 @@ template <class T, int HD> __global__ void __launch_bounds__(32 * kJoinWarps) kv
 // ------------------------------------------------------------------ prompts
 // kv8_tile_kernel: many rows per kv head, on the 5th-generation tensor cores. A CTA takes RT row
 // tiles of 128 rows (token, head) of one (sequence, kv head) and walks the positions NP at a time:
-//   1 factor warp     the blocks' scales, and what follows from them, into a small ring;
+//   1 block warp      a lane per block looks its page up, copies its codes into a ring (one run of memory for
+//                     K and one for V: two bulk copies) and makes the factors of its scales;
 //   4 producer warps  codes to f16 (exact) into a ring of shared-memory stages, K and V alike:
 //                     64 dims x NP positions per 128-byte-swizzled panel. The score product reads
 //                     them K-major, the value product MN-major, so no transpose is made;
-//   1 MMA thread      S = q K^T into tensor memory (two buffers per row tile, so the next scores
-//                     are multiplied while this step's softmax runs), O += P V with P read
-//                     from tensor memory;
+//   RT MMA threads    one per row tile: S = q K^T into tensor memory (two to four buffers per row
+//                     tile, so the next scores are multiplied while this step's softmax runs),
+//                     O += P V with P read from tensor memory;
 //   4 softmax warps   per row tile, one row per thread: scores to registers, running maximum,
 //                     weights to f16 over the scores' own columns. O is rescaled (read, multiplied,
 //                     written back) only when a score passes the row's maximum by 2^8.
-// 16-bit inputs (TERMS = 1): q is scaled by a power of two per row and held in one f16 part, exactly;
-// the weights are one f16 part. f32 inputs (TERMS = 2): q is fixed point in three 8-bit limbs and the
+// 16-bit inputs (TERMS = 1): q is scaled by a power of two per row and held in one f16 part, exactly
+// down to 2^-24 of the row's largest; the weights are one f16 part. f32 inputs (TERMS = 2): q is fixed point in three 8-bit limbs and the
 // scores are integer products (kind::i8) of the codes as they are, summed exactly -- the f32 sums of
 // kind::f16 are cut off, not rounded, and over long sums that shows; the weights are two f16 parts
 // with a product each. The block scales enter as
 // in the kernel above; the value scale as an added log2 where one rounding of the weights follows
 // anyway (TERMS = 1).
-// Bound: the exponentials (16 a clock and SM) and the tensor pipe, about equally.
+// Bound: the tensor pipe and, close behind, shared memory: a step of 64 positions with two row tiles of 128 dims
+// is 1024 clocks of products, 1540 of shared-memory traffic (q is read again for every K panel, and
+// the codes pass it three times) and 1024 of exponentials on each scheduler. Measured (2048 tokens behind
+// 6144 positions, 32 heads, 8 kv heads of 128 dims, bf16): 300 us = 800 TFLOP/s, half of the bf16 rate; about
+// 2100 clocks a step, of which a softmax warp takes 1550 for its 64 columns; and 256 CTAs on 148 SMs
+// take two turns where 1.73 would do. 64 rows over 4099 positions of 8 sequences, 8 kv heads: 49 us.
+// Tried and slower: 128 positions a step with one score buffer (432 us, the chain of a tile's products and softmax
+// lies open), codes kept in registers instead of a ring (354), the store's end waited for one
+// step late (293 here, but 54 against 48 with one row tile), polynomials for some exponentials.
 constexpr uint32_t kTileRows = 128;
 // Rows per (sequence, kv head) from which it may be used, and the blocks of 16 positions times tiles of eight rows
 // that each warp of the other kernel would then have to take. Measured over 64 to 256 dims, 16 to 64
