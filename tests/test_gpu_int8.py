@@ -642,6 +642,69 @@ def test_calls_on_several_streams_at_once():
     assert all(same(host(o), want) for o in outs)
 
 
+@pytest.mark.usefixtures("width")
+def test_cache_offsets_past_32_bits():
+    """The same sequences in a small cache and at the end of one of 4.6 GB for K and for V: append and attention
+    give the same bits."""
+    t = gu.torch()
+    rng = np.random.default_rng(16)
+    lens, new, pages = [100, 70], [40, 1], 70000
+    kv = Kv(rng, 8, 128, 64, lens, spare=0)
+    n = kv.k.shape[0]
+    big = [t.empty((pages, 8, 64, 128), dtype=t.int8, device="cuda:0") for _ in range(2)]
+    bigs = [t.empty((pages, 8, 4), device="cuda:0") for _ in range(2)]
+    for a, b in zip(big + bigs, (kv.dk, kv.dv, kv.dks, kv.dvs)):
+        a[pages - n:] = b
+    total = sum(new)
+    k, v, q = (dev(rng.standard_normal((total, h, 128)).astype(np.float32), "bf16") for h in (8, 8, 16))
+    got = []
+    for cache, shift in ((kv.cache, 0), (int8.Kv8Cache(*big, *bigs), pages - n)):
+        table, cu, at = _with_empty(kv.table + shift, np.array([0, 40, 41], np.int32), np.array(lens, np.int32))
+        b = int8.Kv8Batch(dev(table), dev(cu), dev(at), 40, 100)
+        int8.kv8_append(cache, b, k, v, err=kv.err)
+        out = t.zeros_like(q)
+        ws = t.empty(int8.kv8_attention_workspace(cache, b, q) + 1, dtype=t.uint8, device="cuda:0")
+        int8.kv8_attention(cache, b, q, out, workspace=ws, err=kv.err)
+        got.append(host(out))
+    assert int(kv.err) == 0 and same(got[0], got[1])
+    for a, b in zip(big + bigs, (kv.dk, kv.dv, kv.dks, kv.dvs)):
+        assert same(host(a[pages - n:]), host(b))
+
+
+def test_rows_more_than_32_bits_apart():
+    t = gu.torch()
+    rng = np.random.default_rng(17)
+    far = (1 << 32) + 64
+    pool = t.empty(2 * far + 4096, dtype=t.int8, device="cuda:0")
+    x = rng.standard_normal((3, 300)).astype(np.float32)
+    dx = t.as_strided(pool.view(t.float32), (3, 300), (far // 4, 1))
+    codes = t.as_strided(pool, (3, 300), (far, 1), 2048)
+    y = t.as_strided(pool.view(t.float32), (3, 20), (far // 4, 1), 800)
+    dx.copy_(dev(x))
+    scales = t.empty(3, device="cuda:0")
+    int8.quantize_rows(dx, codes, scales)
+    want, ws = ref.quantize_rows(x)
+    assert same(host(codes.contiguous()), want) and same(host(scales), ws)
+    w, s = _codes(rng, 20, 300), rng.uniform(0.5, 1, 20).astype(np.float32)
+    int8.matmul(codes, scales, _wide(w), dev(s), y)
+    z = t.empty((3, 20), device="cuda:0")
+    int8.matmul(_wide(want), dev(ws), _wide(w), dev(s), z)
+    assert same(host(y.contiguous()), host(z))
+
+
+@pytest.mark.usefixtures("width")
+def test_attention_shared_pages():
+    """Sequences that share a prefix's pages, and a page that stands twice in one sequence."""
+    rng = np.random.default_rng(18)
+    kv = Kv(rng, 2, 64, 16, [90, 90, 90])
+    kv.table[1, :3] = kv.table[0, :3]
+    kv.table[2, 4] = kv.table[2, 1]
+    lens, new = [90, 75, 90], [1, 20, 30]
+    q = dev(rng.standard_normal((51, 4, 64)).astype(np.float32))
+    _check(kv, lens, new, q, _attend(kv, lens, new, q, "f32"), "f32")
+    assert int(kv.err) == 0
+
+
 def test_calls_of_no_tokens():
     t = gu.torch()
     kv = Kv(np.random.default_rng(2), 1, 64, 16, [16])
