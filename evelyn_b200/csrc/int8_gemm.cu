@@ -221,6 +221,8 @@ __global__ void __launch_bounds__(gemm_threads(NT), 1) i8_gemm_kernel(const __gr
     __syncthreads();
     tc_after();
     const uint32_t tm = tmem_base;
+    pdl_wait();
+    pdl_launch_dependents();
 
     if (warp == 0) {
         if (lane == 0) {
@@ -417,6 +419,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) i8_gemm_pair_kernel(const __g
     cl.sync();  // barriers of both CTAs are there
     tc_after();
     const uint32_t tm = tmem_base;
+    pdl_wait();
+    pdl_launch_dependents();
 
     if (warp == 0) {
         if (elect_one()) {
@@ -536,7 +540,7 @@ template <auto kernel> cudaError_t opt_in(uint32_t smem) {
     return e;
 }
 
-// grid and shared memory of a launch in clusters of `cluster` CTAs
+// a launch in clusters of `cluster` CTAs that may begin while the kernel before it ends
 template <auto kernel> cudaError_t go(const Plan& p, uint32_t grid, uint32_t threads, uint32_t smem, uint32_t cluster, cudaStream_t s) {
     cudaError_t e = opt_in<kernel>(kSmemCap + 1024);
     if (e != cudaSuccess) return e;
@@ -545,12 +549,14 @@ template <auto kernel> cudaError_t go(const Plan& p, uint32_t grid, uint32_t thr
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
-    cudaLaunchAttribute at[1];
+    cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = cluster;
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 

@@ -46,6 +46,8 @@ template <class T> __device__ __forceinline__ void widen(const Chunk<T>& c, floa
 }
 template <class T, int C> __global__ void __launch_bounds__(1024) quantize_rows_kernel(const QuantRowsArgs a) {
     __shared__ uint32_t red[32];
+    pdl_wait();
+    pdl_launch_dependents();
     const uint64_t row = blockIdx.x;
     const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
     int8_t* codes = a.codes + row * a.code_stride;
@@ -102,6 +104,8 @@ template <class T, int C> __global__ void __launch_bounds__(1024) quantize_rows_
 template <class T> __global__ void __launch_bounds__(512) quantize_rows_staged_kernel(const QuantRowsArgs a) {
     extern __shared__ __align__(16) uint8_t row_smem[];
     __shared__ uint32_t red[32];
+    pdl_wait();
+    pdl_launch_dependents();
     constexpr uint32_t ES = sizeof(T), NW = kChunk * ES / 4;  // words of a chunk
     const uint64_t row = blockIdx.x;
     const uint8_t* x = reinterpret_cast<const uint8_t*>(static_cast<const T*>(a.x) + row * a.x_stride);
@@ -187,6 +191,8 @@ template <class T> __global__ void __launch_bounds__(512) quantize_rows_staged_k
 // the row read a second time from L2.
 template <class T> __global__ void __launch_bounds__(512) quantize_rows_long_kernel(const QuantRowsArgs a) {
     __shared__ uint32_t red[32];
+    pdl_wait();
+    pdl_launch_dependents();
     const uint64_t row = blockIdx.x;
     const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
     int8_t* codes = a.codes + row * a.code_stride;
@@ -225,21 +231,17 @@ template <class T> cudaError_t launch(const QuantRowsArgs& a, int sms, cudaStrea
         const uint64_t smem = staged_bytes((uint64_t)a.cols * sizeof(T));
         const uint32_t nt = a.cols >= 8192 ? 512 : a.cols >= 1024 ? 256 : 64;
         if (smem > kStagedCap) {
-            quantize_rows_long_kernel<T><<<a.rows, 512, 0, s>>>(a);
-        } else {
-            if (const cudaError_t e = opt_in<quantize_rows_staged_kernel<T>>(kStagedCap)) return e;
-            quantize_rows_staged_kernel<T><<<a.rows, nt, (uint32_t)smem, s>>>(a);
+            return launch_chained(quantize_rows_long_kernel<T>, a.rows, 512, 0, s, a);
         }
-        return cudaGetLastError();
+        if (const cudaError_t e = opt_in<quantize_rows_staged_kernel<T>>(kStagedCap)) return e;
+        return launch_chained(quantize_rows_staged_kernel<T>, a.rows, nt, (uint32_t)smem, s, a);
     }
     // few rows: as many threads as chunks, so that a row is one load deep; many rows: four
     // chunks per thread, all in flight, and more rows on each SM
     const int C = (a.rows <= (uint32_t)(2 * sms) && chunks <= 1024) ? 1 : chunks > 2048 || a.rows > (uint32_t)(2 * sms) ? 4 : 2;
     const uint32_t nt = ((chunks + C - 1) / C + 31) / 32 * 32;
-    if (C == 1) quantize_rows_kernel<T, 1><<<a.rows, nt, 0, s>>>(a);
-    else if (C == 2) quantize_rows_kernel<T, 2><<<a.rows, nt, 0, s>>>(a);
-    else quantize_rows_kernel<T, 4><<<a.rows, nt, 0, s>>>(a);
-    return cudaGetLastError();
+    return launch_chained(C == 1 ? quantize_rows_kernel<T, 1> : C == 2 ? quantize_rows_kernel<T, 2> : quantize_rows_kernel<T, 4>,
+                          a.rows, nt, 0, s, a);
 }
 
 }  // namespace

@@ -360,6 +360,9 @@ __global__ void __launch_bounds__(32 * kWarps, 3) kv8_append_kernel(const __grid
     uint32_t turn_no = 0;  // (two sets of maxima, so that one barrier per block is enough)
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const Kv8AppendArgs& a = p.a;
+    pdl_wait();
+    // (no pdl_launch_dependents: the attention's CTAs would take their places while these run, three beside one
+    // another where there is room first -- a layer's step of 32 sequences 76 us against 64)
     if (blockIdx.x >= p.kv_ctas) {
         const uint32_t item = (blockIdx.x - p.kv_ctas) * kWarps + warp;
         if (item >= p.q_items) return;
@@ -424,8 +427,7 @@ __global__ void __launch_bounds__(32 * kWarps, 3) kv8_append_kernel(const __grid
 }
 
 template <class T, int HD, bool FOUR> cudaError_t launch(const Plan& p, cudaStream_t s) {
-    kv8_append_kernel<T, HD, FOUR><<<p.kv_ctas + (p.q_items + kWarps - 1) / kWarps, 32 * kWarps, 0, s>>>(p);
-    return cudaGetLastError();
+    return launch_chained(kv8_append_kernel<T, HD, FOUR>, p.kv_ctas + (p.q_items + kWarps - 1) / kWarps, 32 * kWarps, 0, s, p);
 }
 template <class T, bool FOUR> cudaError_t by_dim(const Plan& p, cudaStream_t s) {
     return p.a.c.head_dim == 64    ? launch<T, 64, FOUR>(p, s)

@@ -211,6 +211,7 @@ __global__ void __launch_bounds__(32 * kWarps) kv8_split_kernel(const __grid_con
     const Kv8AttnArgs& a = P.a;
     const uint32_t split = blockIdx.x, h = blockIdx.y % a.c.kv_heads, tile = blockIdx.y / a.c.kv_heads, s = blockIdx.z;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    pdl_wait();
     const Span sp = span_of(a, s);
     if (!sp.ok) {
         if (tid == 0) flag_error(a.err, DEV_ERR_POSITION);
@@ -418,6 +419,9 @@ __global__ void __launch_bounds__(32 * kWarps) kv8_split_kernel(const __grid_con
         }
     }
     cp_async_wait<0>();
+    // (not at the start: 32 sequences of 2100 positions 42 us against 32, with the next kernel's CTAs waiting
+    // among this one's)
+    pdl_launch_dependents();
     if (bad_page && lane == 0) flag_error(a.err, DEV_ERR_POSITION);
 
     // ---- the warps' partials, over the rings
@@ -475,6 +479,8 @@ template <class T, int HD> __global__ void __launch_bounds__(32 * kJoinWarps) kv
     const Kv8AttnArgs& a = P.a;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, head = blockIdx.y, s = blockIdx.z;
     const int32_t i = (int32_t)blockIdx.x;
+    pdl_wait();
+    pdl_launch_dependents();
     const Span sp = span_of(a, s);
     if (!sp.ok || i >= sp.n_new) return;
     const uint32_t h = head / P.group, row = (uint32_t)i * P.group + head % P.group, tile = row / P.tile_rows;
@@ -742,6 +748,7 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     // the last row tiles see the most positions: they go first
     const uint32_t tile = P.row_tiles - 1 - blockIdx.x / P.splits, split = blockIdx.x % P.splits, h = blockIdx.y, s = blockIdx.z;
+    pdl_wait();
     const Span sp = span_of(a, s);
     if (!sp.ok) {
         if (tid == 0) flag_error(a.err, DEV_ERR_POSITION);
@@ -801,6 +808,7 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
     __syncthreads();
     tc_after();
     const uint32_t tm = tmem_base;
+    pdl_launch_dependents();  // (not before: a kernel that began meanwhile could hold the tensor memory)
 
     if (warp < 4 * used) {
         // ---------------------------------------------------------------- softmax: one row per thread
@@ -1288,16 +1296,17 @@ template <class T, int HD> cudaError_t launch(const Plan& p, bool tiles, cudaStr
         constexpr uint32_t smem = tile_smem(HD, terms), threads = 32 * (5 * role_of(HD, terms).rt + 5);
         cudaError_t e = opt_in<kv8_tile_kernel<T, HD>>(smem);
         if (e != cudaSuccess) return e;
-        kv8_tile_kernel<T, HD><<<dim3(p.row_tiles * p.splits, p.a.c.kv_heads, p.a.b.n_seqs), threads, smem, s>>>(p);
+        e = launch_chained(kv8_tile_kernel<T, HD>, dim3(p.row_tiles * p.splits, p.a.c.kv_heads, p.a.b.n_seqs), threads, smem, s, p);
+        if (e != cudaSuccess) return e;
     } else {
         cudaError_t e = opt_in<kv8_split_kernel<T, HD>>(split_smem(HD));
         if (e != cudaSuccess) return e;
-        kv8_split_kernel<T, HD>
-            <<<dim3(p.splits, p.row_tiles * p.a.c.kv_heads, p.a.b.n_seqs), 32 * kWarps, split_smem(HD), s>>>(p);
+        e = launch_chained(kv8_split_kernel<T, HD>, dim3(p.splits, p.row_tiles * p.a.c.kv_heads, p.a.b.n_seqs), 32 * kWarps,
+                           split_smem(HD), s, p);
+        if (e != cudaSuccess) return e;
     }
-    if (p.splits > 1)
-        kv8_join_kernel<T, HD><<<dim3(p.a.b.max_new, p.a.heads, p.a.b.n_seqs), 32 * kJoinWarps, 0, s>>>(p);
-    return cudaGetLastError();
+    if (p.splits == 1) return cudaSuccess;
+    return launch_chained(kv8_join_kernel<T, HD>, dim3(p.a.b.max_new, p.a.heads, p.a.b.n_seqs), 32 * kJoinWarps, 0, s, p);
 }
 template <class T> cudaError_t by_dim(const Plan& p, bool tiles, cudaStream_t s) {
     return p.a.c.head_dim == 64    ? launch<T, 64>(p, tiles, s)
