@@ -25,8 +25,8 @@
 // waits for a cluster that waits for it.
 //
 // Bound: few tokens -- HBM, every weight byte once; many tokens -- the tensor pipe. Measured:
-//   1 token, 6144 x 4096, f32 out           8.6 us   2.9 TB/s (a launch, one ring's fill and a cluster's exchange)
-//   33 tokens, 5120 x 25600, bf16, added     30 us   4.5 TB/s (68 % of a copy's rate)
+//   1 token, 6144 x 4096, f32 out           7.6 us   3.3 TB/s (a launch, one ring's fill and a cluster's exchange)
+//   33 tokens, 5120 x 25600, bf16, added     28 us   4.7 TB/s (71 % of a copy's rate)
 //   4096 tokens, 24576 x 4096, bf16         282 us   2920 TOP/s (tensor pipe busy 78 % of the cycles; 535 us with
 //                                                    128 x 256 tiles on single CTAs)
 // Every wait is bounded; on a timeout the CTA records DEV_ERR_WAIT_TIMEOUT, lets its copies and

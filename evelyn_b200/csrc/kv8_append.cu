@@ -16,7 +16,7 @@
 // tokens in turn. Bound: HBM (each new value read once, one byte written). Measured: four
 // prompts of 5003 tokens, 16 heads and 4 kv heads of 256 dims, 94 us = 3.6 TB/s, 55 % of a copy's rate (the norm's
 // 64-bit sums and the rotation keep issue 60 % busy at 24 warps an SM; 296 us with a warp per row of
-// the cache, 127 before the next head's rows were loaded ahead); 32 tokens of a decode step 4.2 us,
+// the cache, 127 before the next head's rows were loaded ahead); 32 tokens of a decode step 3.8 us,
 // a launch and one chain of dependent loads.
 //
 // Norm: the sum of squares and its root are computed in 64 bits and rounded once, then x * r * w

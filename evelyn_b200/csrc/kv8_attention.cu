@@ -30,7 +30,7 @@
 // kv8_join_kernel.
 // Bound: HBM, (2 head_dim + 1/2) bytes per position and kv head. Measured (32 heads, 8 kv heads of 128 dims):
 // 131071 positions of one sequence, f32, 65 us = 4.1 TB/s, 62 % of a copy's rate; 32 sequences of up to
-// 2100, bf16, 33 us = 3.1 TB/s; 517 positions 8.1 us. What holds it: about 370 instructions a block and
+// 2100, bf16, 32 us = 3.2 TB/s; 517 positions 7.4 us. What holds it: about 370 instructions a block and
 // warp, a quarter of them V's widening, issued by three warps a scheduler (issue 46 % busy, all waiting
 // in turn on the ring, the products and the exponentials), and about 4 us from a CTA's start to its first
 // product and from its last one to the join.
@@ -549,7 +549,7 @@ template <class T, int HD> __global__ void __launch_bounds__(32 * kJoinWarps) kv
 // Bound: the tensor pipe and, close behind, shared memory: a step of 64 positions with two row tiles of 128 dims
 // is 1024 clocks of products, 1540 of shared-memory traffic (q is read again for every K panel, and
 // the codes pass it three times) and 1024 of exponentials on each scheduler. Measured (2048 tokens behind
-// 6144 positions, 32 heads, 8 kv heads of 128 dims, bf16): 300 us = 800 TFLOP/s, half of the bf16 rate; about
+// 6144 positions, 32 heads, 8 kv heads of 128 dims, bf16): 297 us = 810 TFLOP/s, half of the bf16 rate; about
 // 2100 clocks a step, of which a softmax warp takes 1550 for its 64 columns; and 256 CTAs on 148 SMs
 // take two turns where 1.73 would do. 64 rows over 4099 positions of 8 sequences, 8 kv heads: 49 us.
 // Tried and slower: 128 positions a step with one score buffer (432 us, the chain of a tile's products and softmax
