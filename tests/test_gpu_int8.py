@@ -705,6 +705,46 @@ def test_attention_shared_pages():
     assert int(kv.err) == 0
 
 
+@pytest.mark.parametrize("captured", [False, True])
+def test_calls_see_what_the_stream_wrote_before(captured):
+    """Calls between other kernels of the stream that write their inputs, read their outputs and write those inputs
+    again: each sees its own round's values (launches begin early, their reads and writes do not)."""
+    t = gu.torch()
+    rng = np.random.default_rng(19)
+    base = dev(rng.integers(-5, 6, (64, 2048)).astype(np.float32))
+    w, s = dev(_codes(rng, 512, 2048)), t.ones(512, device="cuda:0")
+    x, y, acc = t.empty_like(base), t.empty((64, 512), device="cuda:0"), t.zeros((64, 512), device="cuda:0")
+    codes, scales = t.empty((64, 2048), dtype=t.int8, device="cuda:0"), t.empty(64, device="cuda:0")
+    n = 24
+
+    def rounds(stream):
+        for i in range(n):
+            t.mul(base, float(1 + i % 5), out=x)
+            int8.quantize_rows(x, codes, scales, stream=stream)
+            int8.matmul(codes, scales, w, s, y, stream=stream)
+            acc.add_(y)
+
+    stream = t.cuda.Stream()
+    if captured:
+        rounds(0)  # (kernels loaded before the capture)
+        t.cuda.synchronize()
+        g = t.cuda.CUDAGraph()
+        with t.cuda.graph(g, stream=stream):
+            rounds(stream.cuda_stream)
+        acc.zero_()
+        g.replay()
+    else:
+        with t.cuda.stream(stream):
+            rounds(stream.cuda_stream)
+    t.cuda.synchronize()
+    want = t.zeros_like(acc)
+    for i in range(n):
+        c, z = ref.quantize_rows(host(base) * np.float32(1 + i % 5))
+        p = c.astype(np.int64) @ host(w).astype(np.int64).T
+        want += dev((p.astype(np.float32) * z[:, None]).astype(np.float32))
+    assert same(host(acc), host(want))
+
+
 def test_calls_of_no_tokens():
     t = gu.torch()
     kv = Kv(np.random.default_rng(2), 1, 64, 16, [16])
