@@ -8,8 +8,8 @@
 //   x = q . ck (an integer) * (sk * scale * log2 e * step of q) + e,  e = exponent of sv
 //   w = 2^(x - M),  l += w * 2^-e,  O += (w * sv 2^-e) * cv,  o = O / l
 // so w times a mantissa in [1, 2) meets the codes, whatever the size of the value scale, and
-// the power of two leaves the sum exactly. Where e is far below M (value scales that differ by more
-// than 2^80) w would leave f32's range while the sum still needs it: such a block's weights
+// the power of two leaves the sum exactly. Where a block's x are far below M and so is e (value scales that
+// differ by more than 2^80) w would leave f32's range while the sum still needs it: such a block's weights
 // are kept 2^d larger, and 2^-d joins the mantissa and the power of two (aside()).
 //
 // Small-batch kernel (kv8_split_kernel): up to 8 rows (token, head) per CTA that share a kv head;
@@ -87,12 +87,9 @@ __device__ __forceinline__ float rebase(float l, float from, float to) {
 }
 constexpr float kFar = 80.f;
 constexpr float kZeroExp = -100.f, kZeroDown = 1.2676506002282294e30f;  // 2^100
-// d >= 0 and 2^-d for a block of exponent e under the maximum M
-__device__ __forceinline__ float aside(float e, float M, float& f) {
-    const float d = fmaxf(0.f, M - kFar - e);
-    f = exp2_fast(-d);
-    return d;
-}
+// d >= 0 for a block of exponent e whose largest x is `most`, under the maximum M. (M - e alone is no measure: where
+// the scores themselves are large it is large for every block, the one that holds the maximum too.)
+__device__ __forceinline__ float aside(float e, float M, float most) { return fmaxf(0.f, fminf(M - kFar - e, M - most)); }
 // bytes 0, 1 (or 2, 3) of w, biased codes c + 128, as an exact f16 pair: 0x6400 | b is 1024 + b
 __device__ __forceinline__ uint32_t codes_h2(uint32_t w, uint32_t sel) {
     const uint32_t h = __byte_perm(w, 0x64646464u, sel), bias = 0x64806480u;  // 1024 + 128
@@ -370,12 +367,16 @@ __global__ void __launch_bounds__(32 * kWarps) kv8_split_kernel(const __grid_con
                 }
             }
             float off[2] = {M[0], M[1]}, mt[2] = {mant, mant}, dn[2] = {down, down};
-            if (e < fmaxf(M[0], M[1]) - kFar) {  // (rare)
+            if (__any_sync(0xffffffffu, e < fmaxf(M[0], M[1]) - kFar)) {  // (rare)
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    float f;
-                    off[j] -= aside(e, M[j], f);
-                    mt[j] *= f, dn[j] *= f;
+                    float m = fmaxf(x[j], x[j + 2]);
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+                    const float d = aside(e, M[j], m);
+                    off[j] -= d, mt[j] *= exp2_fast(-d);
+                    if (d > 0.f) dn[j] = exp2_fast(-e - d);  // (one exponent: either factor may leave the range)
                 }
             }
             float w[4];
@@ -969,14 +970,15 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
                     if (p0 + (int32_t)i > last) v[i] = 0xff800000u;  // -infinity
             }
             // the largest score: of each block's products, then by the block's factor (not negative)
-            float mx = -INFINITY;
+            float mx = -INFINITY, most[NB];
 #pragma unroll
             for (uint32_t b = 0; b < NB; ++b) {
                 float m = __uint_as_float(v[16 * b]);
 #pragma unroll
                 for (uint32_t i = 1; i < 16; ++i) m = fmaxf(m, __uint_as_float(v[16 * b + i]));
                 // (a hidden block and a factor of 0: 0 * -infinity is not a number)
-                mx = fmaxf(mx, m == -INFINITY ? m : fmaf(m, f[b], e[b]));
+                most[b] = m == -INFINITY ? m : fmaf(m, f[b], e[b]);
+                mx = fmaxf(mx, most[b]);
             }
             if (__any_sync(0xffffffffu, mx > M + kSlack)) {
                 const float m = fmaxf(M, mx), f8 = exp2_fast(M - m);
@@ -1008,9 +1010,9 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
                     uint32_t hi[8], lo[8];
                     float off = e[b] - M, mt = mant[b], dn = down[b];
                     if (RARE && off < -kFar && off != -INFINITY) {
-                        float f;
-                        off += aside(e[b], M, f);
-                        mt *= f, dn *= f;
+                        const float d = aside(e[b], M, most[b]);
+                        off += d, mt *= exp2_fast(-d);
+                        if (d > 0.f) dn = exp2_fast(-e[b] - d);
                     }
 #pragma unroll
                     for (uint32_t i = 0; i < 8; ++i) {

@@ -1,0 +1,108 @@
+"""Attention over the 8-bit cache where scores are far apart or large: heads whose weight lies almost
+whole on one position, scores of any size, and blocks that are not finite beside such positions. Both
+attention kernels, against float64 within bounds that have no term in the number of positions."""
+import numpy as np
+import pytest
+
+from evelyn_b200 import int8
+from tests import gpu_util as gu
+from tests import int8_util as ref
+from tests.test_gpu_int8 import KINDS, Kv, _attend, dev, host, width  # noqa: F401  (a fixture)
+
+pytestmark = pytest.mark.gpu
+
+# (tokens of a sequence: one takes the token kernel, 12 beside many empty sequences the prompt kernel)
+KERNELS = pytest.mark.parametrize("tokens", [1, 12])
+
+
+def _wide(tokens):
+    """Sequences without tokens besides, so that few rows take the prompt kernel."""
+    import tests.test_gpu_int8 as t
+    t._EMPTY[0] = 1800 if tokens > 1 else 0
+
+
+@pytest.fixture(autouse=True)
+def _alone():
+    yield
+    _wide(1)
+
+
+def _put(kv, codes_k, codes_v, ks, vs):
+    """One sequence's positions into the cache and its host mirror: codes [n][dim], scales [n / 16]."""
+    n, page = len(codes_k), kv.k.shape[2]
+    for p in range(-(-n // page)):
+        at, rows = kv.table[0][p], min(page, n - p * page)
+        kv.k[at, 0, :rows], kv.v[at, 0, :rows] = codes_k[p * page:p * page + rows], codes_v[p * page:p * page + rows]
+        for b in range(page // 16):
+            i = p * page // 16 + b
+            if i < len(ks):
+                kv.ks[at, 0, b], kv.vs[at, 0, b] = ks[i], vs[i]
+    for d, a in ((kv.dk, kv.k), (kv.dv, kv.v), (kv.dks, kv.ks), (kv.dvs, kv.vs)):
+        d.copy_(dev(a))
+
+
+def _bound(q, k, v, first, scale, kind):
+    """The attention and how far an implementation that holds its sums in f32 may be from it."""
+    q = q.astype(np.float64)
+    out, tol = np.zeros(q.shape), np.zeros(q.shape)
+    half = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}[kind]
+    for i in range(q.shape[0]):
+        n = max(0, first + i + 1)
+        for h in range(q.shape[1]):
+            x = k[:n] @ q[i, h] * scale
+            w = np.exp(x - x.max())
+            w /= w.sum()
+            out[i, h] = w @ v[:n]
+            # scores: q in fixed point (half a step of 2^-21 of the row's largest), or its f16 products summed in f32
+            # with a cut of at most 2^-23 of the terms' sizes after every 16 dims; seven roundings of the score
+            terms = (np.abs(k[:n]) @ np.abs(q[i, h])).max() * abs(scale)
+            dx = np.abs(q[i, h]).max() * 2.0 ** -22 * np.abs(k[:n]).sum(1).max() * abs(scale) + 7 * 2.0 ** -24 * np.abs(x).max()
+            if kind != "f32":
+                dx += (q.shape[2] / 16 + 1) * 2.0 ** -23 * terms
+            # weights: exp2 2^-22, the value scale 2^-22, and for the 16-bit types 16 bits (2^-15); sums of the
+            # tensor cores: cut off at most 2^-23 each, at most 128 in a row (f32) or 2048 (16 bits) before they are
+            # added rounded to nearest (unbiased: 2^-19 is four times what 30000 of them reach)
+            dw = 2.0 ** -21 + 2.0 ** -19 + (2.0 ** -16 if kind == "f32" else 2.0 ** -15 + 2.0 ** -12)
+            tol[i, h] = (2 * dx + dw) * (w @ np.abs(v[:n])) + 1e-30 + half * np.abs(out[i, h])
+            if kind == "f16":
+                tol[i, h] += 2.0 ** -25
+    return out, tol
+
+
+def _compare(kv, n, tokens, q, kind, scale=0.0):
+    got = host(_attend(kv, [n], [tokens], q, kind, scale=scale)).astype(np.float64)
+    k, v = (ref.values(a, b, kv.table[0], n)[:, 0] for a, b in ((kv.k, kv.ks), (kv.v, kv.vs)))
+    want, tol = _bound(host(q), k, v, n - tokens, scale or 1 / np.sqrt(q.shape[-1]), kind)
+    assert int(kv.err) == 0
+    assert np.isfinite(got).all()
+    off = np.abs(got - want) / tol
+    assert off.max() <= 1, (off.max(), np.abs(got - want).max(), np.abs(want).max())
+
+
+# ------------------------------------------------------------------ large scores
+@KERNELS
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("top", [40, 60, 140, 210, 300, 1e4])
+def test_attention_large_scores(tokens, kind, dim, zeros, top):
+    """Scores up to `top` (in nats), a few nats apart, under ordinary value scales, a block of zeros beside them, either
+    sign of the scale."""
+    _wide(tokens)
+    rng = np.random.default_rng(int(top) + dim)
+    n = 100
+    kv = Kv(rng, 1, dim, 16, [n])
+    sign = rng.choice([-1, 1], dim)
+    level = np.full(n, 100)
+    level[rng.permutation(n)[:20]] = 126
+    level[rng.permutation(n)[:8]] = 127
+    v = rng.integers(-127, 128, (n, dim))
+    vs = np.full(7, 1 / 40, np.float32)
+    if zeros:
+        v[32:48], vs[2] = 0, 0
+        level[40] = 127
+    _put(kv, level[:, None] * sign, v, np.full(7, 1 / 40, np.float32), vs)
+    for scale in (0.25, -0.25):
+        x = sign * (top / (127 / 40) / dim / scale)  # q . k of level 127 is `top`
+        q = dev(np.tile(x, (tokens, 4, 1)).astype(np.float32), kind)
+        _compare(kv, n, tokens, q, kind, scale=scale)
