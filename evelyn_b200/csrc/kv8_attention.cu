@@ -4,13 +4,15 @@
 // sees, with 8-bit codes c and one scale s per block of 16 positions and kv head. The scales are
 // constant over a block, so they leave the products: scores are integer products times one
 // factor per block, and the value scale joins the softmax weight. One pass over the cache with
-// a running maximum M and sum, all in the exponent's base 2:
-//   x = q . ck (an integer) * (sk * scale * log2 e * step of q) + e,  e = exponent of sv
-//   w = 2^(x - M),  l += w * 2^-e,  O += (w * sv 2^-e) * cv,  o = O / l
-// so w times a mantissa in [1, 2) meets the codes, whatever the size of the value scale, and
-// the power of two leaves the sum exactly. Where a block's x are far below M and so is e (value scales that
-// differ by more than 2^80) w would leave f32's range while the sum still needs it: such a block's weights
-// are kept 2^d larger, and 2^-d joins the mantissa and the power of two (aside()).
+// a running maximum M of the scores and their sum, in the exponent's base 2:
+//   x = q . ck (an integer) * (sk * scale * log2 e * step of q),
+//   w = 2^(x - M),  l += w,  O += (w * sv) * cv,  o = O / l
+// The codes meet w * sv in bf16 parts: codes of 8 bits are exact in bf16, and its exponents are f32's, so
+// a weight keeps its bits however far below the maximum it lies (a head that puts nearly all weight on
+// one position of value 0 is made of such weights; in f16 parts they were gone from 16 nats on). Three parts
+// hold an f32 product exactly (f32 outputs), two 16 bits of it, off by at most 2^-15 (16-bit outputs). Value
+// scales near the ends of f32's range (below 2^-60, above 2^80) move the maximum that their positions
+// ask for, so that their products stay inside (lift_of()).
 //
 // Small-batch kernel (kv8_split_kernel): up to 8 rows (token, head) per CTA that share a kv head;
 // positions are the M dimension of the warp's products.
@@ -19,10 +21,8 @@
 //      is as good as an f32 dot product. The K order inside the product is permuted so that a
 //      lane's fragment is 16 neighbouring bytes of a row: the codes reach the tensor cores as they
 //      were copied, with no conversion.
-//   V: mma.sync m16n8k16 in f16: codes are exact in f16, the weights two f16 parts (22 bits) for
-//      f32 outputs, one part for 16-bit outputs (half a step of 2^-11 each, as the prompt kernel).
-//      A lane loads 16 neighbouring dims of four positions and pairs positions with byte
-//      permutes; the weights move to the other operand's layout by two 8x8 transposes.
+//   V: mma.sync m16n8k16 in bf16. A lane loads 16 neighbouring dims of four positions and pairs
+//      positions with byte permutes; the weights move to the other operand's layout by 8x8 transposes.
 //   The maximum is raised only when a score passes it by 2^8, so most blocks cost one vote.
 // A warp takes every 4th block of the CTA's chunk of positions, the next blocks already on their way
 // into a ring of its own (asynchronous copies, each lane its own pieces: no barrier, no registers). The
@@ -45,7 +45,7 @@ namespace {
 constexpr uint32_t kRows = 8;     // rows of a tile (the product's N)
 constexpr uint32_t kWarps = 4;
 constexpr float kNegBig = -1e38f;  // a maximum that no score has reached
-constexpr float kSlack = 8.f;      // weights stay below 2^8 (times a mantissa below 2: far inside f16)
+constexpr float kSlack = 8.f;      // the maximum is raised when a score passes it by this: weights stay below 2^8
 
 struct Plan {
     Kv8AttnArgs a;
@@ -64,9 +64,9 @@ __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, ui
                  : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -80,21 +80,39 @@ __device__ __forceinline__ float exp2_fast(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// 2^from to 2^to for a sum of weights, in two steps: the ratio alone may leave f32's range
-__device__ __forceinline__ float rebase(float l, float from, float to) {
-    const float f = exp2_fast(0.5f * (from - to));
-    return (l * f) * f;
+// What the scores of a block are raised by where they ask for a new maximum: 0 for value scales from 2^-60 to 2^80 and
+// for scales that are 0 (or subnormal, which count as 0) or not finite.
+__device__ __forceinline__ float lift_of(float sv) {
+    const int e = (int)(__float_as_uint(sv) >> 23) - 127;
+    return e == -127 || e == 128 ? 0.f : (float)(max(e - 80, 0) + min(e + 60, 0));
 }
-constexpr float kFar = 80.f;
-constexpr float kZeroExp = -100.f, kZeroDown = 1.2676506002282294e30f;  // 2^100
-// d >= 0 for a block of exponent e whose largest x is `most`, under the maximum M. (M - e alone is no measure: where
-// the scores themselves are large it is large for every block, the one that holds the maximum too.)
-__device__ __forceinline__ float aside(float e, float M, float most) { return fmaxf(0.f, fminf(M - kFar - e, M - most)); }
+__device__ __forceinline__ float zero_if_subnormal(float sv) { return __float_as_uint(sv) < 0x00800000u ? 0.f : sv; }
 // bytes 0, 1 (or 2, 3) of w, biased codes c + 128, as an exact f16 pair: 0x6400 | b is 1024 + b
 __device__ __forceinline__ uint32_t codes_h2(uint32_t w, uint32_t sel) {
     const uint32_t h = __byte_perm(w, 0x64646464u, sel), bias = 0x64806480u;  // 1024 + 128
     const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&h), *reinterpret_cast<const __half2*>(&bias));
     return *reinterpret_cast<const uint32_t*>(&r);
+}
+// The same bytes of plain codes as an exact bf16 pair: 128 + the lower seven bits, less 128 or, for negative ones, 256.
+__device__ __forceinline__ uint32_t codes_b2(uint32_t w, uint32_t sel) {
+    const uint32_t t = __byte_perm(w, 0x43434343u, sel), a = t & 0xff7fff7fu, b = t & 0xff80ff80u;
+    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+// A pair of products as PARTS bf16 pairs: the upper half of each f32's bits, then those of what remains (exact
+// differences), the last of two parts rounded to nearest.
+template <int PARTS> __device__ __forceinline__ void split_b2(float a, float b, uint32_t (&part)[PARTS]) {
+#pragma unroll
+    for (int i = 0; i < PARTS; ++i) {
+        if (PARTS == 2 && i == 1) {
+            const __nv_bfloat162 r = __floats2bfloat162_rn(a, b);
+            part[i] = *reinterpret_cast<const uint32_t*>(&r);
+        } else {
+            const uint32_t x = __float_as_uint(a), y = __float_as_uint(b);
+            part[i] = __byte_perm(x, y, 0x7632);
+            if (i + 1 < PARTS) a -= __uint_as_float(x & 0xffff0000u), b -= __uint_as_float(y & 0xffff0000u);
+        }
+    }
 }
 __device__ __forceinline__ uint32_t pack_h2(float a, float b) {
     const __half2 r = __floats2half2_rn(a, b);
@@ -200,7 +218,7 @@ __global__ void __launch_bounds__(32 * kWarps) kv8_split_kernel(const __grid_con
     constexpr int VC = HD <= 128 ? 1 : 2;        // V loads per position
     constexpr int MT = HD / 16;                  // 16-dim tiles of the output
     constexpr int LD = HD / 8 < 16 ? HD / 8 : 16;  // neighbouring dims of a lane's load
-    constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;  // f16 parts of a weight
+    constexpr int PARTS = sizeof(T) == 4 ? 3 : 2;  // bf16 parts of a weight
     constexpr int D = ring_depth(HD);
     extern __shared__ __align__(16) uint8_t ring_smem[];
     __shared__ float2 sml[kWarps][kRows];
@@ -329,28 +347,22 @@ __global__ void __launch_bounds__(32 * kWarps) kv8_split_kernel(const __grid_con
                     for (int i = 0; i < 3; ++i)
                         mma_s8(acc[i], cur.k[c][0][2 * j], cur.k[c][1][2 * j], cur.k[c][0][2 * j + 1],
                                cur.k[c][1][2 * j + 1], qb[i][c][2 * j], qb[i][c][2 * j + 1]);
-            // value scale = mant * 2^e; 0 (a block of zeros) must not raise the maximum of rows that
-            // see other blocks: kZeroExp; a scale that is not finite reaches the output as it is
-            const uint32_t sb = __float_as_uint(cur.sv);
-            const int eb = (int)((sb >> 23) & 0xffu);
-            const bool plain = eb > 0 && eb < 255;
-            const float e = plain ? (float)(eb - 127) : eb ? 0.f : kZeroExp;
-            const float mant = plain ? __uint_as_float((sb & 0x807fffffu) | 0x3f800000u) : eb ? cur.sv : 0.f;
-            const float down = plain ? __uint_as_float((uint32_t)(254 - eb) << 23) : eb ? 1.f : kZeroDown;  // 2^-e
+            const float sv = zero_if_subnormal(cur.sv), lift = lift_of(sv);
             float x[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 // (the two lower limbs together stay below 2^30)
                 const float d = fmaf((float)acc[2][j], 65536.f, (float)(acc[1][j] * 256 + acc[0][j]));
-                x[j] = fmaf(d, step[j & 1] * cur.sk, e);
+                x[j] = d * (step[j & 1] * cur.sk);
             }
-            if (blk * 16 + 15 > first_last) {
+            const bool edge = blk * 16 + 15 > first_last;
+            if (edge) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     if (blk * 16 + (int32_t)g + (j >> 1) * 8 > last[j & 1]) x[j] = -INFINITY;
             }
             // ---- the running maximum
-            const bool up = fmaxf(x[0], x[2]) > M[0] + kSlack || fmaxf(x[1], x[3]) > M[1] + kSlack;
+            const bool up = fmaxf(x[0], x[2]) + lift > M[0] + kSlack || fmaxf(x[1], x[3]) + lift > M[1] + kSlack;
             if (__any_sync(0xffffffffu, up)) {
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
@@ -358,61 +370,48 @@ __global__ void __launch_bounds__(32 * kWarps) kv8_split_kernel(const __grid_con
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-                    m = fmaxf(M[j], m);
+                    m = fmaxf(M[j], m + lift);
                     const float f = exp2_fast(M[j] - m);
-                    l[j] = rebase(l[j], M[j], m);
+                    l[j] *= f;
                     M[j] = m;
 #pragma unroll
                     for (int i = 0; i < MT; ++i) o[i][j] *= f, o[i][j + 2] *= f;
                 }
             }
-            float off[2] = {M[0], M[1]}, mt[2] = {mant, mant}, dn[2] = {down, down};
-            if (__any_sync(0xffffffffu, e < fmaxf(M[0], M[1]) - kFar)) {  // (rare)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    float m = fmaxf(x[j], x[j + 2]);
-                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
-                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
-                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-                    const float d = aside(e, M[j], m);
-                    off[j] -= d, mt[j] *= exp2_fast(-d);
-                    if (d > 0.f) dn[j] = exp2_fast(-e - d);  // (one exponent: either factor may leave the range)
-                }
-            }
             float w[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] = exp2_fast(x[j] - off[j & 1]);
-            l[0] = fmaf(w[0] + w[2], dn[0], l[0]);
-            l[1] = fmaf(w[1] + w[3], dn[1], l[1]);
-            uint32_t ph[2], pl[2];
+            for (int j = 0; j < 4; ++j) w[j] = exp2_fast(x[j] - M[j & 1]);
+            l[0] += w[0] + w[2];
+            l[1] += w[1] + w[3];
+            uint32_t pw[PARTS][2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                // (a hidden position has weight 0 even where the block's scale is not finite)
-                const float p0 = w[2 * i] > 0.f ? w[2 * i] * mt[0] : 0.f;
-                const float p1 = w[2 * i + 1] > 0.f ? w[2 * i + 1] * mt[1] : 0.f;
-                const uint32_t hi = pack_h2(p0, p1);
-                ph[i] = transpose8(hi);
-                if (TERMS == 2) {
-                    const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-                    pl[i] = transpose8(pack_h2(p0 - back.x, p1 - back.y));
+                float p[2];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    p[j] = w[2 * i + j] * sv;
+                    // (a hidden position has weight 0 even where the block's scale is not finite)
+                    if (edge && x[2 * i + j] == -INFINITY) p[j] = 0.f;
                 }
+                uint32_t part[PARTS];
+                split_b2<PARTS>(p[0], p[1], part);
+#pragma unroll
+                for (int k = 0; k < PARTS; ++k) pw[k][i] = transpose8(part[k]);
             }
             // ---- O^T += V^T w^T: lane dims (128 i + 16 g) + 2 j, + 1 are rows g, g + 8 of tile j
 #pragma unroll
             for (int i = 0; i < VC; ++i)
 #pragma unroll
                 for (int q = 0; q < VW; ++q) {
-                    const uint32_t w0 = cur.v[i][0][q] ^ 0x80808080u, w1 = cur.v[i][1][q] ^ 0x80808080u;
-                    const uint32_t w2 = cur.v[i][2][q] ^ 0x80808080u, w3 = cur.v[i][3][q] ^ 0x80808080u;
+                    const uint32_t w0 = cur.v[i][0][q], w1 = cur.v[i][1][q], w2 = cur.v[i][2][q], w3 = cur.v[i][3][q];
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
                         const uint32_t lo = __byte_perm(w0, w1, j ? 0x7362 : 0x5140);
                         const uint32_t hi = __byte_perm(w2, w3, j ? 0x7362 : 0x5140);
-                        const uint32_t a0 = codes_h2(lo, 0x4140), a1 = codes_h2(lo, 0x4342);
-                        const uint32_t a2 = codes_h2(hi, 0x4140), a3 = codes_h2(hi, 0x4342);
-                        float(&d)[4] = o[(i * VW + q) * 2 + j];
-                        mma_f16(d, a0, a1, a2, a3, ph[0], ph[1]);
-                        if (TERMS == 2) mma_f16(d, a0, a1, a2, a3, pl[0], pl[1]);
+                        const uint32_t a0 = codes_b2(lo, 0x4140), a1 = codes_b2(lo, 0x4342);
+                        const uint32_t a2 = codes_b2(hi, 0x4140), a3 = codes_b2(hi, 0x4342);
+#pragma unroll
+                        for (int k = 0; k < PARTS; ++k) mma_bf16(o[(i * VW + q) * 2 + j], a0, a1, a2, a3, pw[k][0], pw[k][1]);
                     }
                 }
         } else {
@@ -455,7 +454,7 @@ __global__ void __launch_bounds__(32 * kWarps) kv8_split_kernel(const __grid_con
             const float2 ml = sml[k][r];
             const float f = exp2_fast(ml.x - m);
             const float4 p = *reinterpret_cast<const float4*>(&so[k][r][d]);
-            sum += rebase(ml.y, ml.x, m);
+            sum = fmaf(ml.y, f, sum);
             v[0] = fmaf(p.x, f, v[0]), v[1] = fmaf(p.y, f, v[1]), v[2] = fmaf(p.z, f, v[2]), v[3] = fmaf(p.w, f, v[3]);
         }
         if (P.splits == 1) {
@@ -501,7 +500,7 @@ template <class T, int HD> __global__ void __launch_bounds__(32 * kJoinWarps) kv
         const uint64_t p = at + (uint64_t)k * P.tile_rows;
         const float2 ml = P.part_ml[p];
         const float f = exp2_fast(ml.x - m);
-        sum += rebase(ml.y, ml.x, m);
+        sum = fmaf(ml.y, f, sum);
 #pragma unroll
         for (int c = 0; c < N; ++c) {
             const float2 w = *reinterpret_cast<const float2*>(P.part_o + p * HD + 64 * c + 2 * lane);
@@ -540,13 +539,10 @@ template <class T, int HD> __global__ void __launch_bounds__(32 * kJoinWarps) kv
 //   4 softmax warps   per row tile, one row per thread: scores to registers, running maximum,
 //                     weights to f16 over the scores' own columns. O is rescaled (read, multiplied,
 //                     written back) only when a score passes the row's maximum by 2^8.
-// 16-bit inputs (TERMS = 1): q is scaled by a power of two per row and held in one f16 part, exactly
-// down to 2^-24 of the row's largest; the weights are one f16 part. f32 inputs (TERMS = 2): q is fixed point in three 8-bit limbs and the
-// scores are integer products (kind::i8) of the codes as they are, summed exactly -- the f32 sums of
-// kind::f16 are cut off, not rounded, and over long sums that shows; the weights are two f16 parts
-// with a product each. The block scales enter as
-// in the kernel above; the value scale as an added log2 where one rounding of the weights follows
-// anyway (TERMS = 1).
+// 16-bit inputs: q is scaled by a power of two per row and held in f16, exactly down to 2^-24 (its largest just under
+// 2^10); the weights are two bf16 parts, with the value scale as an added log2 in their exponent. f32 inputs: q is fixed point in three
+// 8-bit limbs and the scores are integer products (kind::i8) of the codes as they are, summed exactly -- the f32 sums of
+// kind::f16 are cut off, not rounded, and over long sums that shows; the weights are three bf16 parts.
 // Bound: the tensor pipe and, close behind, shared memory: a step of 64 positions with two row tiles of 128 dims
 // is 1024 clocks of products, 1540 of shared-memory traffic (q is read again for every K panel, and
 // the codes pass it three times) and 1024 of exponentials on each scheduler. Measured (2048 tokens behind
@@ -562,26 +558,26 @@ constexpr uint32_t kTileRows = 128;
 // rows, 300 to 16000 positions of 1 to 64 sequences: 1.2 % over the better kernel's time on average, 26 % at
 // most; on either side of the rule, 32 rows over 4099 positions of 9 sequences with 2 kv heads of
 // 256 dims: 30 us against 51; 32 rows over 600 positions of 2 sequences with 8 of 128: 13.1 against 12.3.
-// (f32 up to 128 dims has one row tile and twice the products, and its rows pay later.)
-__host__ __device__ constexpr uint32_t tile_min(int hd, int terms) { return terms == 2 && hd <= 128 ? 48 : 24; }
+// (f32 up to 128 dims has one row tile and more products, and its rows pay later.)
+__host__ __device__ constexpr uint32_t tile_min(int hd, bool f32) { return f32 && hd <= 128 ? 48 : 24; }
 constexpr uint64_t kTileWork = 3;
 
-struct Role {  // per (HD, TERMS): row tiles, positions per step, stages of f16 panels, of codes
+struct Role {  // per (HD, f32 or not): row tiles, positions per step, stages of f16 panels, of codes
     uint32_t rt, np, stages, raw;
 };
-__host__ __device__ constexpr Role role_of(int hd, int terms) {
-    return hd == 256 ? (terms == 2 ? Role{1, 32, 2, 2} : Role{1, 32, 3, 3}) : terms == 2 ? Role{1, 64, 2, 4} : Role{2, 64, 2, 4};
+__host__ __device__ constexpr Role role_of(int hd, bool f32) {
+    return hd == 256 ? (f32 ? Role{1, 32, 2, 2} : Role{1, 32, 3, 3}) : f32 ? Role{1, 64, 2, 4} : Role{2, 64, 2, 4};
 }
 // bytes of one part of a row tile's q (f16; or an 8-bit limb), of a stage's K
-__host__ __device__ constexpr uint32_t q_part(int hd, int terms) { return kTileRows * hd * (terms == 2 ? 1 : 2); }
-__host__ __device__ constexpr uint32_t q_parts(int terms) { return terms == 2 ? 3 : 1; }
-__host__ __device__ constexpr uint32_t k_stage(int hd, int terms) { return role_of(hd, terms).np * hd * (terms == 2 ? 1 : 2); }
-__host__ __device__ constexpr uint32_t tile_smem(int hd, int terms) {
-    return role_of(hd, terms).rt * q_parts(terms) * q_part(hd, terms) +
-           role_of(hd, terms).stages * (k_stage(hd, terms) + role_of(hd, terms).np * hd * 2) +
-           role_of(hd, terms).raw * role_of(hd, terms).np * hd * 2 + 1024;
+__host__ __device__ constexpr uint32_t q_part(int hd, bool f32) { return kTileRows * hd * (f32 ? 1 : 2); }
+__host__ __device__ constexpr uint32_t q_parts(bool f32) { return f32 ? 3 : 1; }
+__host__ __device__ constexpr uint32_t k_stage(int hd, bool f32) { return role_of(hd, f32).np * hd * (f32 ? 1 : 2); }
+__host__ __device__ constexpr uint32_t tile_smem(int hd, bool f32) {
+    return role_of(hd, f32).rt * q_parts(f32) * q_part(hd, f32) +
+           role_of(hd, f32).stages * (k_stage(hd, f32) + role_of(hd, f32).np * hd * 2) +
+           role_of(hd, f32).raw * role_of(hd, f32).np * hd * 2 + 1024;
 }
-static_assert(tile_smem(256, 2) <= 232448 && tile_smem(256, 1) <= 232448 && tile_smem(128, 1) <= 232448, "shared memory");
+static_assert(tile_smem(256, true) <= 232448 && tile_smem(256, false) <= 232448 && tile_smem(128, false) <= 232448, "shared memory");
 
 __device__ __forceinline__ bool bwait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
     if (mbar_try_wait(bar, parity)) return true;
@@ -642,8 +638,10 @@ __device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint3
         "l"(a), "l"(b), "r"(idesc), "r"(acc)
         : "memory");
 }
-__host__ __device__ constexpr uint32_t f16_idesc(uint32_t n, bool b_mn_major) {
-    return (1u << 4) | ((b_mn_major ? 1u : 0u) << 16) | ((n >> 3) << 17) | ((kTileRows >> 4) << 24);
+__host__ __device__ constexpr uint32_t f16_idesc(uint32_t n) { return (1u << 4) | ((n >> 3) << 17) | ((kTileRows >> 4) << 24); }
+// bf16, B as [K][N]
+__host__ __device__ constexpr uint32_t bf16_idesc(uint32_t n) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((n >> 3) << 17) | ((kTileRows >> 4) << 24);
 }
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
@@ -711,29 +709,36 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 __device__ __forceinline__ uint32_t panel_at(uint32_t rows, uint32_t r, uint32_t p) {
     return (p >> 3) * (rows * 128u) + r * 128u + (((p & 7u) ^ (r & 7u)) << 4);
 }
-// 16 codes to f16, two 16-byte pieces
-__device__ __forceinline__ void codes_to_panel(uint8_t* panel, uint32_t rows, uint32_t r, uint32_t c, uint4 w) {
+// 16 codes to f16 (keys) or bf16 (values), two 16-byte pieces
+template <bool BF16> __device__ __forceinline__ void codes_to_panel(uint8_t* panel, uint32_t rows, uint32_t r, uint32_t c, uint4 w) {
     uint32_t h[8];
     const uint32_t in[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const uint32_t b = in[i] ^ 0x80808080u;
-        h[2 * i] = codes_h2(b, 0x4140);
-        h[2 * i + 1] = codes_h2(b, 0x4342);
+        if constexpr (BF16) {
+            h[2 * i] = codes_b2(in[i], 0x4140);
+            h[2 * i + 1] = codes_b2(in[i], 0x4342);
+        } else {
+            const uint32_t b = in[i] ^ 0x80808080u;
+            h[2 * i] = codes_h2(b, 0x4140);
+            h[2 * i + 1] = codes_h2(b, 0x4342);
+        }
     }
     *reinterpret_cast<uint4*>(panel + panel_at(rows, r, 2 * c)) = make_uint4(h[0], h[1], h[2], h[3]);
     *reinterpret_cast<uint4*>(panel + panel_at(rows, r, 2 * c + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
 }
 
 template <class T, int HD>
-__global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).rt + 5), 1)
+__global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4).rt + 5), 1)
     kv8_tile_kernel(const __grid_constant__ Plan P) {
-    constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
-    constexpr Role R = role_of(HD, TERMS);
+    constexpr bool F32 = sizeof(T) == 4;
+    constexpr int PARTS = F32 ? 3 : 2;  // bf16 parts of a weight
+    constexpr Role R = role_of(HD, F32);
     constexpr uint32_t RT = R.rt, NP = R.np, ST = R.stages, RAW = R.raw, NB = NP / 16;
-    constexpr uint32_t kQPart = q_part(HD, TERMS), kQParts = q_parts(TERMS);
-    constexpr uint32_t kK = k_stage(HD, TERMS), kV = NP * HD * 2, kStage = kK + kV;  // K and V of a stage
-    constexpr uint32_t kSCols = TERMS == 2 ? 3 * NP : NP;  // tensor memory columns of a score buffer
+    constexpr uint32_t kQPart = q_part(HD, F32), kQParts = q_parts(F32);
+    constexpr uint32_t kK = k_stage(HD, F32), kV = NP * HD * 2, kStage = kK + kV;  // K and V of a stage
+    constexpr uint32_t kSCols = F32 ? 3 * NP : NP;  // tensor memory columns of a score buffer, then of its weights
+    static_assert(PARTS * NP / 2 <= kSCols, "tensor memory");
     // log2 of a row tile's score buffers: as many as its share of the tensor memory holds beside O, up to four
     constexpr uint32_t kMostBuffers = HD + 4 * kSCols <= 512 ? 2 : 1, kShared = RT == 1 ? kMostBuffers : 1;
     static_assert(RT * (HD + (kSCols << kShared)) <= 512 && (RT == 1 || HD + 2 * kSCols <= 256), "tensor memory");
@@ -742,7 +747,7 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
     constexpr uint32_t FG = 8, FS = 2 * FG;  // steps of block factors handed over together, and kept
     __shared__ __align__(8) uint64_t k_full[ST], k_empty[ST], v_full[ST], v_empty[ST], f_full[2], f_empty[2], c_full[RAW], c_empty[RAW];
     __shared__ __align__(8) uint64_t s_full[RT][4], p_full[RT][4], o_done[RT][4], q_full, fin[RT];
-    __shared__ float4 f_blk[FS][NB];  // key scale, exponent of the value scale, 2^-exponent, mantissa
+    __shared__ float4 f_blk[FS][NB];  // key scale, log2 of the value scale (f32: 0; -infinity: no such page, infinity: a rare one), its inverse, itself
     __shared__ uint32_t tmem_base;
     __shared__ volatile int abort_flag;
     const Kv8AttnArgs& a = P.a;
@@ -831,11 +836,11 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
             }
             const bool bad = m >= 0x7f800000u;
             // largest magnitude just under 2^10 (f16) or 2^22 (limbs)
-            const int sh = min(100, (TERMS == 2 ? 22 : 10) - ((int)(m >> 23) - 126));
+            const int sh = min(100, (F32 ? 22 : 10) - ((int)(m >> 23) - 126));
             const float up = copysignf(exp2f((float)sh), a.scale);  // (so that the factor is not negative)
             step = bad ? __uint_as_float(0x7fc00000u) : exp2f((float)-sh) * fabsf(a.scale) * 1.4426950408889634f;
             uint8_t* panel = sq + rt * kQParts * kQPart;
-            if constexpr (TERMS == 1) {
+            if constexpr (!F32) {
 #pragma unroll 4
                 for (int d = 0; d < HD; d += 8) {
                     float v[8];
@@ -902,52 +907,59 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
             const uint32_t ts = to + HD + j % nsb * kSCols;
             const int32_t p0 = (b0 + (int32_t)(j * NB)) * 16;
             const bool masked = p0 + (int32_t)NP - 1 > open;
-            float f[NB], e[NB], down[NB], mant[NB];
-            bool far = false;  // a block far below the maximum, or one of zeros
+            float f[NB], e[NB], down[NB], sv[NB];
+            bool rare = false;  // a block of zeros, of a scale near the ends of f32's range or not finite, or without a page
 #pragma unroll
             for (uint32_t b = 0; b < NB; ++b) {
                 const float4 w = f_blk[st][b];
                 f[b] = step * w.x;
-                e[b] = w.y, down[b] = w.z, mant[b] = w.w;
-                far |= e[b] < M - kFar || mant[b] == 0.f;
+                e[b] = w.y, down[b] = w.z, sv[b] = w.w;
+                rare |= fabsf(e[b]) == INFINITY;
             }
             // ---- the usual step: nothing hidden, and the maximum still holds. The weights are made
-            // without looking for the maximum: their sum tells whether one may be too large for f16 (or is
+            // without looking for the maximum: their sum tells whether one passes it by far (or is
             // not a number), and then the scores are read again below.
-            if (TERMS == 1 && j > 0 && !masked && !__any_sync(0xffffffffu, far)) {
-                uint32_t hi[NP / 2];
-                float add = 0.f, tot = 0.f;
-                uint32_t v[2][16];
-                tmem_ld16(ts, v[0]);
+            if (!F32 && j > 0 && !masked && !__any_sync(0xffffffffu, rare)) {
+                uint32_t v[NP];
+                float add = 0.f;
+                tmem_ld16(ts, *reinterpret_cast<uint32_t(*)[16]>(v));
                 tmem_ld_wait();
 #pragma unroll
                 for (uint32_t b = 0; b < NB; ++b) {  // the next block's scores on their way meanwhile
-                    if (b + 1 < NB) tmem_ld16(ts + 16 * (b + 1), v[(b + 1) & 1]);
-                    const uint32_t(&x)[16] = v[b & 1];
+                    if (b + 1 < NB) tmem_ld16(ts + 16 * (b + 1), *reinterpret_cast<uint32_t(*)[16]>(v + 16 * (b + 1)));
                     const uint64_t ff = pack2(f[b], f[b]), off = pack2(e[b] - M, e[b] - M);
                     uint64_t sum = 0;
 #pragma unroll
-                    for (uint32_t i = 0; i < 8; ++i) {
-                        const uint64_t y = fma2(pack2(x[2 * i], x[2 * i + 1]), ff, off);
+                    for (uint32_t i = 16 * b; i < 16 * b + 16; i += 2) {
+                        const uint64_t y = fma2(pack2(v[i], v[i + 1]), ff, off);
                         const float w0 = exp2_fast(lo2(y)), w1 = exp2_fast(hi2(y));
                         sum = add2(sum, pack2(w0, w1));
-                        hi[8 * b + i] = pack_h2(w0, w1);
+                        // (split_b2, the differences of a pair in one addition; the parts take the scores' registers)
+                        const uint32_t a0 = __float_as_uint(w0), a1 = __float_as_uint(w1);
+                        const uint64_t left = add2(pack2(a0, a1), pack2((a0 & 0xffff0000u) ^ 0x80000000u, (a1 & 0xffff0000u) ^ 0x80000000u));
+                        const __nv_bfloat162 r = __floats2bfloat162_rn(lo2(left), hi2(left));
+                        v[i] = __byte_perm(a0, a1, 0x7632);
+                        v[i + 1] = *reinterpret_cast<const uint32_t*>(&r);
                     }
-                    const float s1 = lo2(sum) + hi2(sum);
-                    tot += s1;
-                    add = fmaf(s1, down[b], add);
+                    add = fmaf(lo2(sum) + hi2(sum), down[b], add);
                     if (b + 1 < NB) tmem_ld_wait();
                 }
-                if (__all_sync(0xffffffffu, tot < 16384.f)) {
+                if (__all_sync(0xffffffffu, add < 16384.f)) {
                     l += add;
 #pragma unroll
-                    for (uint32_t b = 0; b < NB; ++b) tmem_st8(ts + 8 * b, hi + 8 * b);
+                    for (uint32_t b = 0; b < NB; ++b) {
+                        uint32_t hi[8], lo[8];
+#pragma unroll
+                        for (uint32_t i = 0; i < 8; ++i) hi[i] = v[16 * b + 2 * i], lo[i] = v[16 * b + 2 * i + 1];
+                        tmem_st8(ts + 8 * b, hi);
+                        tmem_st8(ts + NP / 2 + 8 * b, lo);
+                    }
                     done();
                     continue;
                 }
             }
             uint32_t v[NP];
-            if constexpr (TERMS == 1) {
+            if constexpr (!F32) {
 #pragma unroll
                 for (uint32_t c = 0; c < NP; c += 32) tmem_ld32(ts + c, *reinterpret_cast<uint32_t(*)[32]>(v + c));
                 tmem_ld_wait();
@@ -970,19 +982,18 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
                     if (p0 + (int32_t)i > last) v[i] = 0xff800000u;  // -infinity
             }
             // the largest score: of each block's products, then by the block's factor (not negative)
-            float mx = -INFINITY, most[NB];
+            float mx = -INFINITY;
 #pragma unroll
             for (uint32_t b = 0; b < NB; ++b) {
                 float m = __uint_as_float(v[16 * b]);
 #pragma unroll
                 for (uint32_t i = 1; i < 16; ++i) m = fmaxf(m, __uint_as_float(v[16 * b + i]));
                 // (a hidden block and a factor of 0: 0 * -infinity is not a number)
-                most[b] = m == -INFINITY ? m : fmaf(m, f[b], e[b]);
-                mx = fmaxf(mx, most[b]);
+                mx = fmaxf(mx, m == -INFINITY || e[b] == -INFINITY ? -INFINITY : fmaf(m, f[b], lift_of(sv[b])));
             }
             if (__any_sync(0xffffffffu, mx > M + kSlack)) {
                 const float m = fmaxf(M, mx), f8 = exp2_fast(M - m);
-                l = rebase(l, M, m);
+                l *= f8;
                 M = m;
                 if (j > 0) {
                     ok = warp_wait(&o_done[rt][(j - 1) % nsb], ((j - 1) >> lsb) & 1, &abort_flag);
@@ -999,43 +1010,35 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
                     }
                 }
             }
-            far = false;  // (the maximum may have moved)
-#pragma unroll
-            for (uint32_t b = 0; b < NB; ++b) far |= (e[b] < M - kFar && e[b] != -INFINITY) || mant[b] == 0.f;
-            auto weights = [&](auto rare) {  // rare: hidden positions, or a block far below the maximum
-                constexpr bool RARE = decltype(rare)::value;
+            auto weights = [&](auto some) {  // some: hidden positions, or a block that is rare
+                constexpr bool SOME = decltype(some)::value;
 #pragma unroll
                 for (uint32_t b = 0; b < NB; ++b) {
                     float sum = 0.f;
-                    uint32_t hi[8], lo[8];
-                    float off = e[b] - M, mt = mant[b], dn = down[b];
-                    if (RARE && off < -kFar && off != -INFINITY) {
-                        const float d = aside(e[b], M, most[b]);
-                        off += d, mt *= exp2_fast(-d);
-                        if (d > 0.f) dn = exp2_fast(-e[b] - d);
-                    }
+                    uint32_t part[PARTS][8];
+                    const float off = SOME && e[b] == -INFINITY ? -INFINITY : -M;
 #pragma unroll
                     for (uint32_t i = 0; i < 8; ++i) {
-                        const float x0 = __uint_as_float(v[16 * b + 2 * i]), x1 = __uint_as_float(v[16 * b + 2 * i + 1]);
-                        float w0 = exp2_fast(fmaf(x0, f[b], off)), w1 = exp2_fast(fmaf(x1, f[b], off));
-                        if (RARE) {  // (a product itself is never infinite)
-                            w0 = x0 == -INFINITY ? 0.f : w0;
-                            w1 = x1 == -INFINITY ? 0.f : w1;
+                        float p[2];
+#pragma unroll
+                        for (uint32_t k = 0; k < 2; ++k) {
+                            const float x = __uint_as_float(v[16 * b + 2 * i + k]);
+                            const bool hidden = SOME && x == -INFINITY;  // (a product itself is never infinite)
+                            const float w = hidden ? 0.f : exp2_fast(fmaf(x, f[b], off));
+                            sum += w;
+                            p[k] = hidden ? 0.f : w * sv[b];
                         }
-                        sum += w0 + w1;
-                        if (TERMS == 2 || RARE) w0 *= mt, w1 *= mt;
-                        hi[i] = pack_h2(w0, w1);
-                        if (TERMS == 2) {
-                            const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi[i]));
-                            lo[i] = pack_h2(w0 - back.x, w1 - back.y);
-                        }
+                        uint32_t pp[PARTS];
+                        split_b2<PARTS>(p[0], p[1], pp);
+#pragma unroll
+                        for (int k = 0; k < PARTS; ++k) part[k][i] = pp[k];
                     }
-                    l = fmaf(sum, dn, l);
-                    tmem_st8(ts + 8 * b, hi);
-                    if (TERMS == 2) tmem_st8(ts + NP / 2 + 8 * b, lo);
+                    l += sum;
+#pragma unroll
+                    for (int k = 0; k < PARTS; ++k) tmem_st8(ts + k * (NP / 2) + 8 * b, part[k]);
                 }
             };
-            if (masked || __any_sync(0xffffffffu, far)) weights(std::true_type{});
+            if (masked || __any_sync(0xffffffffu, rare)) weights(std::true_type{});
             else weights(std::false_type{});
             done();
         }
@@ -1092,12 +1095,12 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
         auto piece = [&](uint32_t i) { return pt + 128 * i; };
         auto code_at = [&](uint32_t i) { return row_of(piece(i)) * HD + 16 * col_of(piece(i)); };
         // (blocks without a valid page were not copied: whatever codes lie there have weight 0)
-        auto widen = [&](uint8_t* panel, const uint8_t* raw) {
+        auto widen = [&](auto bf16, uint8_t* panel, const uint8_t* raw) {
             uint4 w[N];
 #pragma unroll
             for (uint32_t i = 0; i < N; ++i) w[i] = *reinterpret_cast<const uint4*>(raw + code_at(i));
 #pragma unroll
-            for (uint32_t i = 0; i < N; ++i) codes_to_panel(panel, NP, row_of(piece(i)), col_of(piece(i)), w[i]);
+            for (uint32_t i = 0; i < N; ++i) codes_to_panel<decltype(bf16)::value>(panel, NP, row_of(piece(i)), col_of(piece(i)), w[i]);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
         };
@@ -1115,11 +1118,11 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
             uint8_t* dst = skv + st * kStage;
             warp_wait(&c_full[rs], (j / RAW) & 1, &abort_flag);
             if (j >= ST) warp_wait(&k_empty[st], (j / ST - 1) & 1, &abort_flag);
-            if (TERMS == 1) widen(dst, raw);
-            else copy(dst, raw);
+            if (F32) copy(dst, raw);
+            else widen(std::false_type{}, dst, raw);
             if (lane == 0) mbar_arrive(&k_full[st]);
             if (j >= ST) warp_wait(&v_empty[st], (j / ST - 1) & 1, &abort_flag);
-            widen(dst + kK, raw + NP * HD);
+            widen(std::true_type{}, dst + kK, raw + NP * HD);
             if (lane == 0) {
                 mbar_arrive(&v_full[st]);
                 mbar_arrive(&c_empty[rs]);
@@ -1163,23 +1166,15 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
                 }
                 ++n;
             };
-            // sv = mant 2^e (TERMS = 2), or e = log2 sv; zeros have mant 0 and an exponent that no maximum
-            // notices; a scale that is not finite makes the weights of the rows that see it so
-            const uint32_t sb = __float_as_uint(sv);
-            const int eb = (int)((sb >> 23) & 0xffu);
-            const bool plain = eb > 0 && eb < 255;
-            const float mant = eb == 0 ? 0.f : TERMS == 2 && plain ? __uint_as_float((sb & 0x807fffffu) | 0x3f800000u) : 1.f;
-            const float down = !plain ? kZeroDown : TERMS == 2 ? __uint_as_float((uint32_t)(254 - eb) << 23) : __fdiv_rn(1.f, sv);
-            const float e = hidden      ? -INFINITY
-                            : eb == 255 ? __uint_as_float(0x7fc00000u)
-                            : eb == 0   ? kZeroExp
-                            : TERMS == 2 ? (float)(eb - 127)
-                                         : log2f(sv);
+            // (a page that is not there: weights of 0 that are not counted; a scale of 0: weights that are)
+            sv = zero_if_subnormal(sv);
+            const bool plain = sv > 0.f && sv < INFINITY && lift_of(sv) == 0.f;
+            const float e = hidden ? -INFINITY : !plain ? INFINITY : F32 ? 0.f : log2f(sv), down = !F32 && plain ? __fdiv_rn(1.f, sv) : 0.f;
             for (uint32_t g = 0; g < LS / FG && j0 + g * FG < steps && ok; ++g) {
                 const uint32_t grp = j0 / FG + g;
                 if (grp >= 2) ok = warp_wait(&f_empty[grp % 2], (grp / 2 - 1) & 1, &abort_flag);
                 __syncwarp();
-                if (lane / NB / FG == g) f_blk[(j0 + lane / NB) % FS][lane % NB] = make_float4(sk, e, down, mant);
+                if (lane / NB / FG == g) f_blk[(j0 + lane / NB) % FS][lane % NB] = make_float4(sk, e, down, sv);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&f_full[grp % 2]);
                 for (uint32_t i = 0; i < FG && j0 + g * FG + i < steps && ok; ++i) copies(j0 + g * FG + i);
@@ -1202,11 +1197,11 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
             if (!ok) return;
             tc_after();
             const uint32_t kb = smem_addr(skv + st * kStage), ds = d + HD + j % nsb * kSCols;
-            if constexpr (TERMS == 1) {
+            if constexpr (!F32) {
 #pragma unroll
                 for (uint32_t k = 0; k < HD / 16; ++k)
                     mma_ss(ds, swizzled_desc(qb + (k / 4) * (kTileRows * 128) + (k % 4) * 32, 16),
-                           swizzled_desc(kb + (k / 4) * (NP * 128) + (k % 4) * 32, 16), f16_idesc(NP, false), k > 0);
+                           swizzled_desc(kb + (k / 4) * (NP * 128) + (k % 4) * 32, 16), f16_idesc(NP), k > 0);
             } else {
 #pragma unroll
                 for (uint32_t x = 0; x < 3; ++x)
@@ -1228,10 +1223,10 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4 ? 2 : 1).
             tc_after();
             const uint32_t pw = d + HD + j % nsb * kSCols;
 #pragma unroll
-            for (uint32_t x = 0; x < (uint32_t)TERMS; ++x)
+            for (uint32_t x = 0; x < (uint32_t)PARTS; ++x)
 #pragma unroll
                 for (uint32_t k = 0; k < NP / 16; ++k)
-                    mma_ts(d, pw + x * (NP / 2) + 8 * k, swizzled_desc(vb + k * 2048, NP * 128), f16_idesc(HD, true),
+                    mma_ts(d, pw + x * (NP / 2) + 8 * k, swizzled_desc(vb + k * 2048, NP * 128), bf16_idesc(HD),
                            j > 0 || x > 0 || k > 0);
             mma_commit(&o_done[rt][j % nsb]);
             mma_commit(&v_empty[st]);
@@ -1257,12 +1252,12 @@ struct Shape {
 Shape shape_of(const Kv8Cache& c, const Kv8Batch& b, uint32_t heads, uint32_t type, int sms) {
     Shape r;
     r.group = heads / c.kv_heads;
-    const int terms = type == GGML_F32 ? 2 : 1;
+    const bool f32 = type == GGML_F32;
     const uint64_t rows = (uint64_t)std::max(1u, b.max_new) * r.group;
     const uint32_t blocks = std::max(1u, (b.max_len + 15) / 16);
-    r.tiles = rows >= tile_min((int)c.head_dim, terms) &&
+    r.tiles = rows >= tile_min((int)c.head_dim, f32) &&
               (double)b.n_seqs * c.kv_heads * blocks * ((rows + kRows - 1) / kRows) >= (double)kTileWork * 3 * kWarps * sms;
-    const Role role = role_of((int)c.head_dim, terms);
+    const Role role = role_of((int)c.head_dim, f32);
     r.tile_rows = r.tiles ? role.rt * kTileRows : kRows;
     r.row_tiles = (uint32_t)((rows + r.tile_rows - 1) / r.tile_rows);
     // chunks of positions: enough CTAs for three on every SM (the prompt kernel: one; one row tile of 256
@@ -1294,8 +1289,8 @@ template <auto kernel> cudaError_t opt_in(uint32_t smem) {
 
 template <class T, int HD> cudaError_t launch(const Plan& p, bool tiles, cudaStream_t s) {
     if (tiles) {
-        constexpr int terms = sizeof(T) == 4 ? 2 : 1;
-        constexpr uint32_t smem = tile_smem(HD, terms), threads = 32 * (5 * role_of(HD, terms).rt + 5);
+        constexpr bool f32 = sizeof(T) == 4;
+        constexpr uint32_t smem = tile_smem(HD, f32), threads = 32 * (5 * role_of(HD, f32).rt + 5);
         cudaError_t e = opt_in<kv8_tile_kernel<T, HD>>(smem);
         if (e != cudaSuccess) return e;
         e = launch_chained(kv8_tile_kernel<T, HD>, dim3(p.row_tiles * p.splits, p.a.c.kv_heads, p.a.b.n_seqs), threads, smem, s, p);

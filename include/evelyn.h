@@ -368,9 +368,12 @@ evl_status evl_kv8_attention_workspace_bytes(const evl_kv8_cache* cache, const e
  * head h / (heads / kv_heads). d_q and d_out [total][heads][head_dim] of `type`, tokens q_stride /
  * out_stride elements apart, 16-byte aligned, strides multiples of 16 bytes. heads a multiple of
  * kv_heads. scale 0: 1 / sqrt(head_dim). A row that sees no position gives zeros; a query row that
- * holds an infinity or a NaN gives NaN. Scores are held in f32 with the base-2 exponent of the
- * value scale added, so they are good to 2^-24 of their size, and beyond 1e38 in magnitude to
- * nothing. Rows of d_out that belong to no sequence are left as they were. One kernel serves all
+ * holds an infinity or a NaN gives NaN, and so does one that sees a block whose value scale is not finite, however
+ * small its weights there. Scores are held in f32. In them each value of q is good to 2^-22 of its row's largest
+ * magnitude (not of its own), so beside a loud channel of q a score may be off by that times sum |k|; the 16-bit
+ * types with many rows hold q exactly to 2^-34 of the largest and sum the products in f32, cut off by up to 2^-23 of
+ * the terms' sizes after every 16 dims. Scores beyond 1e38 in magnitude are good for nothing. Weights keep f32's range, and 24 bits (16-bit types:
+ * 15) however far they lie below the largest. Rows of d_out that belong to no sequence are left as they were. One kernel serves all
  * sequences of a call, chosen by max_new: a batch that mixes prompts with single tokens gives
  * the same sums but is faster as two calls. d_workspace: evl_kv8_attention_workspace_bytes, 256-byte aligned, needing no initial
  * value; calls that may overlap in time need one each. */

@@ -106,3 +106,97 @@ def test_attention_large_scores(tokens, kind, dim, zeros, top):
         x = sign * (top / (127 / 40) / dim / scale)  # q . k of level 127 is `top`
         q = dev(np.tile(x, (tokens, 4, 1)).astype(np.float32), kind)
         _compare(kv, n, tokens, q, kind, scale=scale)
+
+
+# ------------------------------------------------------------------ one position dominates
+def _levels(rng, n, dim, nats, low, high):
+    """Keys whose scores lie `nats` under the largest, at level 127, and a query for them (scale 1 / sqrt(dim))."""
+    sign = rng.choice([-1, 1], dim)
+    top = 2.0 * nats
+    x = sign * (top / (127 / 40) / np.sqrt(dim))
+    return sign, rng.integers(low, high, n), x
+
+
+@KERNELS
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim,n", [(64, 200), (128, 333), (256, 200), (64, 16384)])
+@pytest.mark.parametrize("nats", [8, 12, 16, 20, 25, 40])
+def test_attention_one_position_dominates(tokens, kind, dim, n, nats):
+    """Nearly all weight on one position whose value is zero: the output is made of the others, whose weights are
+    e^-nats of it."""
+    _wide(tokens)
+    rng = np.random.default_rng(nats * 7 + n + dim)
+    kv = Kv(rng, 1, dim, 32, [n])
+    sign, level, x = _levels(rng, n, dim, nats, 60, 67)
+    sink = 5
+    level[sink] = 127
+    v = rng.integers(-127, 128, (n, dim))
+    v[sink] = 0
+    blocks = -(-n // 16)
+    _put(kv, level[:, None] * sign, v, np.full(blocks, 1 / 40, np.float32), rng.uniform(0.5, 1.5, blocks).astype(np.float32) / 40)
+    q = dev(np.tile(x, (tokens, 4, 1)).astype(np.float32), kind)
+    _compare(kv, n, tokens, q, kind)
+
+
+@KERNELS
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim", [64, 256])
+@pytest.mark.parametrize("v_scale,others", [(1e-25, 1e-25), (1e30, 1e30), (1e-30, 1.0), (1e30, 1e-25), (1e36, 1e36), (1e-30, 1e-30)])
+def test_attention_value_scales_at_the_ends(tokens, kind, dim, v_scale, others):
+    """The same with values near the ends of f32's range, alone and beside ordinary ones."""
+    if kind == "f16" and max(v_scale, others) > 100:
+        return  # (f16 outputs end at 65504)
+    _wide(tokens)
+    rng = np.random.default_rng(int(abs(np.log10(v_scale))) + dim)
+    n = 128
+    kv = Kv(rng, 1, dim, 16, [n])
+    sign, level, x = _levels(rng, n, dim, 6, 50, 100)
+    v = rng.integers(-127, 128, (n, dim))
+    vs = np.full(8, others, np.float32)
+    vs[3] = vs[6] = v_scale
+    _put(kv, level[:, None] * sign, v, np.full(8, 1 / 40, np.float32), vs)
+    q = dev(np.tile(x, (tokens, 4, 1)).astype(np.float32), kind)
+    _compare(kv, n, tokens, q, kind)
+
+
+@KERNELS
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("loud", [30, 1000])
+def test_attention_loud_channel_in_q(tokens, kind, dim, loud):
+    """One channel of q many times larger than the others, against keys that are small there."""
+    _wide(tokens)
+    rng = np.random.default_rng(loud + dim)
+    n = 300
+    kv = Kv(rng, 1, dim, 32, [n])
+    k, v = rng.integers(-127, 128, (n, dim)), rng.integers(-127, 128, (n, dim))
+    k[:, 7] = rng.integers(-1, 2, n)
+    _put(kv, k, v, np.full(19, 1 / 60, np.float32), np.full(19, 1 / 40, np.float32))
+    q = rng.standard_normal((tokens, 4, dim)).astype(np.float32)
+    q[..., 7] *= loud
+    _compare(kv, n, tokens, dev(q, kind), kind)
+
+
+@KERNELS
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("value", [np.nan, np.inf])
+@pytest.mark.parametrize("nats", [5, 60, 120])
+def test_attention_block_that_is_not_finite_far_below_the_maximum(tokens, kind, dim, value, nats):
+    """A value scale that is not finite reaches every token that sees its block, however small the weights there, and
+    no token that does not."""
+    _wide(tokens)
+    rng = np.random.default_rng(nats + dim)
+    n = 60
+    kv = Kv(rng, 1, dim, 16, [n])
+    sign, level, x = _levels(rng, n, dim, nats, 60, 67)
+    level[2] = 127
+    vs = np.full(4, 1 / 40, np.float32)
+    vs[3] = value  # positions 48 and on
+    _put(kv, level[:, None] * sign, rng.integers(-127, 128, (n, dim)), np.full(4, 1 / 40, np.float32), vs)
+    q = dev(np.tile(x, (tokens, 4, 1)).astype(np.float32), kind)
+    assert not np.isfinite(host(_attend(kv, [n], [tokens], q, kind))).any()
+    for last in (48, 48 + tokens // 2):  # the last token's length: half of the tokens see the block
+        got = host(_attend(kv, [last], [tokens], q, kind))
+        see = last - 48
+        assert np.isfinite(got[:tokens - see]).all() and not np.isfinite(got[tokens - see:]).any()
