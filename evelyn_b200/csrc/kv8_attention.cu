@@ -21,7 +21,8 @@
 //      is as good as an f32 dot product. The K order inside the product is permuted so that a
 //      lane's fragment is 16 neighbouring bytes of a row: the codes reach the tensor cores as they
 //      were copied, with no conversion.
-//   V: mma.sync m16n8k16 in bf16. A lane loads 16 neighbouring dims of four positions and pairs
+//   V: mma.sync m16n8k16 in bf16; for f32 a block's products are summed there and the blocks in registers, since
+//      the tensor cores' own sums are cut off (66.8 -> 74.5 us at 131071 positions, with the third part). A lane loads 16 neighbouring dims of four positions and pairs
 //      positions with byte permutes; the weights move to the other operand's layout by 8x8 transposes.
 //   The maximum is raised only when a score passes it by 2^8, so most blocks cost one vote.
 // A warp takes every 4th block of the CTA's chunk of positions, the next blocks already on their way
@@ -44,6 +45,7 @@ namespace {
 
 constexpr uint32_t kRows = 8;     // rows of a tile (the product's N)
 constexpr uint32_t kWarps = 4;
+constexpr uint32_t kSumBlocks = 512;  // blocks that a warp sums on the tensor cores (16-bit types; see sum_steps)
 constexpr float kNegBig = -1e38f;  // a maximum that no score has reached
 constexpr float kSlack = 8.f;      // the maximum is raised when a score passes it by this: weights stay below 2^8
 
@@ -54,7 +56,7 @@ struct Plan {
     uint32_t chunk;      // blocks of 16 positions per split
     uint32_t splits;
     uint32_t tile_rows;  // rows of a tile: kRows, or those of the prompt kernel
-    float* part_o;       // [sequence][kv head][row tile][split][tile_rows][head_dim]
+    float* part_o;       // [sequence][kv head][row tile][split][tile_rows][head_dim]; also where sums of long chunks stand
     float2* part_ml;     // same without head_dim: (M, l)
 };
 
@@ -410,8 +412,18 @@ __global__ void __launch_bounds__(32 * kWarps) kv8_split_kernel(const __grid_con
                         const uint32_t hi = __byte_perm(w2, w3, j ? 0x7362 : 0x5140);
                         const uint32_t a0 = codes_b2(lo, 0x4140), a1 = codes_b2(lo, 0x4342);
                         const uint32_t a2 = codes_b2(hi, 0x4140), a3 = codes_b2(hi, 0x4342);
+                        float(&sum)[4] = o[(i * VW + q) * 2 + j];
+                        if constexpr (PARTS == 3) {
+                            // (smallest parts first, into zeros: the tensor cores cut their sums off, O is added rounded)
+                            float d[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                        for (int k = 0; k < PARTS; ++k) mma_bf16(o[(i * VW + q) * 2 + j], a0, a1, a2, a3, pw[k][0], pw[k][1]);
+                            for (int k = PARTS - 1; k >= 0; --k) mma_bf16(d, a0, a1, a2, a3, pw[k][0], pw[k][1]);
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) sum[k] += d[k];
+                        } else {  // (at most kSumBlocks of them in a row)
+#pragma unroll
+                            for (int k = 0; k < PARTS; ++k) mma_bf16(sum, a0, a1, a2, a3, pw[k][0], pw[k][1]);
+                        }
                     }
                 }
         } else {
@@ -561,6 +573,11 @@ constexpr uint32_t kTileRows = 128;
 // (f32 up to 128 dims has one row tile and more products, and its rows pay later.)
 __host__ __device__ constexpr uint32_t tile_min(int hd, bool f32) { return f32 && hd <= 128 ? 48 : 24; }
 constexpr uint64_t kTileWork = 3;
+
+// Steps whose products are added up in tensor memory. Its sums are cut off, not rounded, by up to 2^-23 at
+// each product of 16 positions and one part (values of one sign lose 4.4e-8 each on average); after 96 of them (f32;
+// 1024: 16-bit types) O joins a sum in the workspace, rounded to nearest, and starts again from zero.
+__host__ __device__ constexpr uint32_t sum_steps(uint32_t np, bool f32) { return (f32 ? 96u / 3 : 1024u / 2) / (np / 16); }
 
 struct Role {  // per (HD, f32 or not): row tiles, positions per step, stages of f16 panels, of codes
     uint32_t rt, np, stages, raw;
@@ -739,6 +756,7 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4).rt + 5),
     constexpr uint32_t kK = k_stage(HD, F32), kV = NP * HD * 2, kStage = kK + kV;  // K and V of a stage
     constexpr uint32_t kSCols = F32 ? 3 * NP : NP;  // tensor memory columns of a score buffer, then of its weights
     static_assert(PARTS * NP / 2 <= kSCols, "tensor memory");
+    constexpr uint32_t G = sum_steps(NP, F32);
     // log2 of a row tile's score buffers: as many as its share of the tensor memory holds beside O, up to four
     constexpr uint32_t kMostBuffers = HD + 4 * kSCols <= 512 ? 2 : 1, kShared = RT == 1 ? kMostBuffers : 1;
     static_assert(RT * (HD + (kSCols << kShared)) <= 512 && (RT == 1 || HD + 2 * kSCols <= 256), "tensor memory");
@@ -883,7 +901,10 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4).rt + 5),
         // no row of this warp hides a position before this one
         const int32_t open = sp.base + min(r0 + (int32_t)(rt * kTileRows + quad * 32), rows - 1) / (int32_t)P.group;
         const uint32_t to = tm + rt * kTileCols + ((quad * 32) << 16);  // O, then the score buffers
-        float M = kNegBig, l = 0.f;
+        const uint64_t slot = ((((uint64_t)s * a.c.kv_heads + h) * P.row_tiles + tile) * P.splits + split) * P.tile_rows +
+                              rt * kTileRows + lr;
+        float* part = P.part_o + slot * HD;
+        float M = kNegBig, l = 0.f, Msum = 0.f;  // Msum: the maximum under which the sum in the workspace stands
         bool ok = true;
         for (uint32_t j = 0; j < steps && ok; ++j) {
             const uint32_t st = j % FS, fg = j / FG % 2;
@@ -903,6 +924,32 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4).rt + 5),
             if (idle) {  // (what these rows add up goes nowhere)
                 done();
                 continue;
+            }
+            if (j && j % G == 0) {
+                ok = warp_wait(&o_done[rt][(j - 1) % nsb], ((j - 1) >> lsb) & 1, &abort_flag);
+                if (!ok) break;
+                tc_after();
+                const float f = exp2_fast(Msum - M);
+#pragma unroll 1
+                for (uint32_t c = 0; c < HD; c += 16) {
+                    uint32_t o[16];
+                    tmem_ld16(to + c, o);
+                    tmem_ld_wait();
+                    if (live) {
+#pragma unroll
+                        for (int i = 0; i < 16; i += 4) {
+                            float4 y = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]), __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
+                            float4* at = reinterpret_cast<float4*>(part + c + i);
+                            if (j > G) {
+                                const float4 x = *at;
+                                y.x = fmaf(x.x, f, y.x), y.y = fmaf(x.y, f, y.y), y.z = fmaf(x.z, f, y.z), y.w = fmaf(x.w, f, y.w);
+                            }
+                            *at = y;
+                        }
+                    }
+                    __syncwarp();
+                }
+                Msum = M;
             }
             const uint32_t ts = to + HD + j % nsb * kSCols;
             const int32_t p0 = (b0 + (int32_t)(j * NB)) * 16;
@@ -995,7 +1042,7 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4).rt + 5),
                 const float m = fmaxf(M, mx), f8 = exp2_fast(M - m);
                 l *= f8;
                 M = m;
-                if (j > 0) {
+                if (j % G) {  // (a step that starts O again finds nothing to move)
                     ok = warp_wait(&o_done[rt][(j - 1) % nsb], ((j - 1) >> lsb) & 1, &abort_flag);
                     if (!ok) break;
                     tc_after();
@@ -1047,8 +1094,6 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4).rt + 5),
         if (ok) {
             const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);  // a row that sees nothing: zeros
             T* out = static_cast<T*>(a.out) + (uint64_t)(sp.q0 + tok) * a.out_stride + (uint64_t)head * HD;
-            const uint64_t slot = ((((uint64_t)s * a.c.kv_heads + h) * P.row_tiles + tile) * P.splits + split) * P.tile_rows +
-                                  rt * kTileRows + lr;
             if (live && P.splits > 1) P.part_ml[slot] = make_float2(M, l);
             for (uint32_t c = 0; c < HD; c += 32) {
                 uint32_t o[32];
@@ -1059,12 +1104,23 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4).rt + 5),
 #pragma unroll
                     for (int i = 0; i < 32; ++i) o[i] = 0;
                 }
+                if (steps > G && live) {
+                    const float f = exp2_fast(Msum - M);
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) {
+                        const float4 x = *reinterpret_cast<const float4*>(part + c + i);
+                        o[i] = __float_as_uint(fmaf(x.x, f, __uint_as_float(o[i])));
+                        o[i + 1] = __float_as_uint(fmaf(x.y, f, __uint_as_float(o[i + 1])));
+                        o[i + 2] = __float_as_uint(fmaf(x.z, f, __uint_as_float(o[i + 2])));
+                        o[i + 3] = __float_as_uint(fmaf(x.w, f, __uint_as_float(o[i + 3])));
+                    }
+                }
                 __syncwarp();
                 if (!live) {
                 } else if (P.splits > 1) {
 #pragma unroll
                     for (int i = 0; i < 32; i += 4)
-                        *reinterpret_cast<uint4*>(P.part_o + slot * HD + c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                        *reinterpret_cast<uint4*>(part + c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
                 } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
                     for (int i = 0; i < 32; i += 4)
@@ -1227,7 +1283,7 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4).rt + 5),
 #pragma unroll
                 for (uint32_t k = 0; k < NP / 16; ++k)
                     mma_ts(d, pw + x * (NP / 2) + 8 * k, swizzled_desc(vb + k * 2048, NP * 128), bf16_idesc(HD),
-                           j > 0 || x > 0 || k > 0);
+                           j % G || x > 0 || k > 0);
             mma_commit(&o_done[rt][j % nsb]);
             mma_commit(&v_empty[st]);
         }
@@ -1247,7 +1303,7 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4).rt + 5),
 struct Shape {
     uint32_t group, row_tiles, tile_rows, chunk, splits;
     bool tiles;      // the prompt kernel
-    uint64_t slots;  // partials
+    uint64_t slots;  // partials in the workspace (0: none)
 };
 Shape shape_of(const Kv8Cache& c, const Kv8Batch& b, uint32_t heads, uint32_t type, int sms) {
     Shape r;
@@ -1269,8 +1325,11 @@ Shape shape_of(const Kv8Cache& c, const Kv8Batch& b, uint32_t heads, uint32_t ty
     const uint64_t want = std::max<uint64_t>(1, (r.tiles ? 1ull : c.head_dim == 256 && r.row_tiles == 1 ? 2ull : 3ull) * sms / std::max<uint64_t>(1, tiles));
     r.chunk = std::max(8u, (uint32_t)((blocks + want - 1) / want));
     r.chunk = (r.chunk + 3) / 4 * 4;
+    if (!r.tiles && !f32) r.chunk = std::min(r.chunk, kSumBlocks * kWarps);
     r.splits = (blocks + r.chunk - 1) / r.chunk;
-    r.slots = tiles * r.splits;
+    // (one chunk: only for sums that leave tensor memory)
+    const bool sums = r.tiles && std::min(r.chunk, blocks) * 16 > sum_steps(role.np, f32) * role.np;
+    r.slots = r.splits > 1 || sums ? tiles * r.splits : 0;
     return r;
 }
 
@@ -1315,7 +1374,7 @@ template <class T> cudaError_t by_dim(const Plan& p, bool tiles, cudaStream_t s)
 
 uint64_t kv8_attention_ws_bytes(const Kv8Cache& c, const Kv8Batch& b, uint32_t heads, uint32_t type, int sms) {
     const Shape sh = shape_of(c, b, heads, type, sms);
-    return sh.splits == 1 ? 0 : sh.slots * sh.tile_rows * (c.head_dim + 2) * 4;
+    return sh.slots * sh.tile_rows * (c.head_dim + 2) * 4;
 }
 
 cudaError_t launch_kv8_attention(const Kv8AttnArgs& a, int sms, cudaStream_t s) {

@@ -200,3 +200,21 @@ def test_attention_block_that_is_not_finite_far_below_the_maximum(tokens, kind, 
         got = host(_attend(kv, [last], [tokens], q, kind))
         see = last - 48
         assert np.isfinite(got[:tokens - see]).all() and not np.isfinite(got[tokens - see:]).any()
+
+
+# ------------------------------------------------------------------ long sums
+@KERNELS
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim,n", [(64, 30001), (128, 30001), (256, 30001), (128, 5000), (64, 70001)])
+def test_attention_values_of_one_sign_over_many_positions(tokens, kind, dim, n):
+    """Sums that only grow: a cut instead of a rounding at each addition would show as a bias with the length."""
+    import tests.test_gpu_int8 as t
+    t._EMPTY[0] = 1800  # (many sequences: one chunk of positions per row)
+    rng = np.random.default_rng(dim)
+    kv = Kv(rng, 1, dim, 64, [n])
+    sign, level, x = _levels(rng, n, dim, 1, 90, 128)
+    v = rng.integers(64, 128, (n, dim))
+    blocks = -(-n // 16)
+    _put(kv, level[:, None] * sign, v, np.full(blocks, 1 / 40, np.float32), np.full(blocks, 1 / 40, np.float32))
+    q = dev(np.tile(x, (tokens, 4, 1)).astype(np.float32), kind)
+    _compare(kv, n, tokens, q, kind)
