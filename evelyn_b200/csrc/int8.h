@@ -40,6 +40,9 @@ struct I8GemmArgs {
     int32_t* err = nullptr;     // optional
 };
 cudaError_t launch_i8_gemm(const I8GemmArgs& a, int sms, cudaStream_t s);
+// How that launch cuts the product on the current device: tokens of a tile (0: CTA pairs, 256 x 256) and CTAs that share
+// its K. By rows, out, cols, type and whether there is an addition.
+void i8_gemm_cut(const I8GemmArgs& a, int sms, uint32_t& tokens, uint32_t& split);
 
 // ---------------------------------------------------------------- kv8_append.cu, kv8_attention.cu
 struct Kv8Cache {

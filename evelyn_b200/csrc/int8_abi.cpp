@@ -203,6 +203,25 @@ evl_status evl_i8_matmul(const int8_t* d_x, uint64_t x_stride, const float* d_x_
     });
 }
 
+// Not part of the public surface: how evl_i8_matmul cuts a product on the current device, so that the tests can
+// see that their shapes reach every kernel (the rule is a fitted estimate).
+evl_status evl_internal_i8_cut(uint32_t rows, uint32_t out, uint32_t cols, uint32_t type, uint32_t add, uint32_t* tokens,
+                               uint32_t* split) {
+    return guarded([&] {
+        elem_bytes(type);
+        require(rows && out && cols && tokens && split, "null argument");
+        int dev = 0;
+        cuda_check(cudaGetDevice(&dev), "cudaGetDevice");
+        I8GemmArgs a;
+        a.rows = rows;
+        a.out = out;
+        a.cols = cols;
+        a.type = type;
+        a.add = add ? tokens : nullptr;  // (only whether there is one)
+        i8_gemm_cut(a, sm_count(dev), *tokens, *split);
+    });
+}
+
 evl_status evl_kv8_append(const evl_kv8_cache* cache, const evl_kv8_batch* batch, const evl_kv8_prep* prep,
                           uint32_t type, const void* d_k, uint64_t k_stride, const void* d_v, uint64_t v_stride,
                           const void* d_q, uint64_t q_stride, uint32_t heads, void* d_q_out, uint64_t q_out_stride,

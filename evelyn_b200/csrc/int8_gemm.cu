@@ -668,7 +668,7 @@ template <class T> cudaError_t launch_pair(Plan& p, int sms, cudaStream_t s) {
     return go<i8_gemm_pair_kernel<T>>(p, grid, kPairThreads, kPairStages * kPairStage + 1024, 2, s);
 }
 
-template <class T> cudaError_t by_tokens(Plan& p, int sms, cudaStream_t s) {
+template <class T> Cut cut_for(Plan& p, int sms) {
     p.slices = (p.a.cols + kSlice - 1) / kSlice;
     Cut best;
     consider<16, T>(best, p, sms);
@@ -679,8 +679,13 @@ template <class T> cudaError_t by_tokens(Plan& p, int sms, cudaStream_t s) {
     if (p.a.rows > 128) {
         const uint64_t tiles = (uint64_t)((p.a.out + 255) / 256) * ((p.a.rows + 255) / 256);
         const double c = cost_of(0, tiles, 1, p.slices, p.a.add != nullptr, sms);
-        if (c < best.cost) best.nt = 0, best.cost = c;
+        if (c < best.cost) best.nt = 0, best.split = 1, best.cost = c;
     }
+    return best;
+}
+
+template <class T> cudaError_t by_tokens(Plan& p, int sms, cudaStream_t s) {
+    const Cut best = cut_for<T>(p, sms);
     switch (best.nt) {
         case 0: return launch_pair<T>(p, sms, s);
         case 16: return launch<16, T>(p, best.split, sms, s);
@@ -702,6 +707,13 @@ cudaError_t launch_i8_gemm(const I8GemmArgs& a, int sms, cudaStream_t s) {
         case GGML_BF16: return by_tokens<__nv_bfloat16>(p, sms, s);
         default: return cudaErrorInvalidValue;
     }
+}
+
+void i8_gemm_cut(const I8GemmArgs& a, int sms, uint32_t& tokens, uint32_t& split) {
+    Plan p;
+    p.a = a;
+    const Cut c = a.type == GGML_F32 ? cut_for<float>(p, sms) : a.type == GGML_F16 ? cut_for<__half>(p, sms) : cut_for<__nv_bfloat16>(p, sms);
+    tokens = c.nt, split = c.split;
 }
 
 }  // namespace evl
