@@ -66,6 +66,11 @@ def _need(ok: bool, msg: str):
         raise EvelynError(1, msg)
 
 
+def _u32(what: str, *sizes: int):
+    """The C ABI's counts have 32 bits; a larger one must not arrive there as another."""
+    _need(all(n < 1 << 32 for n in sizes), f"{what} must be below 2^32")
+
+
 def _device_of(*tensors, known=()):
     """The device that all of them are on (None for objects that name none)."""
     found = {d for d in known if d is not None}
@@ -114,6 +119,7 @@ def quantize_rows(x, codes, scales, stream: int = 0) -> None:
         _device_of(x, codes, scales)
         kind, xs, cs = _kind(x), _rows(x, "x"), _rows(codes, "codes")
         rows, cols = x.shape
+        _u32("rows and cols", rows, cols)
         _named(codes, "int8", "codes")
         _need(tuple(codes.shape) == (rows, cols), "codes must have the shape of x")
         _flat(scales, rows, "float32", "scales")
@@ -134,6 +140,7 @@ def matmul(x, x_scales, w, w_scales, y, add=None, err=None, stream: int = 0) -> 
         kind, xst, wst, yst = _kind(y), _rows(x, "x"), _rows(w, "w"), _rows(y, "y")
         rows, cols = x.shape
         out = w.shape[0]
+        _u32("rows, out and cols", rows, out, cols)
         _named(x, "int8", "x")
         _named(w, "int8", "w")
         _need(w.shape[1] == cols, "x and w must have the same number of columns")
@@ -160,6 +167,7 @@ class Kv8Cache:
     def __init__(self, k, v, k_scales, v_scales):
         stride, sstride = _rows(k, "k", 4), _rows(k_scales, "k_scales", 3)
         pages, heads, page, dim = k.shape
+        _u32("the cache's dimensions", pages, heads, page, dim)
         _need(tuple(v.shape) == tuple(k.shape) and _rows(v, "v", 4) == stride, "k and v must have one layout")
         _need(tuple(k_scales.shape) == (pages, heads, page // 16) and tuple(v_scales.shape) == tuple(k_scales.shape)
               and _rows(v_scales, "v_scales", 3) == sstride, "scales must be [pages][kv heads][page size / 16]")
@@ -187,6 +195,7 @@ class Kv8Batch:
         _flat(cu, n + 1, "int32", "cu")
         _flat(lens, n, "int32", "lens")
         _need(max_new >= 0 and max_len >= 0, "max_new and max_len must not be negative")
+        _u32("sequences, max_new, max_len and the page table's stride", n, max_new, max_len, tstride)
         # a table row holds as many entries as its shape says, whatever the stride
         _need(page_table.shape[1] == tstride or n <= 1 or page_table.shape[1] <= tstride, "page_table rows overlap")
         self.n_seqs, self.max_new, self.max_len = n, int(max_new), int(max_len)
@@ -210,6 +219,7 @@ class Kv8Batch:
 def _heads(t, total: int, dim: int, what: str) -> tuple[int, int]:
     stride = _rows(t, what, 3)
     _need(t.shape[0] == total and t.shape[2] == dim, f"{what} must be [{total}][heads][{dim}]")
+    _u32(f"{what}'s tokens and heads", total, t.shape[1])
     return t.shape[1], stride
 
 
@@ -251,6 +261,7 @@ def _append_plan(cache, k, v, q, q_out, rope, q_norm, k_norm):
         _named(rope, "float32", "rope")
         _need(len(rope.shape) == 3 and rope.shape[2] == 2, "rope must be [positions][rope dim / 2][2]")
         rl, rd = rope.shape[0], 2 * rope.shape[1]
+        _u32("rope's dimensions", rl, rd)
         _need(_rows(rope, "rope", 3) == rd, "rope must be contiguous")
     for t, what in ((q_norm, "q_norm"), (k_norm, "k_norm")):
         if t is not None:
@@ -261,6 +272,7 @@ def _append_plan(cache, k, v, q, q_out, rope, q_norm, k_norm):
 def kv8_attention_workspace(cache: Kv8Cache, batch: Kv8Batch, q) -> int:
     """Bytes of workspace that kv8_attention needs for queries of q's shape (may be 0)."""
     n = C.c_size_t()
+    _u32("q's tokens and heads", q.shape[0], q.shape[1])
     _check(runtime.lib().evl_kv8_attention_workspace_bytes(cache._ref, batch._of(q.shape[0], cache.page_size),
                                                            _kind(q), q.shape[1], C.byref(n)))
     return int(n.value)

@@ -1,0 +1,26 @@
+"""More calls of the 8-bit serving operators that are refused before anything is launched (no GPU needed)."""
+import pytest
+
+from evelyn_b200 import int8
+from tests.test_int8_args import Fake, _batch, _kv, _rows, refused
+
+FAR = 1 << 32
+
+
+def test_sizes_that_do_not_fit_32_bits():
+    """The C ABI takes them in 32 bits: cut to those they would pass every check as small sizes."""
+    bad = lambda fn, *a, **k: refused("InvalidInput", "2^32", fn, *a, **k)  # noqa: E731
+    bad(int8.quantize_rows, Fake((1, FAR + 64)), Fake((1, FAR + 64), "int8"), Fake((1,)))
+    bad(int8.quantize_rows, Fake((FAR + 1, 32)), Fake((FAR + 1, 32), "int8"), Fake((FAR + 1,)))
+    bad(int8.matmul, Fake((2, 32), "int8"), Fake((2,)), Fake((FAR + 8, 32), "int8"), Fake((FAR + 8,)), Fake((2, FAR + 8)))
+    bad(int8.matmul, Fake((FAR + 2, 32), "int8"), Fake((FAR + 2,)), Fake((8, 32), "int8"), Fake((8,)), Fake((FAR + 2, 8)))
+    bad(int8.matmul, Fake((2, FAR + 32), "int8"), Fake((2,)), Fake((8, FAR + 32), "int8"), Fake((8,)), Fake((2, 8)))
+    bad(_kv, pages=FAR + 4)
+    bad(_kv, heads=FAR + 2)
+    bad(_batch, max_new=FAR + 1)
+    bad(_batch, width=FAR + 4, max_len=FAR + 1)
+    bad(int8.Kv8Batch, Fake((2, 4), "int32", stride=(FAR + 4, 1)), Fake((3,), "int32"), Fake((2,), "int32"), 2, 64)
+    bad(int8.kv8_append, _kv(), _batch(), _rows(), _rows(), q=_rows(heads=FAR + 2), q_out=_rows(heads=FAR + 2))
+    bad(int8.kv8_append, _kv(), _batch(), _rows(), _rows(), rope=Fake((FAR + 64, 32, 2)))
+    bad(int8.kv8_attention, _kv(), _batch(), _rows(heads=FAR + 2), _rows(heads=FAR + 2))
+    bad(int8.kv8_attention_workspace, _kv(), _batch(), _rows(heads=FAR + 2))
