@@ -259,7 +259,8 @@ def _append_plan(cache, k, v, q, q_out, rope, q_norm, k_norm):
         _need(oh == heads and q.dtype == k.dtype and q_out.dtype == k.dtype, "q and q_out must have one shape and k's type")
     if rope is not None:
         _named(rope, "float32", "rope")
-        _need(len(rope.shape) == 3 and rope.shape[2] == 2, "rope must be [positions][rope dim / 2][2]")
+        _need(len(rope.shape) == 3 and rope.shape[2] == 2 and rope.shape[0] > 0,
+              "rope must be [positions][rope dim / 2][2]")
         rl, rd = rope.shape[0], 2 * rope.shape[1]
         _u32("rope's dimensions", rl, rd)
         _need(_rows(rope, "rope", 3) == rd, "rope must be contiguous")

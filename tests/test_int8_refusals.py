@@ -24,3 +24,8 @@ def test_sizes_that_do_not_fit_32_bits():
     bad(int8.kv8_append, _kv(), _batch(), _rows(), _rows(), rope=Fake((FAR + 64, 32, 2)))
     bad(int8.kv8_attention, _kv(), _batch(), _rows(heads=FAR + 2), _rows(heads=FAR + 2))
     bad(int8.kv8_attention_workspace, _kv(), _batch(), _rows(heads=FAR + 2))
+
+
+def test_a_rope_table_without_positions():
+    """Its address is null, which the C ABI takes for no rotation at all."""
+    refused("InvalidInput", "rope", int8.kv8_append, _kv(), _batch(), _rows(), _rows(), rope=Fake((0, 32, 2), at=0))
