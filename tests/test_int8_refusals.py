@@ -29,3 +29,9 @@ def test_sizes_that_do_not_fit_32_bits():
 def test_a_rope_table_without_positions():
     """Its address is null, which the C ABI takes for no rotation at all."""
     refused("InvalidInput", "rope", int8.kv8_append, _kv(), _batch(), _rows(), _rows(), rope=Fake((0, 32, 2), at=0))
+
+
+@pytest.mark.parametrize("scale", [1e-60, -1e-60, 1e-40, float("nan")])
+def test_a_scale_that_f32_does_not_hold(scale):
+    """Rounded to 0 it would stand for 1 / sqrt(head dim)."""
+    refused("InvalidInput", "scale", int8.kv8_attention, _kv(), _batch(), _rows(heads=4), _rows(heads=4), scale=scale)
