@@ -284,7 +284,7 @@ def kv8_attention(cache: Kv8Cache, batch: Kv8Batch, q, out, scale: float = 0.0, 
     """out [tokens][heads][head dim] = attention of q over the cache, each token up to its own
     position (evl_kv8_attention); scale 0 is 1 / sqrt(head dim). workspace: a device buffer of
     kv8_attention_workspace bytes, 256-byte aligned."""
-    _need(scale == 0 or abs(scale) >= 2.0 ** -126, "scale must be finite and 0 or a normal f32 number")
+    _need(scale == 0 or abs(scale) > 2.0 ** -150, "scale must be finite and 0 or a number that f32 holds")
     key = ("attention", cache.head_dim, cache._device, batch._device, _layout(q, out, workspace, err))
     plan = _plans.get(key)
     if plan is None:

@@ -1,7 +1,7 @@
 """More calls of the 8-bit serving operators that are refused before anything is launched (no GPU needed)."""
 import pytest
 
-from evelyn_b200 import int8
+from evelyn_b200 import EvelynError, int8
 from tests.test_int8_args import Fake, _batch, _kv, _rows, refused
 
 FAR = 1 << 32
@@ -31,7 +31,15 @@ def test_a_rope_table_without_positions():
     refused("InvalidInput", "rope", int8.kv8_append, _kv(), _batch(), _rows(), _rows(), rope=Fake((0, 32, 2), at=0))
 
 
-@pytest.mark.parametrize("scale", [1e-60, -1e-60, 1e-40, float("nan")])
+@pytest.mark.parametrize("scale", [1e-60, -1e-60, 2.0 ** -150, float("nan")])
 def test_a_scale_that_f32_does_not_hold(scale):
     """Rounded to 0 it would stand for 1 / sqrt(head dim)."""
     refused("InvalidInput", "scale", int8.kv8_attention, _kv(), _batch(), _rows(heads=4), _rows(heads=4), scale=scale)
+
+
+def test_the_smallest_scales_that_f32_holds_are_taken():
+    """(up to the device: the arguments themselves are fine)"""
+    for scale in (1e-40, -1.4e-45):
+        with pytest.raises(EvelynError) as e:
+            int8.kv8_attention(_kv(), _batch(), _rows(heads=4), _rows(heads=4), scale=scale)
+        assert "scale" not in str(e.value)
