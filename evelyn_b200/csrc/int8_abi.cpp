@@ -133,6 +133,13 @@ void check_rows(const void* p, uint64_t stride, uint64_t width, uint64_t es, con
     if (stride < width || stride > (1ull << 40)) raise(EVL_ERR_INVALID_INPUT, w + ": the stride does not hold a token's heads");
 }
 
+// Whether two blocks of rows [rows][width], `stride` bytes apart in both (a single row has none), share memory.
+bool share_memory(const void* a, const void* b, uint64_t rows, uint64_t width, uint64_t stride) {
+    const uint64_t p = reinterpret_cast<uintptr_t>(a), q = reinterpret_cast<uintptr_t>(b), d = p < q ? q - p : p - q;
+    if (d >= (rows - 1) * stride + width) return false;
+    return rows == 1 || d % stride < width || stride - d % stride < width;
+}
+
 }  // namespace
 
 extern "C" {
@@ -182,6 +189,10 @@ evl_status evl_i8_matmul(const int8_t* d_x, uint64_t x_stride, const float* d_x_
         require(y_stride >= out && y_stride <= (1ull << 40) && (!d_add || (add_stride >= out && add_stride <= (1ull << 40))),
                 "strides of y and add must hold a row");
         require(d_add != d_y || add_stride == y_stride, "add in place needs the stride of y");
+        // (an output is written as soon as its own addition is read; blocks of different strides are not looked into)
+        require(!d_add || d_add == d_y || (rows > 1 && add_stride != y_stride) ||
+                    !share_memory(d_add, d_y, rows, out * es, y_stride * es),
+                "add may be y, but must not overlap it otherwise");
         OnDeviceOf on(d_x);
         I8GemmArgs a;
         a.x = d_x;

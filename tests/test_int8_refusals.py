@@ -43,3 +43,26 @@ def test_the_smallest_scales_that_f32_holds_are_taken():
         with pytest.raises(EvelynError) as e:
             int8.kv8_attention(_kv(), _batch(), _rows(heads=4), _rows(heads=4), scale=scale)
         assert "scale" not in str(e.value)
+
+
+def _product(add_at, y_at=1 << 20, rows=4, out=8, add_stride=24, y_stride=24, kind="float32"):
+    int8.matmul(Fake((rows, 32), "int8"), Fake((rows,)), Fake((out, 32), "int8"), Fake((out,)),
+                Fake((rows, out), kind, stride=(y_stride, 1), at=y_at),
+                add=Fake((rows, out), kind, stride=(add_stride, 1), at=add_at))
+
+
+@pytest.mark.parametrize("off", [-7, -1, 1, 7, 17, 23, 24, 25, -24, 72, 79, -72, -79])
+def test_additions_that_overlap_other_outputs(off):
+    refused("InvalidInput", "overlap", _product, (1 << 20) + 4 * off)
+
+
+def test_an_addition_that_overlaps_a_single_row():
+    refused("InvalidInput", "overlap", _product, (1 << 20) + 28, rows=1, add_stride=400)
+
+
+@pytest.mark.parametrize("off", [8, 12, 16, -8, -16, 80, 100, -80, 32, 88])
+def test_additions_beside_the_outputs_are_taken(off):
+    """(up to the device) other columns of the same buffer, or memory apart"""
+    with pytest.raises(EvelynError) as e:
+        _product((1 << 20) + 4 * off)
+    assert "overlap" not in str(e.value)
