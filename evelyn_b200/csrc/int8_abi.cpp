@@ -274,6 +274,9 @@ evl_status evl_kv8_append(const evl_kv8_cache* cache, const evl_kv8_batch* batch
             check_rows(d_q, q_stride, (uint64_t)heads * a.c.head_dim, es, "q");
             check_rows(d_q_out, q_out_stride, (uint64_t)heads * a.c.head_dim, es, "q_out");
             require(d_q != d_q_out || q_stride == q_out_stride, "q made ready in place needs one stride");
+            require(d_q == d_q_out || q_stride != q_out_stride ||
+                        !share_memory(d_q, d_q_out, a.b.total, (uint64_t)heads * a.c.head_dim * es, q_stride * es),
+                    "q_out may be q, but must not overlap it otherwise");
             a.heads = heads;
             a.q = d_q;
             a.q_out = d_q_out;

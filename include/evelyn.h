@@ -347,7 +347,7 @@ typedef struct evl_kv8_prep {
 /* Appends the batch's new keys and values (d_k, d_v [total][kv_heads][head_dim] of `type`,
  * tokens k_stride / v_stride elements apart) to the cache, keys made ready by `prep` (NULL: as
  * they are), and makes the queries ready on the way: d_q [total][heads][head_dim], tokens
- * q_stride apart, to d_q_out (d_q NULL: none; d_q_out may be d_q with the same stride). A block's
+ * q_stride apart, to d_q_out (d_q NULL: none; d_q_out may be d_q with the same stride, no other overlap). A block's
  * scale is the largest of its values / 127 since its first position was written: when new
  * tokens raise it, the codes of the block's earlier positions move to the new scale,
  * rint(c * (s_old / s_new)). Rows of the block behind the sequence's last token are left as

@@ -66,3 +66,17 @@ def test_additions_beside_the_outputs_are_taken(off):
     with pytest.raises(EvelynError) as e:
         _product((1 << 20) + 4 * off)
     assert "overlap" not in str(e.value)
+
+
+@pytest.mark.parametrize("off", [-16, 16, 64, 512, -512])
+def test_queries_made_ready_over_other_queries(off):
+    """d_q_out may be d_q itself; shifted by less than a row, one warp would write what another has yet to read."""
+    q, o = (_rows(heads=4, stride=(512, 64, 1), at=at) for at in (1 << 20, (1 << 20) + 4 * off))
+    refused("InvalidInput", "overlap", int8.kv8_append, _kv(), _batch(), _rows(), _rows(), q=q, q_out=o)
+
+
+def test_queries_made_ready_beside_the_others_are_taken():
+    with pytest.raises(EvelynError) as e:
+        q, o = (_rows(heads=4, stride=(512, 64, 1), at=at) for at in (1 << 20, (1 << 20) + 4 * 256))
+        int8.kv8_append(_kv(), _batch(), _rows(), _rows(), q=q, q_out=o)
+    assert "overlap" not in str(e.value)
