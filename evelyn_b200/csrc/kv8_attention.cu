@@ -10,7 +10,7 @@
 // The codes meet w * sv in bf16 parts: codes of 8 bits are exact in bf16, and its exponents are f32's, so
 // a weight keeps its bits however far below the maximum it lies (a head that puts nearly all weight on
 // one position of value 0 is made of such weights; in f16 parts they were gone from 16 nats on). Three parts
-// hold an f32 product exactly (f32 outputs), two 16 bits of it, off by at most 2^-15 (16-bit outputs). Value
+// hold an f32 product exactly (f32 outputs), two are off by at most 2^-16 of it (16-bit outputs). Value
 // scales near the ends of f32's range (below 2^-60, above 2^80) move the maximum that their positions
 // ask for, so that their products stay inside (lift_of()).
 //
@@ -101,19 +101,18 @@ __device__ __forceinline__ uint32_t codes_b2(uint32_t w, uint32_t sel) {
     const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
     return *reinterpret_cast<const uint32_t*>(&r);
 }
-// A pair of products as PARTS bf16 pairs: the upper half of each f32's bits, then those of what remains (exact
-// differences), the last of two parts rounded to nearest.
+// A pair of products as PARTS bf16 pairs. Two: each rounded to nearest. Three: the upper half of each f32's bits, of what
+// remains, and the rest (differences and the last part are exact).
 template <int PARTS> __device__ __forceinline__ void split_b2(float a, float b, uint32_t (&part)[PARTS]) {
 #pragma unroll
     for (int i = 0; i < PARTS; ++i) {
-        if (PARTS == 2 && i == 1) {
+        if constexpr (PARTS == 2) {
             const __nv_bfloat162 r = __floats2bfloat162_rn(a, b);
             part[i] = *reinterpret_cast<const uint32_t*>(&r);
         } else {
-            const uint32_t x = __float_as_uint(a), y = __float_as_uint(b);
-            part[i] = __byte_perm(x, y, 0x7632);
-            if (i + 1 < PARTS) a -= __uint_as_float(x & 0xffff0000u), b -= __uint_as_float(y & 0xffff0000u);
+            part[i] = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
         }
+        if (i + 1 < PARTS) a -= __uint_as_float(part[i] << 16), b -= __uint_as_float(part[i] & 0xffff0000u);
     }
 }
 __device__ __forceinline__ uint32_t pack_h2(float a, float b) {
@@ -967,26 +966,28 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4).rt + 5),
             // without looking for the maximum: their sum tells whether one passes it by far (or is
             // not a number), and then the scores are read again below.
             if (!F32 && j > 0 && !masked && !__any_sync(0xffffffffu, rare)) {
-                uint32_t v[NP];
+                uint32_t hi[NP / 2], lo[NP / 2], v[2][16];
                 float add = 0.f;
-                tmem_ld16(ts, *reinterpret_cast<uint32_t(*)[16]>(v));
+                tmem_ld16(ts, v[0]);
                 tmem_ld_wait();
 #pragma unroll
                 for (uint32_t b = 0; b < NB; ++b) {  // the next block's scores on their way meanwhile
-                    if (b + 1 < NB) tmem_ld16(ts + 16 * (b + 1), *reinterpret_cast<uint32_t(*)[16]>(v + 16 * (b + 1)));
+                    if (b + 1 < NB) tmem_ld16(ts + 16 * (b + 1), v[(b + 1) & 1]);
+                    const uint32_t(&x)[16] = v[b & 1];
                     const uint64_t ff = pack2(f[b], f[b]), off = pack2(e[b] - M, e[b] - M);
                     uint64_t sum = 0;
 #pragma unroll
-                    for (uint32_t i = 16 * b; i < 16 * b + 16; i += 2) {
-                        const uint64_t y = fma2(pack2(v[i], v[i + 1]), ff, off);
+                    for (uint32_t i = 0; i < 8; ++i) {
+                        const uint64_t y = fma2(pack2(x[2 * i], x[2 * i + 1]), ff, off);
                         const float w0 = exp2_fast(lo2(y)), w1 = exp2_fast(hi2(y));
                         sum = add2(sum, pack2(w0, w1));
-                        // (split_b2, the differences of a pair in one addition; the parts take the scores' registers)
-                        const uint32_t a0 = __float_as_uint(w0), a1 = __float_as_uint(w1);
-                        const uint64_t left = add2(pack2(a0, a1), pack2((a0 & 0xffff0000u) ^ 0x80000000u, (a1 & 0xffff0000u) ^ 0x80000000u));
+                        // (split_b2, the differences of a pair in one operation)
+                        const __nv_bfloat162 h = __floats2bfloat162_rn(w0, w1);
+                        const uint32_t hb = *reinterpret_cast<const uint32_t*>(&h);
+                        const uint64_t left = fma2(pack2(hb << 16, hb & 0xffff0000u), pack2(-1.f, -1.f), pack2(w0, w1));
                         const __nv_bfloat162 r = __floats2bfloat162_rn(lo2(left), hi2(left));
-                        v[i] = __byte_perm(a0, a1, 0x7632);
-                        v[i + 1] = *reinterpret_cast<const uint32_t*>(&r);
+                        hi[8 * b + i] = hb;
+                        lo[8 * b + i] = *reinterpret_cast<const uint32_t*>(&r);
                     }
                     add = fmaf(lo2(sum) + hi2(sum), down[b], add);
                     if (b + 1 < NB) tmem_ld_wait();
@@ -995,11 +996,8 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4).rt + 5),
                     l += add;
 #pragma unroll
                     for (uint32_t b = 0; b < NB; ++b) {
-                        uint32_t hi[8], lo[8];
-#pragma unroll
-                        for (uint32_t i = 0; i < 8; ++i) hi[i] = v[16 * b + 2 * i], lo[i] = v[16 * b + 2 * i + 1];
-                        tmem_st8(ts + 8 * b, hi);
-                        tmem_st8(ts + NP / 2 + 8 * b, lo);
+                        tmem_st8(ts + 8 * b, hi + 8 * b);
+                        tmem_st8(ts + NP / 2 + 8 * b, lo + 8 * b);
                     }
                     done();
                     continue;

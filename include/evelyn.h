@@ -373,7 +373,7 @@ evl_status evl_kv8_attention_workspace_bytes(const evl_kv8_cache* cache, const e
  * magnitude (not of its own), so beside a loud channel of q a score may be off by that times sum |k|; the 16-bit
  * types with many rows hold q exactly to 2^-34 of the largest and sum the products in f32, cut off by up to 2^-23 of
  * the terms' sizes after every 16 dims. Scores beyond 1e38 in magnitude are good for nothing. Weights keep f32's range, and 24 bits (16-bit types:
- * 15) however far they lie below the largest; their sums over the positions are off by a bounded number of cut-off additions (f32: 96 of
+ * 16) however far they lie below the largest; their sums over the positions are off by a bounded number of cut-off additions (f32: 96 of
  * at most 2^-23; 16-bit types: 1024) and otherwise rounded to nearest, whatever the length. Rows of d_out that belong to no sequence are left as they were. One kernel serves all
  * sequences of a call, chosen by max_new: a batch that mixes prompts with single tokens gives
  * the same sums but is faster as two calls. d_workspace: evl_kv8_attention_workspace_bytes, 256-byte aligned, needing no initial
