@@ -56,8 +56,9 @@ struct Plan {
     uint32_t chunk;      // blocks of 16 positions per split
     uint32_t splits;
     uint32_t tile_rows;  // rows of a tile: kRows, or those of the prompt kernel
-    float* part_o;       // [sequence][kv head][row tile][split][tile_rows][head_dim]; also where sums of long chunks stand
+    float* part_o;       // [sequence][kv head][row tile][split][tile_rows][head_dim]
     float2* part_ml;     // same without head_dim: (M, l)
+    float4* sums;        // of long chunks: [sequence][kv head][row tile][split][128 rows at a time][head_dim / 4][128]
 };
 
 __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -900,9 +901,10 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4).rt + 5),
         // no row of this warp hides a position before this one
         const int32_t open = sp.base + min(r0 + (int32_t)(rt * kTileRows + quad * 32), rows - 1) / (int32_t)P.group;
         const uint32_t to = tm + rt * kTileCols + ((quad * 32) << 16);  // O, then the score buffers
-        const uint64_t slot = ((((uint64_t)s * a.c.kv_heads + h) * P.row_tiles + tile) * P.splits + split) * P.tile_rows +
-                              rt * kTileRows + lr;
-        float* part = P.part_o + slot * HD;
+        const uint64_t place = ((((uint64_t)s * a.c.kv_heads + h) * P.row_tiles + tile) * P.splits + split) * RT + rt;
+        // (a warp's rows side by side: with a row's values side by side each access touched 32 lines, 283 us against 231
+        // for 300 tokens over 4000 positions of 2 sequences, 256 dims)
+        float4* sums = P.sums + place * (HD / 4 * kTileRows) + lr;
         float M = kNegBig, l = 0.f, Msum = 0.f;  // Msum: the maximum under which the sum in the workspace stands
         bool ok = true;
         for (uint32_t j = 0; j < steps && ok; ++j) {
@@ -924,29 +926,31 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4).rt + 5),
                 done();
                 continue;
             }
-            if (j && j % G == 0) {
+            if (j && j % G == 0) {  // (rows past the last one have their places in the workspace too)
+                float4 x[2][8];
+                auto fetch = [&](uint32_t c) {
+#pragma unroll
+                    for (uint32_t i = 0; i < 8; ++i) x[c & 1][i] = sums[(8 * c + i) * kTileRows];
+                };
+                fetch(0);
                 ok = warp_wait(&o_done[rt][(j - 1) % nsb], ((j - 1) >> lsb) & 1, &abort_flag);
                 if (!ok) break;
                 tc_after();
+                const bool first = j == G;
                 const float f = exp2_fast(Msum - M);
-#pragma unroll 1
-                for (uint32_t c = 0; c < HD; c += 16) {
-                    uint32_t o[16];
-                    tmem_ld16(to + c, o);
-                    tmem_ld_wait();
-                    if (live) {
 #pragma unroll
-                        for (int i = 0; i < 16; i += 4) {
-                            float4 y = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]), __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
-                            float4* at = reinterpret_cast<float4*>(part + c + i);
-                            if (j > G) {
-                                const float4 x = *at;
-                                y.x = fmaf(x.x, f, y.x), y.y = fmaf(x.y, f, y.y), y.z = fmaf(x.z, f, y.z), y.w = fmaf(x.w, f, y.w);
-                            }
-                            *at = y;
-                        }
+                for (uint32_t c = 0; c < HD / 32; ++c) {
+                    uint32_t o[32];
+                    tmem_ld32(to + 32 * c, o);
+                    if (c + 1 < HD / 32) fetch(c + 1);  // on their way meanwhile
+                    tmem_ld_wait();
+#pragma unroll
+                    for (uint32_t i = 0; i < 8; ++i) {
+                        const float4 y = x[c & 1][i];
+                        float4 z = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+                        if (!first) z = make_float4(fmaf(y.x, f, z.x), fmaf(y.y, f, z.y), fmaf(y.z, f, z.z), fmaf(y.w, f, z.w));
+                        sums[(8 * c + i) * kTileRows] = z;
                     }
-                    __syncwarp();
                 }
                 Msum = M;
             }
@@ -1092,6 +1096,7 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4).rt + 5),
         if (ok) {
             const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);  // a row that sees nothing: zeros
             T* out = static_cast<T*>(a.out) + (uint64_t)(sp.q0 + tok) * a.out_stride + (uint64_t)head * HD;
+            const uint64_t slot = place * kTileRows + lr;
             if (live && P.splits > 1) P.part_ml[slot] = make_float2(M, l);
             for (uint32_t c = 0; c < HD; c += 32) {
                 uint32_t o[32];
@@ -1102,11 +1107,11 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4).rt + 5),
 #pragma unroll
                     for (int i = 0; i < 32; ++i) o[i] = 0;
                 }
-                if (steps > G && live) {
+                if (steps > G) {
                     const float f = exp2_fast(Msum - M);
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4) {
-                        const float4 x = *reinterpret_cast<const float4*>(part + c + i);
+                    for (uint32_t i = 0; i < 32; i += 4) {
+                        const float4 x = sums[(c + i) / 4 * kTileRows];
                         o[i] = __float_as_uint(fmaf(x.x, f, __uint_as_float(o[i])));
                         o[i + 1] = __float_as_uint(fmaf(x.y, f, __uint_as_float(o[i + 1])));
                         o[i + 2] = __float_as_uint(fmaf(x.z, f, __uint_as_float(o[i + 2])));
@@ -1118,7 +1123,7 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4).rt + 5),
                 } else if (P.splits > 1) {
 #pragma unroll
                     for (int i = 0; i < 32; i += 4)
-                        *reinterpret_cast<uint4*>(part + c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                        *reinterpret_cast<uint4*>(P.part_o + slot * HD + c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
                 } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
                     for (int i = 0; i < 32; i += 4)
@@ -1301,7 +1306,7 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4).rt + 5),
 struct Shape {
     uint32_t group, row_tiles, tile_rows, chunk, splits;
     bool tiles;      // the prompt kernel
-    uint64_t slots;  // partials in the workspace (0: none)
+    uint64_t slots, sums;  // tiles with partials in the workspace (0: one chunk), with sums there (0: they stay in tensor memory)
 };
 Shape shape_of(const Kv8Cache& c, const Kv8Batch& b, uint32_t heads, uint32_t type, int sms) {
     Shape r;
@@ -1325,9 +1330,8 @@ Shape shape_of(const Kv8Cache& c, const Kv8Batch& b, uint32_t heads, uint32_t ty
     r.chunk = (r.chunk + 3) / 4 * 4;
     if (!r.tiles && !f32) r.chunk = std::min(r.chunk, kSumBlocks * kWarps);
     r.splits = (blocks + r.chunk - 1) / r.chunk;
-    // (one chunk: only for sums that leave tensor memory)
-    const bool sums = r.tiles && std::min(r.chunk, blocks) * 16 > sum_steps(role.np, f32) * role.np;
-    r.slots = r.splits > 1 || sums ? tiles * r.splits : 0;
+    r.slots = r.splits > 1 ? tiles * r.splits : 0;
+    r.sums = r.tiles && std::min(r.chunk, blocks) * 16 > sum_steps(role.np, f32) * role.np ? tiles * r.splits : 0;
     return r;
 }
 
@@ -1372,7 +1376,7 @@ template <class T> cudaError_t by_dim(const Plan& p, bool tiles, cudaStream_t s)
 
 uint64_t kv8_attention_ws_bytes(const Kv8Cache& c, const Kv8Batch& b, uint32_t heads, uint32_t type, int sms) {
     const Shape sh = shape_of(c, b, heads, type, sms);
-    return sh.slots * sh.tile_rows * (c.head_dim + 2) * 4;
+    return sh.slots * sh.tile_rows * (c.head_dim + 2) * 4 + sh.sums * sh.tile_rows * c.head_dim * 4;
 }
 
 cudaError_t launch_kv8_attention(const Kv8AttnArgs& a, int sms, cudaStream_t s) {
@@ -1388,6 +1392,7 @@ cudaError_t launch_kv8_attention(const Kv8AttnArgs& a, int sms, cudaStream_t s) 
     p.splits = sh.splits;
     p.part_o = reinterpret_cast<float*>(a.ws);
     p.part_ml = reinterpret_cast<float2*>(p.part_o + sh.slots * sh.tile_rows * a.c.head_dim);
+    p.sums = reinterpret_cast<float4*>(p.part_ml + sh.slots * sh.tile_rows);  // (tiles have 128 rows or 256: 16-byte aligned)
     switch (a.type) {
         case GGML_F32: return by_dim<float>(p, sh.tiles, s);
         case GGML_F16: return by_dim<__half>(p, sh.tiles, s);
