@@ -566,12 +566,13 @@ template <class T, int HD> __global__ void __launch_bounds__(32 * kJoinWarps) kv
 // step late (293 here, but 54 against 48 with one row tile), polynomials for some exponentials.
 constexpr uint32_t kTileRows = 128;
 // Rows per (sequence, kv head) from which it may be used, and the blocks of 16 positions times tiles of eight rows
-// that each warp of the other kernel would then have to take. Measured over 64 to 256 dims, 16 to 64
-// rows, 300 to 16000 positions of 1 to 64 sequences: 1.2 % over the better kernel's time on average, 26 % at
-// most; on either side of the rule, 32 rows over 4099 positions of 9 sequences with 2 kv heads of
-// 256 dims: 30 us against 51; 32 rows over 600 positions of 2 sequences with 8 of 128: 13.1 against 12.3.
-// (f32 up to 128 dims has one row tile and more products, and its rows pay later.)
-__host__ __device__ constexpr uint32_t tile_min(int hd, bool f32) { return f32 && hd <= 128 ? 48 : 24; }
+// that each warp of the other kernel would then have to take. Measured over 64 to 256 dims, bf16 and f32, 16 to 96
+// rows, 600 to 16000 positions of 1 to 32 sequences: 1.4 % over the better kernel's time on average, 34 % at
+// most; on either side of the rule, 32 rows over 4099 positions of 9 sequences with 8 kv heads of 128 dims,
+// bf16: 50 us against 60; 16 rows: 47 against 40; 32 rows over 600 positions of 2 sequences: 14.0 against 11.9.
+// (f32 has one row tile and more products, and its rows pay later: 48 rows over the 4099 positions 110 against 84, 64 rows 112
+// against 105.)
+__host__ __device__ constexpr uint32_t tile_min(bool f32) { return f32 ? 64 : 24; }
 constexpr uint64_t kTileWork = 3;
 
 // Steps whose products are added up in tensor memory. Its sums are cut off, not rounded, by up to 2^-23 at
@@ -1314,7 +1315,7 @@ Shape shape_of(const Kv8Cache& c, const Kv8Batch& b, uint32_t heads, uint32_t ty
     const bool f32 = type == GGML_F32;
     const uint64_t rows = (uint64_t)std::max(1u, b.max_new) * r.group;
     const uint32_t blocks = std::max(1u, (b.max_len + 15) / 16);
-    r.tiles = rows >= tile_min((int)c.head_dim, f32) &&
+    r.tiles = rows >= tile_min(f32) &&
               (double)b.n_seqs * c.kv_heads * blocks * ((rows + kRows - 1) / kRows) >= (double)kTileWork * 3 * kWarps * sms;
     const Role role = role_of((int)c.head_dim, f32);
     r.tile_rows = r.tiles ? role.rt * kTileRows : kRows;

@@ -11,8 +11,8 @@ from tests.test_gpu_int8 import KINDS, Kv, _attend, dev, host, width  # noqa: F4
 
 pytestmark = pytest.mark.gpu
 
-# (tokens of a sequence: one takes the token kernel, 12 beside many empty sequences the prompt kernel)
-KERNELS = pytest.mark.parametrize("tokens", [1, 12])
+# (tokens of a sequence: one takes the token kernel, 16 beside many empty sequences the prompt kernel)
+KERNELS = pytest.mark.parametrize("tokens", [1, 16])
 
 
 def _wide(tokens):
@@ -187,7 +187,7 @@ def test_attention_block_that_is_not_finite_far_below_the_maximum(tokens, kind, 
     no token that does not."""
     _wide(tokens)
     rng = np.random.default_rng(nats + dim)
-    n = 60
+    n = max(60, 48 + tokens)  # all tokens see the block
     kv = Kv(rng, 1, dim, 16, [n])
     sign, level, x = _levels(rng, n, dim, nats, 60, 67)
     level[2] = 127
