@@ -29,8 +29,11 @@
 //   33 tokens, 5120 x 25600, bf16, added     28 us   4.7 TB/s (71 % of a copy's rate)
 //   4096 tokens, 24576 x 4096, bf16         282 us   2920 TOP/s (tensor pipe busy 78 % of the cycles; 535 us with
 //                                                    128 x 256 tiles on single CTAs)
-// Every wait is bounded; on a timeout the CTA records DEV_ERR_WAIT_TIMEOUT, lets its copies and
-// MMAs land, frees its tensor memory and leaves.
+// Every wait on an mbarrier is bounded; on a timeout the CTA records DEV_ERR_WAIT_TIMEOUT, lets its copies and
+// MMAs land, frees its tensor memory and leaves. The allocation of tensor memory and the cluster's barriers have no
+// limit of their own: a CTA that holds tensor memory waits only for its cluster, whose CTAs start together, and
+// for the kernel before it in the stream, all of whose CTAs hold what they need by then; so one that waits
+// for the allocation waits for CTAs that come to their end.
 #include <cooperative_groups.h>
 #include <cuda.h>
 #include <cudaTypedefs.h>

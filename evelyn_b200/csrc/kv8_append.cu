@@ -14,10 +14,11 @@
 // pairs (NeoX rotation: dims 2u, 2u+1 and the same + rope_dim / 2; else four neighbours), so both
 // halves of a rotated pair sit in one lane. Query rows: a warp takes up to 512 / head_dim heads of up to eight
 // tokens in turn. Bound: HBM (each new value read once, one byte written). Measured: four
-// prompts of 5003 tokens, 16 heads and 4 kv heads of 256 dims, 94 us = 3.6 TB/s, 55 % of a copy's rate (the norm's
-// 64-bit sums and the rotation keep issue 60 % busy at 24 warps an SM; 296 us with a warp per row of
-// the cache, 127 before the next head's rows were loaded ahead); 32 tokens of a decode step 3.8 us,
-// a launch and one chain of dependent loads.
+// prompts of 5003 tokens, 16 heads and 4 kv heads of 256 dims, 94 us = 3.6 TB/s, 55 % of a copy's rate (no norm there; issue
+// 60 % busy at 24 warps an SM, and the 80 registers of three CTAs make the 256-dim kernels spill, 96 bytes stored and 272
+// loaded in this one; 296 us with a warp per row of the cache, 127 before the next head's rows were loaded ahead). The
+// same tokens with 32 and 8 heads of 128 dims, bf16, q and k normed, NeoX pairs: 165 us for 346 MB, 103 without
+// the norm: its sums in 64 bits. 32 tokens of a decode step 3.9 us, a launch and one chain of dependent loads.
 //
 // Norm: the sum of squares and its root are computed in 64 bits and rounded once, then x * r * w
 // in f32; rotation in f32, each product and sum rounded once. So codes and scales are the same

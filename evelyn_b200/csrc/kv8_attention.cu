@@ -17,24 +17,25 @@
 // Small-batch kernel (kv8_split_kernel): up to 8 rows (token, head) per CTA that share a kv head;
 // positions are the M dimension of the warp's products.
 //   K: mma.sync m16n8k32 on the codes as they are. q is fixed point in three signed 8-bit limbs
-//      (22 bits below the row's largest magnitude), the integer products are exact, so a score
-//      is as good as an f32 dot product. The K order inside the product is permuted so that a
+//      (22 bits below the row's largest magnitude, so beside a loud channel the small values of q
+//      keep fewer), the integer products are exact. The K order inside the product is permuted so that a
 //      lane's fragment is 16 neighbouring bytes of a row: the codes reach the tensor cores as they
 //      were copied, with no conversion.
-//   V: mma.sync m16n8k16 in bf16; for f32 a block's products are summed there and the blocks in registers, since
-//      the tensor cores' own sums are cut off (66.8 -> 74.5 us at 131071 positions, with the third part). A lane loads 16 neighbouring dims of four positions and pairs
-//      positions with byte permutes; the weights move to the other operand's layout by 8x8 transposes.
+//   V: mma.sync m16n8k16 in bf16. A lane loads 16 neighbouring dims of four positions and pairs positions
+//      with byte permutes; the weights move to the other operand's layout by 8x8 transposes. For f32 a
+//      block's products are summed there and the blocks in registers, since the tensor cores' own sums
+//      are cut off (with the third part 64.7 -> 67.6 us at 131071 positions).
 //   The maximum is raised only when a score passes it by 2^8, so most blocks cost one vote.
 // A warp takes every 4th block of the CTA's chunk of positions, the next blocks already on their way
 // into a ring of its own (asynchronous copies, each lane its own pieces: no barrier, no registers). The
 // warps' partials meet in shared memory; a sequence of more than one chunk leaves (O, M, l) in the workspace for
 // kv8_join_kernel.
 // Bound: HBM, (2 head_dim + 1/2) bytes per position and kv head. Measured (32 heads, 8 kv heads of 128 dims):
-// 131071 positions of one sequence, f32, 65 us = 4.1 TB/s, 62 % of a copy's rate; 32 sequences of up to
-// 2100, bf16, 32 us = 3.2 TB/s; 517 positions 7.4 us. What holds it: about 370 instructions a block and
-// warp, a quarter of them V's widening, issued by three warps a scheduler (issue 46 % busy, all waiting
-// in turn on the ring, the products and the exponentials), and about 4 us from a CTA's start to its first
-// product and from its last one to the join.
+// 131071 positions of one sequence, f32, 68 us = 4.0 TB/s, 61 % of a copy's rate; 32 sequences of up to
+// 2100, bf16, 34 us = 3.0 TB/s; 517 positions 7.9 us. What holds the long one: its instructions, a third of them
+// V's widening, issued by three warps a scheduler (issue 53 % busy, all waiting in turn on the ring, the
+// products and the exponentials); the 32 sequences: 256 CTAs of four warps, seven warps an SM, of which the longest
+// sequence's decide; all: about 4 us from a CTA's start to its first product and from its last one to the join.
 #include <algorithm>
 #include <atomic>
 
@@ -542,36 +543,39 @@ template <class T, int HD> __global__ void __launch_bounds__(32 * kJoinWarps) kv
 // tiles of 128 rows (token, head) of one (sequence, kv head) and walks the positions NP at a time:
 //   1 block warp      a lane per block looks its page up, copies its codes into a ring (one run of memory for
 //                     K and one for V: two bulk copies) and makes the factors of its scales;
-//   4 producer warps  codes to f16 (exact) into a ring of shared-memory stages, K and V alike:
-//                     64 dims x NP positions per 128-byte-swizzled panel. The score product reads
+//   4 producer warps  codes to f16 (K; f32: as they are) and bf16 (V), exactly, into a ring of shared-memory
+//                     stages: 64 dims x NP positions per 128-byte-swizzled panel. The score product reads
 //                     them K-major, the value product MN-major, so no transpose is made;
 //   RT MMA threads    one per row tile: S = q K^T into tensor memory (two to four buffers per row
 //                     tile, so the next scores are multiplied while this step's softmax runs),
 //                     O += P V with P read from tensor memory;
 //   4 softmax warps   per row tile, one row per thread: scores to registers, running maximum,
-//                     weights to f16 over the scores' own columns. O is rescaled (read, multiplied,
+//                     weights to bf16 parts over the scores' own columns. O is rescaled (read, multiplied,
 //                     written back) only when a score passes the row's maximum by 2^8.
 // 16-bit inputs: q is scaled by a power of two per row and held in f16, exactly down to 2^-24 (its largest just under
-// 2^10); the weights are two bf16 parts, with the value scale as an added log2 in their exponent. f32 inputs: q is fixed point in three
-// 8-bit limbs and the scores are integer products (kind::i8) of the codes as they are, summed exactly -- the f32 sums of
-// kind::f16 are cut off, not rounded, and over long sums that shows; the weights are three bf16 parts.
+// 2^10); the weights are two bf16 parts, with the value scale as an added log2 in their exponent. f32 inputs: q is fixed
+// point in three 8-bit limbs and the scores are integer products (kind::i8) of the codes as they are, summed exactly
+// -- the f32 sums of kind::f16 are cut off, not rounded, and over long sums that shows; the weights are three bf16 parts.
 // Bound: the tensor pipe and, close behind, shared memory: a step of 64 positions with two row tiles of 128 dims
-// is 1024 clocks of products, 1540 of shared-memory traffic (q is read again for every K panel, and
-// the codes pass it three times) and 1024 of exponentials on each scheduler. Measured (2048 tokens behind
-// 6144 positions, 32 heads, 8 kv heads of 128 dims, bf16): 297 us = 810 TFLOP/s, half of the bf16 rate; about
-// 2100 clocks a step, of which a softmax warp takes 1550 for its 64 columns; and 256 CTAs on 148 SMs
-// take two turns where 1.73 would do. 64 rows over 4099 positions of 8 sequences, 8 kv heads: 49 us.
-// Tried and slower: 128 positions a step with one score buffer (432 us, the chain of a tile's products and softmax
-// lies open), codes kept in registers instead of a ring (354), the store's end waited for one
-// step late (293 here, but 54 against 48 with one row tile), polynomials for some exponentials.
+// is 1536 clocks of products (512 of them the weights' second part), 1800 of shared-memory traffic (q is read again
+// for every K panel, the codes pass it three times, V once for each part) and 1024 of exponentials on each scheduler.
+// Measured (2048 tokens behind 6144 positions, 32 heads, 8 kv heads of 128 dims, bf16): 364 us = 660 TFLOP/s; the tensor
+// pipe of the busiest SM is active 69 % of the time, and 256 CTAs on 148 SMs take two turns where 1.73 would do. 64 rows
+// over 4099 positions of 8 sequences, 8 kv heads: 55 us; 512 f32 tokens over 4096 positions, 8 kv heads of 128: 182.
+// (One f16 part took 297, 48 and 120 us, without the range.) Parts left out to time the rest: without the second
+// product 3 us less, without its conversions 44, without both 79: softmax warps and products hold one another up.
+// Tried and slower: parts cut instead of rounded (380 us against 375), scalar operations instead of pairs (380), the
+// largest score looked for first so that parts can be stored at once (380); with one f16 part 128 positions a step with
+// one score buffer (432 against 316), codes kept in registers instead of a ring (354 against 331), the store's end
+// waited for one step late (293 against 297, but 54 against 48 with one row tile), polynomials for some exponentials.
 constexpr uint32_t kTileRows = 128;
 // Rows per (sequence, kv head) from which it may be used, and the blocks of 16 positions times tiles of eight rows
 // that each warp of the other kernel would then have to take. Measured over 64 to 256 dims, bf16 and f32, 16 to 96
 // rows, 600 to 16000 positions of 1 to 32 sequences: 1.4 % over the better kernel's time on average, 34 % at
 // most; on either side of the rule, 32 rows over 4099 positions of 9 sequences with 8 kv heads of 128 dims,
 // bf16: 50 us against 60; 16 rows: 47 against 40; 32 rows over 600 positions of 2 sequences: 14.0 against 11.9.
-// (f32 has one row tile and more products, and its rows pay later: 48 rows over the 4099 positions 110 against 84, 64 rows 112
-// against 105.)
+// (f32 has one row tile and more products, and its rows pay later: 48 rows over the 4099 positions 110 against 84,
+// 64 rows 112 against 105.)
 __host__ __device__ constexpr uint32_t tile_min(bool f32) { return f32 ? 64 : 24; }
 constexpr uint64_t kTileWork = 3;
 
@@ -766,7 +770,8 @@ __global__ void __launch_bounds__(32 * (5 * role_of(HD, sizeof(T) == 4).rt + 5),
     constexpr uint32_t FG = 8, FS = 2 * FG;  // steps of block factors handed over together, and kept
     __shared__ __align__(8) uint64_t k_full[ST], k_empty[ST], v_full[ST], v_empty[ST], f_full[2], f_empty[2], c_full[RAW], c_empty[RAW];
     __shared__ __align__(8) uint64_t s_full[RT][4], p_full[RT][4], o_done[RT][4], q_full, fin[RT];
-    __shared__ float4 f_blk[FS][NB];  // key scale, log2 of the value scale (f32: 0; -infinity: no such page, infinity: a rare one), its inverse, itself
+    // key scale, log2 of the value scale (f32: 0; -infinity: no such page, infinity: a rare one), its inverse, itself
+    __shared__ float4 f_blk[FS][NB];
     __shared__ uint32_t tmem_base;
     __shared__ volatile int abort_flag;
     const Kv8AttnArgs& a = P.a;
@@ -1321,8 +1326,9 @@ Shape shape_of(const Kv8Cache& c, const Kv8Batch& b, uint32_t heads, uint32_t ty
     r.tile_rows = r.tiles ? role.rt * kTileRows : kRows;
     r.row_tiles = (uint32_t)((rows + r.tile_rows - 1) / r.tile_rows);
     // chunks of positions: enough CTAs for three on every SM (the prompt kernel: one; one row tile of 256
-    // dims: two, as many as run at once -- 32768 positions over 4 kv heads 25 us against 34 with three;
-    // several row tiles read the same pages, and three measured better: 29 against 37), each with at
+    // dims: two, as many as run at once -- 32768 positions over 4 kv heads 27 us against 37 with three;
+    // several row tiles read the same pages, and three measured better: 2 tokens over 4099 positions of 9 sequences 21
+    // against 26, though 4 over 32768 of one 49 against 37), each with at
     // least 8 blocks (two per warp, two steps of the prompt kernel). More chunks measured slower: a
     // CTA's fixed cost is about 4 us.
     const uint64_t tiles = (uint64_t)b.n_seqs * c.kv_heads * r.row_tiles;

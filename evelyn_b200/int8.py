@@ -112,7 +112,7 @@ def _check_err(err):
 
 def quantize_rows(x, codes, scales, stream: int = 0) -> None:
     """Rows of x [rows][cols] to codes [rows][cols] int8 and scales [rows] float32:
-    scale = max|x| / 127, code = round(x / scale) (evl_i8_quantize_rows)."""
+    scale = max|x| / 127, code = x * (1 / scale) rounded to nearest even (evl_i8_quantize_rows)."""
     key = ("rows", _layout(x, codes, scales))
     plan = _plans.get(key)
     if plan is None:

@@ -267,8 +267,8 @@ evl_status evl_attention_decode_noalloc(const float* d_q, const void* d_k_pages,
  * its first one (the calling thread's current device is left as it was) and is asynchronous
  * on `stream` (a stream of that device; NULL: its default stream), so it can be captured
  * into a graph. No call allocates device memory or keeps anything. `type` is the element
- * type of the activations: 0 F32, 1 F16, 30 BF16. Arithmetic is f32 (integer sums exact),
- * rounded once to the output type.
+ * type of the activations: 0 F32, 1 F16, 30 BF16. Arithmetic is f32 (integer sums exact; what
+ * attention holds its weights and sums in: see there), rounded once to the output type.
  * A group of values in 8 bits is codes c in [-127, 127] and one f32 scale s, value s * c:
  * s = max|x| / 127, c = x * (1 / s) rounded to nearest even. A group whose largest magnitude
  * is below 2^-100 has s = 0 and codes 0; one that holds an infinity or a NaN has s = NaN and
@@ -368,16 +368,19 @@ evl_status evl_kv8_attention_workspace_bytes(const evl_kv8_cache* cache, const e
  * head h / (heads / kv_heads). d_q and d_out [total][heads][head_dim] of `type`, tokens q_stride /
  * out_stride elements apart, 16-byte aligned, strides multiples of 16 bytes. heads a multiple of
  * kv_heads. scale 0: 1 / sqrt(head_dim). A row that sees no position gives zeros; a query row that
- * holds an infinity or a NaN gives NaN, and so does one that sees a block whose value scale is not finite, however
- * small its weights there. Scores are held in f32. In them each value of q is good to 2^-22 of its row's largest
- * magnitude (not of its own), so beside a loud channel of q a score may be off by that times sum |k|; the 16-bit
- * types with many rows hold q exactly to 2^-34 of the largest and sum the products in f32, cut off by up to 2^-23 of
- * the terms' sizes after every 16 dims. Scores beyond 1e38 in magnitude are good for nothing. Weights keep f32's range, and 24 bits (16-bit types:
- * 16) however far they lie below the largest; their sums over the positions are off by a bounded number of cut-off additions (f32: 96 of
- * at most 2^-23; 16-bit types: 1024) and otherwise rounded to nearest, whatever the length. Rows of d_out that belong to no sequence are left as they were. One kernel serves all
+ * holds an infinity or a NaN gives NaN, and so does one that sees a block whose value scale is not
+ * finite, however small its weights there. Scores are held in f32. In them each value of q is good
+ * to 2^-22 of its row's largest magnitude (not of its own), so beside a loud channel of q a score
+ * may be off by that times sum |k|; the 16-bit types with many rows hold q exactly to 2^-34 of
+ * the largest and sum the products in f32, cut off by up to 2^-23 of the terms' sizes after every
+ * 16 dims. Scores beyond 1e38 in magnitude are good for nothing. Weights keep f32's range, and 24
+ * bits (16-bit types: 16) however far they lie below the largest; their sums over the positions are
+ * off by a bounded number of cut-off additions (f32: 96 of at most 2^-23; 16-bit types: 1024) and
+ * otherwise rounded to nearest, whatever the length. Rows of d_out that belong to no sequence are
+ * left as they were. One kernel serves all
  * sequences of a call, chosen by max_new: a batch that mixes prompts with single tokens gives
- * the same sums but is faster as two calls. d_workspace: evl_kv8_attention_workspace_bytes, 256-byte aligned, needing no initial
- * value; calls that may overlap in time need one each. */
+ * the same sums but is faster as two calls. d_workspace: evl_kv8_attention_workspace_bytes, 256-byte
+ * aligned, needing no initial value; calls that may overlap in time need one each. */
 evl_status evl_kv8_attention(const evl_kv8_cache* cache, const evl_kv8_batch* batch, uint32_t type, const void* d_q,
                              uint64_t q_stride, uint32_t heads, float scale, void* d_out, uint64_t out_stride,
                              void* d_workspace, size_t workspace_bytes, int32_t* d_err, void* stream);
