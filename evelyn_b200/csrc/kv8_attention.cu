@@ -87,10 +87,10 @@ __device__ __forceinline__ float exp2_fast(float x) {
 // What the scores of a block are raised by where they ask for a new maximum: 0 for value scales from 2^-60 to 2^80 and
 // for scales that are 0 (or subnormal, which count as 0) or not finite.
 __device__ __forceinline__ float lift_of(float sv) {
-    const int e = (int)(__float_as_uint(sv) >> 23) - 127;
+    const int e = (int)(__float_as_uint(sv) >> 23 & 0xffu) - 127;
     return e == -127 || e == 128 ? 0.f : (float)(max(e - 80, 0) + min(e + 60, 0));
 }
-__device__ __forceinline__ float zero_if_subnormal(float sv) { return __float_as_uint(sv) < 0x00800000u ? 0.f : sv; }
+__device__ __forceinline__ float zero_if_subnormal(float sv) { return abs_bits(sv) < 0x00800000u ? 0.f : sv; }
 // bytes 0, 1 (or 2, 3) of w, biased codes c + 128, as an exact f16 pair: 0x6400 | b is 1024 + b
 __device__ __forceinline__ uint32_t codes_h2(uint32_t w, uint32_t sel) {
     const uint32_t h = __byte_perm(w, 0x64646464u, sel), bias = 0x64806480u;  // 1024 + 128

@@ -218,3 +218,59 @@ def test_attention_values_of_one_sign_over_many_positions(tokens, kind, dim, n):
     _put(kv, level[:, None] * sign, v, np.full(blocks, 1 / 40, np.float32), np.full(blocks, 1 / 40, np.float32))
     q = dev(np.tile(x, (tokens, 4, 1)).astype(np.float32), kind)
     _compare(kv, n, tokens, q, kind)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_attention_long_chunks_joined_captured_and_replayed(kind, dim, sign):
+    """Forty sequences over the same pages: chunks so long that their sums leave tensor memory, several of them joined.
+    Eager, captured and replayed twice over a workspace full of NaN: the same bits for all sequences."""
+    t = gu.torch()
+    rng = np.random.default_rng(dim)
+    n, tokens, seqs = 32773, 16, 40
+    kv = Kv(rng, 1, dim, 64, [n])
+    signs, level, x = _levels(rng, n, dim, 3, 60, 128)
+    v = rng.integers(32, 128, (n, dim)) * sign
+    blocks = -(-n // 16)
+    _put(kv, level[:, None] * signs, v, np.full(blocks, 1 / 40, np.float32), rng.uniform(0.5, 1.5, blocks).astype(np.float32) / 40)
+    one = np.tile(x, (tokens, 4, 1)) * rng.uniform(0.3, 1, (tokens, 4, 1))
+    q = dev(np.tile(one, (seqs, 1, 1)).astype(np.float32), kind)
+    b = int8.Kv8Batch(dev(np.tile(kv.table, (seqs, 1))), dev(np.arange(seqs + 1, dtype=np.int32) * tokens),
+                      dev(np.full(seqs, n, np.int32)), tokens, n)
+    out = t.full(q.shape, 7.0, dtype=q.dtype, device="cuda:0")
+    ws = t.full((int8.kv8_attention_workspace(kv.cache, b, q),), 255, dtype=t.uint8, device="cuda:0")
+    int8.kv8_attention(kv.cache, b, q, out, workspace=ws, err=kv.err)
+    got = host(out)
+    k, w = (ref.values(a, s, kv.table[0], n)[:, 0] for a, s in ((kv.k, kv.ks), (kv.v, kv.vs)))
+    want, tol = _bound(host(q)[:tokens], k, w, n - tokens, 1 / np.sqrt(dim), kind)
+    assert int(kv.err) == 0 and (np.abs(got[:tokens] - want) / tol).max() <= 1
+    got = got.reshape(seqs, tokens, 4, dim)
+    assert np.array_equal(got, np.broadcast_to(got[:1], got.shape))
+    side, g = t.cuda.Stream(), t.cuda.CUDAGraph()
+    t.cuda.synchronize()
+    with t.cuda.graph(g, stream=side):
+        int8.kv8_attention(kv.cache, b, q, out, workspace=ws, err=kv.err, stream=side.cuda_stream)
+    for _ in range(2):
+        out.fill_(7.0)
+        ws.fill_(255)
+        g.replay()
+        gu.sync()
+        assert np.array_equal(host(out).reshape(got.shape), got)
+
+
+@KERNELS
+@pytest.mark.parametrize("kind", KINDS)
+def test_attention_scales_of_minus_zero(tokens, kind):
+    """A value scale of -0 is a scale of 0: its positions count in the weights and add nothing, here nearly all of them."""
+    _wide(tokens)
+    rng = np.random.default_rng(3)
+    n, dim = 100, 128
+    kv = Kv(rng, 1, dim, 16, [n])
+    sign, level, x = _levels(rng, n, dim, 60, 60, 67)
+    level[20] = 127
+    vs = np.full(7, 1 / 40, np.float32)
+    vs[1] = -0.0
+    _put(kv, level[:, None] * sign, rng.integers(-127, 128, (n, dim)), np.full(7, 1 / 40, np.float32), vs)
+    q = dev(np.tile(x, (tokens, 4, 1)).astype(np.float32), kind)
+    _compare(kv, n, tokens, q, kind)
