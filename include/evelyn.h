@@ -289,7 +289,8 @@ evl_status evl_i8_quantize_rows(uint32_t type, const void* d_x, uint64_t x_strid
  * x [rows][cols] and w [out][cols] int8 with rows x_stride / w_stride bytes apart (multiples
  * of 16, the buffers 16-byte aligned; what lies between cols and the stride is not read into
  * the sums); d_add (optional) and d_y of `type`, rows add_stride / y_stride elements apart.
- * d_add may be d_y (a residual added in place) but no other overlap with d_y is allowed.
+ * d_add may be d_y (a residual added in place) but no other overlap with d_y is allowed (it is
+ * refused where both have one stride or there is one row).
  * cols from 1 to 131071 (the int32 sums then cannot overflow); rows or out may be 0. */
 evl_status evl_i8_matmul(const int8_t* d_x, uint64_t x_stride, const float* d_x_scales, uint32_t rows,
                          const int8_t* d_w, uint64_t w_stride, const float* d_w_scales, uint32_t out, uint32_t cols,
